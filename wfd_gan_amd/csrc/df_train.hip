@@ -53,11 +53,16 @@ __global__ void bn_tall_partial_kernel(const float* __restrict__ Z, int ldz, int
 // association, so the result is deterministic.  mean, invstd = 1/sqrt(M2/M + eps); running stats with the unbiased
 // variance, as nn.BatchNorm1d does in training mode.
 constexpr int CG = 16;
-__device__ __forceinline__ void chan_fold(float& mu, float& m2, float& cnt, float mb, float qb, float cb) {
+// The roundings are spelled out (contraction off; `fused`: one rounding for the product and its sum), so that the result does
+// not hang on what the compiler fuses: these are the bits that checkpoints trained with earlier builds were made with.
+__device__ __forceinline__ void chan_fold(float& mu, float& m2, float& cnt, float mb, float qb, float cb, bool fused) {
+#pragma clang fp contract(off)
     if (cb <= 0.f) return;
     const float tot = cnt + cb, delta = mb - mu;
+    const float w = cnt * cb / tot, d2 = delta * delta;
+    const float t = fused ? fmaf(d2, w, qb) : qb + d2 * w;
     mu += delta * (cb / tot);
-    m2 += qb + delta * delta * (cnt * cb / tot);
+    m2 += t;
     cnt = tot;
 }
 __global__ void bn_tall_combine_kernel(const float* __restrict__ part, int nchunk, int rows_per_chunk, int M, int N,
@@ -80,15 +85,18 @@ __global__ void bn_tall_combine_kernel(const float* __restrict__ part, int nchun
                 cb[k] = in ? (float)min(rows_per_chunk, M - c * rows_per_chunk) : 0.f;
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) chan_fold(mu, m2, cnt, mb[k], qb[k], cb[k]);
+            for (int k = 0; k < 8; ++k) chan_fold(mu, m2, cnt, mb[k], qb[k], cb[k], true);
         }
     sh[0][g][threadIdx.x] = mu; sh[1][g][threadIdx.x] = m2; sh[2][g][threadIdx.x] = cnt;
     __syncthreads();
     if (!ok || g != 0) return;
-    for (int k = 1; k < CG; ++k) chan_fold(mu, m2, cnt, sh[0][k][threadIdx.x], sh[1][k][threadIdx.x], sh[2][k][threadIdx.x]);
+#pragma unroll
+    for (int k = 1; k < CG; ++k)
+        chan_fold(mu, m2, cnt, sh[0][k][threadIdx.x], sh[1][k][threadIdx.x], sh[2][k][threadIdx.x], k == 4 || k == 10);
     mean[n] = mu;
     invstd[n] = 1.0f / sqrtf(m2 / (float)M + eps);
     if (rmean) {
+#pragma clang fp contract(off)
         rmean[n] = (1.f - momentum) * rmean[n] + momentum * mu;
         rvar[n] = (1.f - momentum) * rvar[n] + momentum * (m2 / ((float)M - 1.f));
     }
@@ -255,6 +263,7 @@ __global__ void adamax_kernel(float* __restrict__ p, const float* __restrict__ g
     const float t = (float)(step[0] + 1);
     const float clr = lr / (1.f - powf(b1, t));
     for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) {
+#pragma clang fp contract(off)      // every operation rounded on its own
         const float gg = g[i];
         const float mm = b1 * m[i] + (1.f - b1) * gg;
         const float uu = fmaxf(b2 * u[i], fabsf(gg) + eps);
