@@ -488,6 +488,56 @@ int wfd_adamax(float* p, const float* g, float* m, float* u, long n, float lr, f
 /* correct[0] += #{rows whose first-maximum logit index equals the label} (src/train_df.py:141-143,153-155) */
 int wfd_argmax_correct(const float* logits, int ldl, int M, int C, const int* labels, int* correct, void* stream);
 
+/* ---- classifier head: layer norm, scores of given labels, a student's loss from a teacher's top logits --------------------
+ * NO COUNTERPART IN THE REFERENCE; they stand beside its nn.BatchNorm1d (src/model.py:23), nn.CrossEntropyLoss and argmax
+ * accuracy (src/train_df.py:111-157) and take rows of fp32, bf16 or fp16: `dtype` 0 fp32, 1 bf16, 2 fp16, leading dimensions
+ * in elements, any alignment the type itself has.  Sums, statistics and losses are fp32 whatever the rows' type.  M = 0 is a
+ * call with nothing to do.  Rows need no padding, and nothing behind a row's last element is read or written.
+ * `work` (fp32, as many floats as the matching _floats function says, none = may be NULL) is scratch of one call in flight:
+ * calls that may overlap -- other streams, graphs that replay side by side -- each need their own.  Every result is
+ * deterministic: no atomics order a sum. */
+
+/* nn.LayerNorm over the last dimension: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), N <= 2^24.
+ * weight / bias may be NULL (1 / 0) and are of `wdtype` = dtype or 0 (fp32).  mean / rstd [M] may be NULL (inference).
+ * Y may be X. */
+int wfd_layer_norm_fwd(const void* X, int ldx, int dtype, const void* weight, const void* bias, int wdtype, int M, int N,
+                       float eps, void* Y, int ldy, float* mean, float* rstd, void* stream);
+/* its backward from the saved mean / rstd: dx, and dweight / dbias [N] of `wdtype` (either may be NULL) summed over the rows in
+ * a fixed order.  DX may be DY or X.  M = 0 stores zeros to dweight / dbias. */
+int wfd_layer_norm_bwd(const void* DY, int lddy, const void* X, int ldx, int dtype, const void* weight, int wdtype,
+                       const float* mean, const float* rstd, int M, int N, void* DX, int lddx, void* dweight, void* dbias,
+                       float* work, void* stream);
+int wfd_layer_norm_bwd_floats(int M, int N, int dtype);
+
+/* Scores over V classes (V <= 2^28) at a temperature > 0, p = softmax(x / T), in one pass over the logits:
+ *   logprob[m] = ln p(labels[m]); a label < 0 is none (0), a label >= V a mistake (NaN)
+ *   entropy[m] = -sum p ln p
+ *   top_logprob / top_index [M][k]: the k (0 .. 64, <= V) largest logits in order, equal ones by lower index, NaN before all
+ *   stat[m] = {max x, ln sum exp((x - max) / T)}, what the backward needs: their (scaled) sum is the log-sum-exp
+ * logprob, entropy and stat may be NULL.  A row of nothing but -inf (everything masked): logprob and top_logprob -inf, entropy 0,
+ * stat {-inf, 0}.  A row with NaN or +inf: NaN. */
+int wfd_label_scores(const void* logits, int ldl, int dtype, int M, int V, const int* labels, float temperature, int k,
+                     float* logprob, float* entropy, float* stat, float* top_logprob, int* top_index, float* work,
+                     void* stream);
+int wfd_label_scores_floats(int M, int V, int dtype, int k);
+/* dlogits = the gradient of sum_m d_logprob[m] * logprob[m] + d_entropy[m] * entropy[m]; either may be NULL (0).  stat and
+ * entropy are wfd_label_scores' at the same temperature.  A row of nothing but -inf has gradient 0.  dlogits may be logits. */
+int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, const int* labels, float temperature,
+                         const float* stat, const float* entropy, const float* d_logprob, const float* d_entropy,
+                         void* dlogits, int lddl, void* stream);
+
+/* Distillation from a teacher's K (0 .. 256) top logits, with a label mixed in.  q = softmax(t_value / T) over the entries of a
+ * row of t_index / t_value [M][ldt] whose index is >= 0, p = softmax(x / T), p1 = softmax(x):
+ *   loss[m] = weight * T^2 * sum_j q_j (ln q_j - ln p(index_j)) - label_weight * ln p1(labels[m])
+ * and, when dlogits is not NULL, its gradient times grad_scale * row_scale[m] (row_scale NULL: 1) in the same call.  An index
+ * that occurs twice counts twice.  No entry: the first term is 0; a label < 0: the second is 0 (labels may be NULL when
+ * label_weight is 0).  An index or a label >= V is a mistake: the row's loss and gradient are NaN.  A row of nothing but -inf:
+ * loss +inf where a term is left, gradient 0.  dlogits may be logits. */
+int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int* t_index, const float* t_value, int ldt, int K,
+                const int* labels, float temperature, float weight, float label_weight, const float* row_scale,
+                float grad_scale, float* loss, void* dlogits, int lddl, float* work, void* stream);
+int wfd_distill_floats(int M, int V, int dtype);
+
 /* ---- peer-to-peer ("mesh") gradient exchange over xGMI (SURVEY section 8 e) ------------------------------------------------
  * NO COUNTERPART IN THE REFERENCE (src/mlp_df_wgan_train.py:98-100 picks one device); it replaces what a DistributedDataParallel
  * wrapper's all-reduce + src/mlp_df_wgan_train.py:230,275 (optimizer.step()) would do.  One process per GPU.  Every rank

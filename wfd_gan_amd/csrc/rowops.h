@@ -1,0 +1,163 @@
+// Row-wise building blocks of the classifier-head kernels (layernorm.hip, scores.hip, distill.hip): 16-byte pieces of rows in
+// fp32 / bf16 / fp16, held packed in registers, and reductions over the G threads ("team") that share a row.
+#pragma once
+#include "common.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+#define WFD_F32 0
+#define WFD_BF16 1
+#define WFD_F16 2
+
+static inline bool wfd_dtype_ok(int t) { return t >= WFD_F32 && t <= WFD_F16; }
+
+template <class T> struct Pack { static constexpr int N = 16 / (int)sizeof(T); };   // elements of one 16-byte piece
+
+// Rows begin wherever their stride puts them (an odd width of 16-bit values leaves every second row off even a 4-byte border):
+// gfx950 serves 16-byte accesses at any address, so pieces are counted from the row's first element, unaligned, and only the
+// last, partial one is taken element by element.
+struct __attribute__((packed, aligned(2))) Raw16u { unsigned v[4]; };
+struct Raw16 { unsigned v[4]; };
+
+template <class T> __device__ __forceinline__ Raw16 load16(const T* p) {
+    Raw16u r = *reinterpret_cast<const Raw16u*>(p);
+    return Raw16{{r.v[0], r.v[1], r.v[2], r.v[3]}};
+}
+template <class T> __device__ __forceinline__ void store16(T* p, const Raw16& r) {
+    *reinterpret_cast<Raw16u*>(p) = Raw16u{{r.v[0], r.v[1], r.v[2], r.v[3]}};
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16_t v) { return (float)v; }
+__device__ __forceinline__ float to_f32(f16_t v) { return (float)v; }
+template <class T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }    // round to nearest even
+
+// element e of a packed piece (e is a constant after unrolling)
+template <class T> __device__ __forceinline__ float elem(const Raw16& r, int e);
+template <> __device__ __forceinline__ float elem<float>(const Raw16& r, int e) { return __uint_as_float(r.v[e]); }
+template <> __device__ __forceinline__ float elem<bf16_t>(const Raw16& r, int e) {
+    return __uint_as_float((e & 1) ? (r.v[e >> 1] & 0xffff0000u) : (r.v[e >> 1] << 16));
+}
+template <> __device__ __forceinline__ float elem<f16_t>(const Raw16& r, int e) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    h2 h;
+    __builtin_memcpy(&h, &r.v[e >> 1], 4);
+    return (float)h[e & 1];
+}
+
+template <class T> __device__ __forceinline__ Raw16 pack(const float* f) {
+    Raw16 r;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.v[e] = __float_as_uint(f[e]);
+    } else {
+        typedef T t2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const t2 h = {(T)f[2 * e], (T)f[2 * e + 1]};
+            __builtin_memcpy(&r.v[e], &h, 4);
+        }
+    }
+    return r;
+}
+
+// the raw pattern of `fill` in every element
+template <class T> __device__ __forceinline__ unsigned raw_fill(float fill) {
+    float f[8] = {fill, fill, fill, fill, fill, fill, fill, fill};
+    return pack<T>(f).v[0];
+}
+
+// elements [i0, i0 + Pack<T>::N) of a row of n; those past the end read as `fill`
+template <class T> __device__ __forceinline__ Raw16 load_piece(const T* row, int i0, int n, float fill) {
+    constexpr int E = Pack<T>::N;
+    if (i0 + E <= n) return load16(row + i0);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = i0 + e < n ? to_f32(row[i0 + e]) : fill;
+    return pack<T>(f);
+}
+template <class T> __device__ __forceinline__ void store_piece(T* row, int i0, int n, const float* f) {
+    constexpr int E = Pack<T>::N;
+    if (i0 + E <= n) {
+        store16(row + i0, pack<T>(f));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (i0 + e < n) row[i0 + e] = from_f32<T>(f[e]);
+}
+
+// ---- reductions over the lanes of a wave: DPP inside 16 lanes (no LDS latency), two lane exchanges above ----------------
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lanes_sum16(float v) {
+    v += dpp<0xB1>(v);      // quad_perm 1,0,3,2
+    v += dpp<0x4E>(v);      // quad_perm 2,3,0,1
+    v += dpp<0x141>(v);     // row_half_mirror
+    v += dpp<0x140>(v);     // row_mirror
+    return v;
+}
+__device__ __forceinline__ float lanes_max16(float v) {
+    v = fmaxf(v, dpp<0xB1>(v));
+    v = fmaxf(v, dpp<0x4E>(v));
+    v = fmaxf(v, dpp<0x141>(v));
+    v = fmaxf(v, dpp<0x140>(v));
+    return v;
+}
+template <int G> __device__ __forceinline__ float lanes_sum(float v) {
+    v = lanes_sum16(v);
+    if constexpr (G >= 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (G >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+template <int G> __device__ __forceinline__ float lanes_max(float v) {
+    v = lanes_max16(v);
+    if constexpr (G >= 32) v = fmaxf(v, __shfl_xor(v, 16, 64));
+    if constexpr (G >= 64) v = fmaxf(v, __shfl_xor(v, 32, 64));
+    return v;
+}
+
+// Two sums over a team of G threads; G <= 64 stays inside the wave, above it the wave sums meet in `slot` (2 * G / 64 floats of
+// LDS that nothing else touches until the next barrier after this one) and are added in wave order by every thread.
+template <int G> __device__ __forceinline__ float2 team_sum2(float a, float b, float* slot) {
+    a = lanes_sum<(G < 64 ? G : 64)>(a);
+    b = lanes_sum<(G < 64 ? G : 64)>(b);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) { slot[2 * w] = a; slot[2 * w + 1] = b; }
+        __syncthreads();
+        a = 0.f; b = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) { a += slot[2 * i]; b += slot[2 * i + 1]; }
+    }
+    return make_float2(a, b);
+}
+template <int G> __device__ __forceinline__ float team_sum(float a, float* slot) {
+    a = lanes_sum<(G < 64 ? G : 64)>(a);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) slot[w] = a;
+        __syncthreads();
+        a = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) a += slot[i];
+    }
+    return a;
+}
+template <int G> __device__ __forceinline__ float team_max(float a, float* slot) {
+    a = lanes_max<(G < 64 ? G : 64)>(a);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) slot[w] = a;
+        __syncthreads();
+        a = slot[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) a = fmaxf(a, slot[i]);
+    }
+    return a;
+}

@@ -1,0 +1,359 @@
+"""Tensor-level entry points of the classifier-head kernels (include/wfdgan.h, "classifier head"): layer norm with its
+backward, the scores of given labels over many classes (log probability, entropy, top alternatives) with their gradient, and the
+loss of a student that learns from a teacher's top logits.
+
+Rows lie along the last dimension and may be float32, bfloat16 or float16; leading dimensions are free; rows with a stride are
+read where they are, anything else is copied first.  As everywhere in this package the backward is a call of its own in closed
+form (no autograd graph), there is no CPU path, and a call only enqueues work on the current stream of the tensors' device.
+
+Results go into fresh tensors, or into those of an earlier call's result passed as ``out=`` (same sizes): then a call allocates
+nothing, which is what a loop or a captured graph wants.  Such a result belongs to one call in flight: give calls that may
+overlap (other streams, graphs that replay side by side) results of their own.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from ._lib import lib
+
+MAX_ALTERNATIVES = 64
+MAX_TEACHER_ENTRIES = 256
+_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INT32 = 1 << 31
+
+
+class NormOutput(NamedTuple):
+    y: torch.Tensor
+    mean: Optional[torch.Tensor]          # fp32, one per row: what the backward needs
+    rstd: Optional[torch.Tensor]
+
+
+class NormGradients(NamedTuple):
+    dx: torch.Tensor
+    dweight: Optional[torch.Tensor]
+    dbias: Optional[torch.Tensor]
+    work: torch.Tensor
+
+
+class LabelScores(NamedTuple):
+    logprob: Optional[torch.Tensor]       # fp32, shape of the labels
+    entropy: Optional[torch.Tensor]
+    stat: Optional[torch.Tensor]          # fp32 (..., 2): row maximum, log of the sum of exponentials about it
+    top_logprob: Optional[torch.Tensor]   # fp32 (..., k)
+    top_index: Optional[torch.Tensor]     # int32 (..., k)
+    work: Optional[torch.Tensor]
+
+
+class DistillOutput(NamedTuple):
+    loss: torch.Tensor                    # fp32, one per row
+    dlogits: Optional[torch.Tensor]
+    work: Optional[torch.Tensor]
+
+
+# ---- argument checks -------------------------------------------------------------------------------------------------
+def _code(t: torch.Tensor, name: str) -> int:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
+    c = _CODES.get(t.dtype)
+    if c is None:
+        raise TypeError(f"{name}: float32, bfloat16 or float16 rows, got {t.dtype}")
+    return c
+
+
+def _rows(t: torch.Tensor, name: str):
+    """(tensor whose storage is read, rows, columns, row stride)"""
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise ValueError(f"{name}: needs a last dimension of at least one element, got shape {tuple(t.shape)}")
+    n = t.shape[-1]
+    m = t.numel() // n
+    if m >= _INT32 or n >= _INT32:
+        raise ValueError(f"{name}: {m} rows of {n} are more than 2^31 - 1")
+    if t.is_contiguous():
+        return t, m, n, n
+    if t.dim() == 2 and (t.stride(1) == 1 or n == 1) and n <= t.stride(0) < _INT32:
+        return t, m, n, t.stride(0)
+    return t.contiguous(), m, n, n
+
+
+def _same_device(dev: torch.device, who: str, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{who}: {name} is on {t.device}, the rows are on {dev}")
+    if dev.type != "cuda":
+        raise RuntimeError(f"{who}: these kernels run on the MI355X only (got a {dev} tensor); there is no CPU fallback")
+
+
+def _vector(t, who: str, name: str, numel: int, dtype) -> torch.Tensor:
+    """An optional per-row or per-column operand: its dtype and size checked, contiguous."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError(f"{who}: {name} must be a {dtype} tensor, got {getattr(t, 'dtype', type(t).__name__)}")
+    if t.numel() != numel:
+        raise ValueError(f"{who}: {name} has {t.numel()} elements, expected {numel}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _result(t, who: str, name: str, numel: int, dtype, dev):
+    """One tensor of an earlier result that is written again."""
+    if t is None or t.dtype != dtype or t.numel() != numel or t.device != dev or not t.is_contiguous():
+        got = None if t is None else (t.dtype, tuple(t.shape), t.device)
+        raise ValueError(f"{who}: out.{name} must be a contiguous {dtype} tensor of {numel} elements on {dev}, got {got}")
+    return t
+
+
+def _scratch(t, who: str, floats: int, dev):
+    if floats == 0:
+        return t
+    if t is None or t.dtype != torch.float32 or t.numel() < floats or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{who}: out.work must hold {floats} float32 on {dev} (take out from a call of these sizes)")
+    return t
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _launch(dev: torch.device, fn, *args):
+    if dev.index == torch.cuda.current_device():
+        fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        return
+    with torch.cuda.device(dev):
+        fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _temperature(t: float, who: str) -> float:
+    t = float(t)
+    if not 0.0 < t < float("inf"):
+        raise ValueError(f"{who}: temperature must be positive and finite, got {t}")
+    return t
+
+
+# ---- layer norm --------------------------------------------------------------------------------------------------------
+def _norm_weights(who, code, n, **w):
+    dtypes = {t.dtype for t in w.values() if t is not None}
+    if len(dtypes) > 1:
+        raise TypeError(f"{who}: weight and bias must have one dtype, got {sorted(map(str, dtypes))}")
+    wd = dtypes.pop() if dtypes else torch.float32
+    if wd != torch.float32 and _CODES.get(wd) != code:
+        raise TypeError(f"{who}: weight and bias must be float32 or have the rows' dtype, got {wd}")
+    return wd, [_vector(t, who, name, n, wd) for name, t in w.items()]
+
+
+def norm_output_like(x: torch.Tensor, stats: bool = True) -> NormOutput:
+    """Buffers for ``layer_norm(x, ..., out=...)``."""
+    f = dict(dtype=torch.float32, device=x.device)
+    lead = x.shape[:-1]
+    return NormOutput(torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(lead, **f) if stats else None,
+                      torch.empty(lead, **f) if stats else None)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               *, stats: bool = True, out: Optional[NormOutput] = None) -> NormOutput:
+    """``(x - mean) * rstd * weight + bias`` over the last dimension; mean and rstd are returned for the backward unless
+    ``stats`` is false.  ``out.y`` may be ``x``."""
+    who = "layer_norm"
+    code = _code(x, "x")
+    xr, m, n, ld = _rows(x, "x")
+    wd, (w, b) = _norm_weights(who, code, n, weight=weight, bias=bias)
+    if not float(eps) >= 0.0:
+        raise ValueError(f"{who}: eps must not be negative, got {eps}")
+    dev = x.device
+    _same_device(dev, who, weight=w, bias=b)
+    if out is None:
+        out = norm_output_like(x, stats)
+    else:
+        _result(out.y, who, "y", x.numel(), x.dtype, dev)
+        if stats:
+            _result(out.mean, who, "mean", m, torch.float32, dev)
+            _result(out.rstd, who, "rstd", m, torch.float32, dev)
+    _launch(dev, lib().layer_norm_fwd, xr.data_ptr(), ld, code, _ptr(w), _ptr(b), _CODES[wd], m, n, float(eps),
+            out.y.data_ptr(), n, _ptr(out.mean) if stats else 0, _ptr(out.rstd) if stats else 0)
+    return out
+
+
+def norm_gradients_like(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                        bias: Optional[torch.Tensor] = None) -> NormGradients:
+    """Buffers for ``layer_norm_backward(..., out=...)``; without a weight (bias) there is no dweight (dbias)."""
+    n = x.shape[-1]
+    floats = lib().layer_norm_bwd_floats(x.numel() // n, n, _code(x, "x"))
+    if floats < 0:
+        raise ValueError(f"layer_norm_backward: rows of {n} are not supported")
+    grad = lambda w: None if w is None else torch.empty(n, dtype=w.dtype, device=x.device)
+    return NormGradients(torch.empty(x.shape, dtype=x.dtype, device=x.device), grad(weight), grad(bias),
+                         torch.empty(floats, dtype=torch.float32, device=x.device))
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
+                        rstd: torch.Tensor, *, bias: bool = True, out: Optional[NormGradients] = None) -> NormGradients:
+    """Gradients of ``layer_norm`` from its saved mean and rstd: dx in the rows' dtype, dweight and dbias in the weight's (both
+    float32 without a weight, where dweight is None); sums over the rows are fp32 in a fixed order.  ``out.dx`` may be ``dy`` or
+    ``x``."""
+    who = "layer_norm_backward"
+    code = _code(x, "x")
+    if _code(dy, "dy") != code or dy.shape != x.shape:
+        raise ValueError(f"{who}: dy {dy.dtype} {tuple(dy.shape)} does not match x {x.dtype} {tuple(x.shape)}")
+    xr, m, n, ldx = _rows(x, "x")
+    dyr, _, _, lddy = _rows(dy, "dy")
+    wd, (w,) = _norm_weights(who, code, n, weight=weight)
+    if mean is None or rstd is None:
+        raise ValueError(f"{who}: needs the mean and rstd that layer_norm returned")
+    mean, rstd = _vector(mean, who, "mean", m, torch.float32), _vector(rstd, who, "rstd", m, torch.float32)
+    dev = x.device
+    _same_device(dev, who, dy=dy, weight=w, mean=mean, rstd=rstd)
+    if out is None:
+        like = torch.empty(0, dtype=wd, device=dev)
+        out = norm_gradients_like(x, w, like if bias else None)
+    else:
+        _result(out.dx, who, "dx", x.numel(), x.dtype, dev)
+        for name, t in (("dweight", out.dweight), ("dbias", out.dbias)):
+            if t is not None:
+                _result(t, who, name, n, wd, dev)
+        _scratch(out.work, who, lib().layer_norm_bwd_floats(m, n, code), dev)
+    _launch(dev, lib().layer_norm_bwd, dyr.data_ptr(), lddy, xr.data_ptr(), ldx, code, _ptr(w), _CODES[wd], mean.data_ptr(),
+            rstd.data_ptr(), m, n, out.dx.data_ptr(), n, _ptr(out.dweight), _ptr(out.dbias), out.work.data_ptr())
+    return out
+
+
+# ---- scores of given labels ------------------------------------------------------------------------------------------
+def scores_like(logits: torch.Tensor, k: int = 0) -> LabelScores:
+    """Buffers for ``label_logprobs(logits, ..., k, out=...)``."""
+    v = logits.shape[-1]
+    floats = lib().label_scores_floats(logits.numel() // v, v, _code(logits, "logits"), k)
+    if floats < 0:
+        raise ValueError(f"label_logprobs: {k} alternatives of {v} classes are not supported (at most {MAX_ALTERNATIVES})")
+    lead, dev = logits.shape[:-1], logits.device
+    f = dict(dtype=torch.float32, device=dev)
+    return LabelScores(torch.empty(lead, **f), torch.empty(lead, **f), torch.empty(*lead, 2, **f),
+                       torch.empty(*lead, k, **f) if k else None,
+                       torch.empty(*lead, k, dtype=torch.int32, device=dev) if k else None,
+                       torch.empty(floats, **f) if floats else None)
+
+
+def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int = 0, *, temperature: float = 1.0,
+                   out: Optional[LabelScores] = None) -> LabelScores:
+    """Log probability of each row's label under softmax(logits / temperature), the entropy of that distribution and its ``k``
+    largest classes in order (equal logits: the lower index first), all in one pass over the logits.
+
+    ``labels``: int32, one per row; negative = no label (log probability 0), >= classes = NaN; None: ``logprob`` is left
+    unwritten.  A row of nothing but -inf has log probabilities -inf and entropy 0; one with NaN or +inf is NaN."""
+    who = "label_logprobs"
+    code = _code(logits, "logits")
+    xr, m, v, ld = _rows(logits, "logits")
+    k = int(k)
+    if not 0 <= k <= min(v, MAX_ALTERNATIVES):
+        raise ValueError(f"{who}: k must be 0 .. {min(v, MAX_ALTERNATIVES)}, got {k}")
+    y = _vector(labels, who, "labels", m, torch.int32)
+    temperature = _temperature(temperature, who)
+    dev = logits.device
+    _same_device(dev, who, labels=y)
+    if out is None:
+        out = scores_like(logits, k)
+        if y is None:
+            out = out._replace(logprob=None)
+    else:
+        if y is not None:
+            _result(out.logprob, who, "logprob", m, torch.float32, dev)
+        if out.entropy is not None:
+            _result(out.entropy, who, "entropy", m, torch.float32, dev)
+        if out.stat is not None:
+            _result(out.stat, who, "stat", 2 * m, torch.float32, dev)
+        if k:
+            _result(out.top_logprob, who, "top_logprob", m * k, torch.float32, dev)
+            _result(out.top_index, who, "top_index", m * k, torch.int32, dev)
+        _scratch(out.work, who, lib().label_scores_floats(m, v, code, k), dev)
+    _launch(dev, lib().label_scores, xr.data_ptr(), ld, code, m, v, _ptr(y), temperature, k, _ptr(out.logprob) if y is not None else 0,
+            _ptr(out.entropy), _ptr(out.stat), _ptr(out.top_logprob) if k else 0, _ptr(out.top_index) if k else 0, _ptr(out.work))
+    return out
+
+
+def label_logprobs_backward(logits: torch.Tensor, labels: Optional[torch.Tensor], scores: LabelScores,
+                            d_logprob: Optional[torch.Tensor], d_entropy: Optional[torch.Tensor] = None, *,
+                            temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``(d_logprob * logprob + d_entropy * entropy).sum()`` with respect to the logits.  ``scores`` is what
+    ``label_logprobs`` returned for these logits at this temperature (its stat and, with ``d_entropy``, its entropy are read).
+    ``out`` may be ``logits`` itself."""
+    who = "label_logprobs_backward"
+    code = _code(logits, "logits")
+    xr, m, v, ld = _rows(logits, "logits")
+    y = _vector(labels, who, "labels", m, torch.int32)
+    if d_logprob is not None and y is None:
+        raise ValueError(f"{who}: d_logprob needs the labels")
+    if scores.stat is None or (d_entropy is not None and scores.entropy is None):
+        raise ValueError(f"{who}: scores lacks the stat or entropy that label_logprobs returned")
+    stat = _vector(scores.stat, who, "scores.stat", 2 * m, torch.float32)
+    ent = _vector(scores.entropy, who, "scores.entropy", m, torch.float32) if d_entropy is not None else None
+    dl, dh = _vector(d_logprob, who, "d_logprob", m, torch.float32), _vector(d_entropy, who, "d_entropy", m, torch.float32)
+    temperature = _temperature(temperature, who)
+    dev = logits.device
+    _same_device(dev, who, labels=y, stat=stat, entropy=ent, d_logprob=dl, d_entropy=dh)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    elif out is not logits or not logits.is_contiguous():
+        _result(out, who, "dlogits", logits.numel(), logits.dtype, dev)
+    _launch(dev, lib().label_scores_bwd, xr.data_ptr(), ld, code, m, v, _ptr(y), temperature, stat.data_ptr(), _ptr(ent),
+            _ptr(dl), _ptr(dh), out.data_ptr(), v)
+    return out
+
+
+# ---- distillation ------------------------------------------------------------------------------------------------------
+def distill_output_like(logits: torch.Tensor, grad: bool = True) -> DistillOutput:
+    """Buffers for ``distill_loss(logits, ..., out=...)``."""
+    v = logits.shape[-1]
+    floats = lib().distill_floats(logits.numel() // v, v, _code(logits, "logits"))
+    if floats < 0:
+        raise ValueError(f"distill_loss: {v} classes are not supported")
+    f = dict(dtype=torch.float32, device=logits.device)
+    return DistillOutput(torch.empty(logits.shape[:-1], **f),
+                         torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None,
+                         torch.empty(floats, **f) if floats else None)
+
+
+def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_value: torch.Tensor,
+                 labels: Optional[torch.Tensor] = None, *, temperature: float = 1.0, weight: float = 1.0,
+                 label_weight: float = 0.0, row_scale: Optional[torch.Tensor] = None, grad_scale: float = 1.0, grad: bool = True,
+                 out: Optional[DistillOutput] = None) -> DistillOutput:
+    """Per-row loss of a student against a teacher's top logits, and its gradient in the same call:
+
+        weight * T^2 * KL(softmax(teacher_value / T) || softmax(logits / T) at teacher_index) - label_weight * ln softmax(logits)[label]
+
+    ``teacher_index`` (int32) and ``teacher_value`` (float32: logits or log probabilities, their offset does not matter) are
+    (..., K) with K <= 256; an index < 0 is no entry, an index that occurs twice counts twice.  ``labels`` (int32) are needed
+    when ``label_weight`` is not 0; negative = no label.  ``dlogits`` carries ``grad_scale * row_scale`` (the losses do not).
+    An index or label >= classes makes its row NaN.  ``out.dlogits`` may be ``logits``."""
+    who = "distill_loss"
+    code = _code(logits, "logits")
+    xr, m, v, ld = _rows(logits, "logits")
+    for name, t, dt in (("teacher_index", teacher_index, torch.int32), ("teacher_value", teacher_value, torch.float32)):
+        if not isinstance(t, torch.Tensor) or t.dtype != dt:
+            raise TypeError(f"{who}: {name} must be a {dt} tensor, got {getattr(t, 'dtype', type(t).__name__)}")
+        if t.dim() == 0 or t.shape[:-1] != logits.shape[:-1] or t.shape != teacher_index.shape:
+            raise ValueError(f"{who}: {name} {tuple(t.shape)} does not go with logits {tuple(logits.shape)}")
+    k = teacher_index.shape[-1]
+    if k > MAX_TEACHER_ENTRIES:
+        raise ValueError(f"{who}: at most {MAX_TEACHER_ENTRIES} entries of the teacher per row, got {k}")
+    ti, tv = teacher_index.contiguous(), teacher_value.contiguous()
+    y = _vector(labels, who, "labels", m, torch.int32)
+    label_weight, weight, grad_scale = float(label_weight), float(weight), float(grad_scale)
+    for name, f in (("weight", weight), ("label_weight", label_weight)):
+        if not f - f == 0.0:
+            raise ValueError(f"{who}: {name} must be finite, got {f}")
+    if label_weight != 0.0 and y is None:
+        raise ValueError(f"{who}: label_weight needs labels")
+    rs = _vector(row_scale, who, "row_scale", m, torch.float32)
+    temperature = _temperature(temperature, who)
+    dev = logits.device
+    _same_device(dev, who, teacher_index=ti, teacher_value=tv, labels=y, row_scale=rs)
+    if out is None:
+        out = distill_output_like(logits, grad)
+    else:
+        _result(out.loss, who, "loss", m, torch.float32, dev)
+        if grad:
+            _result(out.dlogits, who, "dlogits", logits.numel(), logits.dtype, dev)
+        _scratch(out.work, who, lib().distill_floats(m, v, code), dev)
+    _launch(dev, lib().distill, xr.data_ptr(), ld, code, m, v, _ptr(ti) if k else 0, _ptr(tv) if k else 0, k, k, _ptr(y),
+            temperature, weight, label_weight, _ptr(rs), grad_scale, out.loss.data_ptr(), _ptr(out.dlogits) if grad else 0, v,
+            _ptr(out.work))
+    return out
