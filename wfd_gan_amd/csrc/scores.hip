@@ -8,6 +8,8 @@
 
 namespace {
 
+__device__ __forceinline__ int cdiv_dev(int a, int b) { return (a + b - 1) / b; }
+
 struct Scores {
     const void* X;
     const int* labels;
@@ -16,8 +18,10 @@ struct Scores {
     float* stat;
     float* top_lp;
     int* top_idx;
+    float* work;          // [M][splits][3 + 2 k]: a part's statistics, its alternatives' values and indices
     int ld, M, V, k;
     float inv_t;
+    int splits, chunk;    // parts of a row and their length (a multiple of a step)
 };
 struct ScoresBwd {
     const void* X;
@@ -29,6 +33,7 @@ struct ScoresBwd {
     void* DX;
     int ld, lddx, M, V;
     float inv_t;
+    int chunks;           // workgroups (long rows) or pieces (short rows) per row
 };
 
 // order of alternatives: larger value first (NaN before every number, -0 as 0), then the lower index
@@ -41,87 +46,515 @@ __device__ __forceinline__ unsigned long long order_key(float v, int i) {
     return ((unsigned long long)order_bits(v) << 32) | (unsigned)~i;
 }
 
-__device__ __forceinline__ unsigned long long block_max_key(unsigned long long v, unsigned long long* slot) {
+// ---- what one workgroup knows of its part of a row -----------------------------------------------------------------------
+// Running statistics: m = max(largest so far, -FLT_MAX), s = sum exp2((x - m) c), u = sum exp2((x - m) c) (x - m) c with
+// c = log2(e) / T.  The floor under m keeps x - m defined for rows of -inf (their s stays 0, which is how they are told) and for
+// rows at the type's lowest value (x - m = 0).  exp2 of -inf is 0, and u takes no exponent below FAINT, so masked classes add
+// nothing; NaN and +inf reach s as NaN.
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOWEST = -3.402823466e38f;
+constexpr float FAINT = -1e4f;            // an exponent whose exponential is 0: stands in where 0 * -inf would be NaN
+
+struct Stat {
+    float m, s, u;
+};
+__device__ __forceinline__ void stat_to(Stat& a, float m, float c) {          // moves a to a maximum m >= a.m
+    const float d = fmaxf(a.m - m, -1e30f) * c, w = __builtin_amdgcn_exp2f(d);
+    a.u = w * fmaf(a.s, d, a.u);
+    a.s *= w;
+    a.m = m;
+}
+template <int N> __device__ __forceinline__ void stat_add(Stat& a, const float (&f)[N], float top, float c) {
+    if (top > a.m) stat_to(a, top, c);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float d = (f[e] - a.m) * c, w = __builtin_amdgcn_exp2f(d);
+        a.s += w;
+        a.u = fmaf(w, fmaxf(d, FAINT), a.u);
+    }
+}
+// over a team of G threads; slot: 3 * G / 64 floats of LDS.  Every thread gets the sum, added in a fixed order.
+template <int G> __device__ __forceinline__ Stat stat_team(Stat a, float c, float* slot) {
+    const float m = lanes_max<(G < 64 ? G : 64)>(a.m);
+    stat_to(a, m, c);
+    a.s = lanes_sum<(G < 64 ? G : 64)>(a.s);
+    a.u = lanes_sum<(G < 64 ? G : 64)>(a.u);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) { slot[3 * w] = a.m; slot[3 * w + 1] = a.s; slot[3 * w + 2] = a.u; }
+        __syncthreads();
+        float top = slot[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) top = fmaxf(top, slot[3 * i]);
+        Stat r{top, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            Stat b{slot[3 * i], slot[3 * i + 1], slot[3 * i + 2]};
+            stat_to(b, top, c);
+            r.s += b.s;
+            r.u += b.u;
+        }
+        a = r;
+    }
+    return a;
+}
+
+// what the statistics of a whole row say; `empty`: nothing but -inf
+struct RowEnd {
+    float m, log_s, entropy;
+    bool empty;
+};
+__device__ __forceinline__ RowEnd row_end(const Stat& a) {
+    RowEnd r;
+    r.empty = a.s == 0.f;
+    const float l2 = __log2f(a.s);
+    r.m = r.empty ? -INFINITY : a.m;
+    r.log_s = r.empty ? 0.f : LN2 * l2;
+    r.entropy = r.empty ? 0.f : LN2 * (l2 - a.u / a.s);
+    return r;
+}
+__device__ __forceinline__ float row_lp(const RowEnd& r, float x, float inv_t) {
+    return r.empty ? -INFINITY : (x - r.m) * inv_t - r.log_s;
+}
+__device__ __forceinline__ void row_store(const Scores& g, long row, const RowEnd& r, float xy, int y) {
+    if (g.stat) { g.stat[2 * row] = r.m; g.stat[2 * row + 1] = r.log_s; }
+    if (g.entropy) g.entropy[row] = r.entropy;
+    if (g.logprob) g.logprob[row] = y < 0 ? 0.f : y >= g.V ? NAN : row_lp(r, xy, g.inv_t);
+}
+
+// ---- alternatives of a part of a row --------------------------------------------------------------------------------------
+// Every thread has left the largest value of each group of pieces that it visited in LDS.  The (k / waves)-th largest thread
+// maximum of a wave, the smallest such of all waves, is a value that at least k elements reach (tau).  Only groups whose maximum
+// reaches tau are read again; what reaches tau there goes to a list (expected length: k and a few), whose order is found by
+// counting.  When more elements than the list holds reach tau, they are ties at tau but for a few: those above tau are listed and the
+// rest is filled up by walking the ties in index order.  Rows with NaN, and rows that defeat even this (thousands above
+// tau), take the k largest one after another.
+constexpr int CAND = 1024;
+constexpr int U = 4;                      // pieces per group
+
+template <int NT> struct PickLds {
+    unsigned long long key[CAND];
+    unsigned long long best[NT / 64 ? NT / 64 : 1];
+    float tau[NT / 64 ? NT / 64 : 1];
+    int count, run[NT / 64 ? NT / 64 : 1];
+};
+
+template <int NT> __device__ __forceinline__ void team_sync() {
+    if constexpr (NT > 64) __syncthreads();
+    else __builtin_amdgcn_wave_barrier(), __threadfence_block();
+}
+template <int NT> __device__ __forceinline__ unsigned long long team_max_key(unsigned long long v, unsigned long long* slot) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         const unsigned long long w = __shfl_xor(v, o, 64);
         v = w > v ? w : v;
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = slot[0];
-    for (int i = 1; i < 4; ++i) v = slot[i] > v ? slot[i] : v;
+    if constexpr (NT > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = slot[0];
+        for (int i = 1; i < NT / 64; ++i) v = slot[i] > v ? slot[i] : v;
+    }
     return v;
 }
 
-template <class T> __global__ __launch_bounds__(256) void scores_kernel(Scores g) {
-    __shared__ float slot[3][8];
-    __shared__ unsigned long long kslot[4];
-    const long row = blockIdx.x;
-    const T* x = (const T*)g.X + row * g.ld;
-    const int t = threadIdx.x, V = g.V;
-    float m = -INFINITY;
-    for (int i = t; i < V; i += 256) m = fmaxf(m, to_f32(x[i]));
-    m = team_max<256>(m, slot[0]);
-    float s = 0.f, u = 0.f;
-    for (int i = t; i < V; i += 256) {
-        const float z = (to_f32(x[i]) - m) * g.inv_t, e = __expf(z);
-        s += e;
-        if (e != 0.f) u = fmaf(z, e, u);
+// the n-th largest (n >= 1) of the 64 lanes' values (no NaN): how many lanes are above each lane's value
+__device__ __forceinline__ float lanes_nth(float v, int n) {
+    int above = 0, same = 0;
+    const int me = threadIdx.x & 63;
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) {
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+        above += w > v;
+        same += (w == v) & (i < me);
     }
-    const float2 su = team_sum2<256>(s, u, slot[1]);
-    // -inf - -inf is NaN: a row of nothing but -inf has to be told from one that also holds a NaN
-    const bool none = m == -INFINITY;
-    int bad = 0;
-    if (none)
-        for (int i = t; i < V; i += 256) bad |= isnan(to_f32(x[i]));
-    bad = __syncthreads_or(bad);
-    const bool empty = none && !bad;
-    const float log_s = empty ? 0.f : logf(su.x);
-    if (t == 0) {
-        if (g.stat) { g.stat[2 * row] = m; g.stat[2 * row + 1] = log_s; }
-        if (g.entropy) g.entropy[row] = empty ? 0.f : log_s - su.y / su.x;
-        if (g.labels && g.logprob) {
-            const int y = g.labels[row];
-            float lp = 0.f;
-            if (y >= V) lp = NAN;
-            else if (y >= 0) lp = empty ? -INFINITY : (to_f32(x[y]) - m) * g.inv_t - log_s;
-            g.logprob[row] = lp;
+    const unsigned long long hit = __ballot(above + same == n - 1);
+    const int src = __ffsll((long long)hit) - 1;
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), src));
+}
+
+// Leaves the k best of x[0, n) (indices from `base`) at out_val / out_idx in order, places without an element as index -1.
+// gmax[it * NT + t]: the group maxima.  sum: the part's s (NaN tells of NaN or +inf).
+template <class T, int NT>
+__device__ __forceinline__ void pick(const T* x, int n, int base, int k, int niter, const float* gmax, float tmax, float sum, PickLds<NT>& l,
+                     float* out_val, int* out_idx) {
+    constexpr int E = Pack<T>::N, W = NT / 64;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    bool slow = sum != sum;
+    if (!slow) {
+        const float mine = lanes_nth(tmax, (k + W - 1) / W);
+        if (lane == 0) l.tau[wave] = mine;
+        if (t == 0) l.count = 0;
+        team_sync<NT>();
+        float tau = l.tau[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) tau = fminf(tau, l.tau[i]);
+        int total = 0;
+        bool ties = false;
+        for (int pass = 0; pass < 2; ++pass) {
+            for (int it = 0; it < niter; ++it) {
+                const float gm = gmax[it * NT + t];
+                if (pass ? gm > tau : gm >= tau) {
+#pragma unroll
+                    for (int j = 0; j < U; ++j) {
+                        const long i0 = ((long)(it * U + j) * NT + t) * E;
+                        if (i0 >= n) continue;
+                        const Raw16 d = load_piece(x, (int)i0, n, -INFINITY);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const float f = elem<T>(d, e);
+                            if ((pass ? f > tau : f >= tau) && i0 + e < n) {
+                                const int at = atomicAdd(&l.count, 1);
+                                if (at < CAND) l.key[at] = order_key(f, base + (int)i0 + e);
+                            }
+                        }
+                    }
+                }
+            }
+            team_sync<NT>();
+            total = l.count;
+            team_sync<NT>();
+            if (total <= CAND) break;
+            if (pass == 0) {
+                ties = true;
+                if (t == 0) l.count = 0;
+                team_sync<NT>();
+            } else {
+                slow = true;
+            }
+        }
+        if (!slow) {
+            // order by counting: the list is short, every thread reads all of it (broadcasts)
+            for (int a = t; a < total; a += NT) {
+                const unsigned long long key = l.key[a];
+                int rank = 0;
+                for (int b = 0; b < total; ++b) rank += l.key[b] > key;
+                if (rank < k) {
+                    const int i = (int)~(unsigned)key;
+                    out_val[rank] = to_f32(x[i - base]);
+                    out_idx[rank] = i;
+                }
+            }
+            int have = total;
+            if (ties && have < k) {
+                // ties at tau in index order, E elements per thread at a time, until there are enough
+                for (long p0 = 0; p0 * E < n && have < k; p0 += NT) {
+                    const long i0 = (p0 + t) * E;
+                    unsigned hit = 0;
+                    if (i0 < n) {
+                        const Raw16 d = load_piece(x, (int)i0, n, -INFINITY);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) hit |= (elem<T>(d, e) == tau && i0 + e < n) ? 1u << e : 0u;
+                    }
+                    int before = __popc(hit);                           // inclusive count over the lanes
+#pragma unroll
+                    for (int o = 1; o < 64; o <<= 1) {
+                        const int v = __shfl_up(before, o, 64);
+                        if (lane >= o) before += v;
+                    }
+                    if (lane == 63) l.run[wave] = before;
+                    team_sync<NT>();
+                    int at = have + before - __popc(hit), all = 0;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        if (i < wave) at += l.run[i];
+                        all += l.run[i];
+                    }
+                    for (int e = 0; e < E; ++e)
+                        if (hit >> e & 1) {
+                            if (at < k) { out_val[at] = tau; out_idx[at] = base + (int)i0 + e; }
+                            ++at;
+                        }
+                    have += all;
+                    team_sync<NT>();
+                }
+            }
+            for (int a = have + t; a < k; a += NT) { out_val[a] = -INFINITY; out_idx[a] = -1; }
+            return;
         }
     }
     unsigned long long last = ~0ull;
-    for (int j = 0; j < g.k; ++j) {
+    for (int j = 0; j < k; ++j) {
         unsigned long long best = 0;
-        for (int i = t; i < V; i += 256) {
-            const unsigned long long key = order_key(to_f32(x[i]), i);
+        for (int i = t; i < n; i += NT) {
+            const unsigned long long key = order_key(to_f32(x[i]), base + i);
             if (key < last && key > best) best = key;
         }
-        last = block_max_key(best, kslot);
+        last = team_max_key<NT>(best, l.best);
         if (t == 0) {
             const int i = (int)~(unsigned)last;
-            g.top_idx[row * g.k + j] = i;
-            g.top_lp[row * g.k + j] = empty ? -INFINITY : (to_f32(x[i]) - m) * g.inv_t - log_s;
+            out_val[j] = last ? to_f32(x[i - base]) : -INFINITY;
+            out_idx[j] = last ? i : -1;
         }
     }
 }
 
-template <class T> __global__ __launch_bounds__(256) void scores_bwd_kernel(ScoresBwd g) {
+// ---- one walk over a part of a row ----------------------------------------------------------------------------------------
+template <class T, int NT, bool PICK>
+__device__ __forceinline__ Stat walk(const T* x, int n, float c, float* gmax, float& tmax) {
+    constexpr int E = Pack<T>::N, STEP = NT * U * E;
+    const int t = threadIdx.x;
+    Stat a{LOWEST, 0.f, 0.f};
+    tmax = -INFINITY;
+    int it = 0;
+    auto take = [&](const Raw16 (&d)[U]) {
+        float f[U * E];
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[j * E + e] = elem<T>(d[j], e);
+        float top = f[0];
+#pragma unroll
+        for (int e = 1; e < U * E; ++e) top = fmaxf(top, f[e]);
+        if constexpr (PICK) {
+            gmax[it * NT + t] = top;
+            tmax = fmaxf(tmax, top);
+        }
+        stat_add(a, f, top, c);
+    };
+    for (; (long)(it + 1) * STEP <= n; ++it) {
+        Raw16 d[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) d[j] = load16(x + (long)it * STEP + (j * NT + t) * E);
+        take(d);
+    }
+    if ((long)it * STEP < n) {
+        Raw16 d[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const long i0 = (long)it * STEP + (j * NT + t) * E;
+            const unsigned none = raw_fill<T>(-INFINITY);
+            d[j] = Raw16{{none, none, none, none}};
+            if (i0 < n) d[j] = load_piece(x, (int)i0, n, -INFINITY);
+        }
+        take(d);
+    }
+    return a;
+}
+
+template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scores_kernel(Scores g) {
+    constexpr int E = Pack<T>::N, STEP = NT * U * E;
+    extern __shared__ float gmax[];
+    __shared__ float slot[3 * (NT / 64)];
+    __shared__ PickLds<PICK ? NT : 64> l;
+    const long part = blockIdx.x, row = part / g.splits;
+    const int sp = (int)(part - row * g.splits);
+    const int lo = sp * g.chunk, n = min(g.chunk, g.V - lo);
+    const T* x = (const T*)g.X + row * g.ld + lo;
+    const int y = g.labels ? g.labels[row] : -1;
+    const float xy = g.splits == 1 && y >= 0 && y < g.V ? to_f32(x[y]) : 0.f;
+    const float c = g.inv_t * LOG2E;
+    float tmax;
+    Stat a = walk<T, NT, PICK>(x, n, c, gmax, tmax);
+    a = stat_team<NT>(a, c, slot);
+    float* w = g.work + part * (3 + 2 * g.k);
+    const bool whole = g.splits == 1;
+    RowEnd r{};
+    if (whole) {
+        r = row_end(a);
+        if (threadIdx.x == 0) row_store(g, row, r, xy, y);
+    } else if (threadIdx.x == 0) {
+        w[0] = a.m; w[1] = a.s; w[2] = a.u;
+    }
+    if constexpr (PICK) {
+        float* val = whole ? g.top_lp + row * g.k : w + 3;
+        int* idx = whole ? g.top_idx + row * g.k : (int*)(w + 3 + g.k);
+        pick<T, NT>(x, n, lo, g.k, cdiv_dev(n, STEP), gmax, tmax, a.s, l, val, idx);
+        if (whole) {
+            team_sync<NT>();
+            for (int j = threadIdx.x; j < g.k; j += NT) val[j] = row_lp(r, val[j], g.inv_t);
+        }
+    }
+}
+
+// the parts of a row: statistics in part order, alternatives from the parts' lists
+template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Scores g) {
+    extern __shared__ unsigned long long keys[];              // splits * k
+    __shared__ unsigned long long list[CAND];
+    __shared__ unsigned long long slot[4];
+    __shared__ int count;
     const long row = blockIdx.x;
+    const int t = threadIdx.x, S = g.splits, k = g.k;
+    const T* x = (const T*)g.X + row * g.ld;
+    const int y = g.labels ? g.labels[row] : -1;
+    const float xy = y >= 0 && y < g.V ? to_f32(x[y]) : 0.f;
+    const float* w = g.work + row * S * (3 + 2 * k);
+    const float c = g.inv_t * LOG2E;
+    Stat a{LOWEST, 0.f, 0.f};
+    for (int i = 0; i < S; ++i) a.m = fmaxf(a.m, w[(long)i * (3 + 2 * k)]);
+    for (int i = 0; i < S; ++i) {
+        const float* p = w + (long)i * (3 + 2 * k);
+        Stat b{p[0], p[1], p[2]};
+        stat_to(b, a.m, c);
+        a.s += b.s;
+        a.u += b.u;
+    }
+    const RowEnd r = row_end(a);
+    if (t == 0) row_store(g, row, r, xy, y);
+    if (k == 0) return;
+    if (t == 0) count = 0;
+    // a part's last entry, where its list is full, is reached by k elements: what is below the largest such is out
+    unsigned long long floor_ = 0;
+    for (int i = t; i < S * k; i += 256) {
+        const int s = i / k, j = i - s * k;
+        const float* p = w + (long)s * (3 + 2 * k) + 3;
+        const int at = ((const int*)p)[k + j];
+        const unsigned long long key = at < 0 ? 0ull : order_key(p[j], at);
+        keys[i] = key;
+        if (j == k - 1 && key > floor_) floor_ = key;
+    }
+    floor_ = team_max_key<256>(floor_, slot);
+    for (int i = t; i < S * k; i += 256)
+        if (keys[i] >= floor_ && keys[i]) {
+            const int at = atomicAdd(&count, 1);
+            if (at < CAND) list[at] = keys[i];
+        }
+    __syncthreads();
+    const bool all = count > CAND;
+    const unsigned long long* from = all ? keys : list;
+    const int n = all ? S * k : count;
+    for (int i = t; i < n; i += 256) {
+        const unsigned long long key = from[i];
+        if (!key) continue;
+        int rank = 0;
+        for (int b = 0; b < n; ++b) rank += from[b] > key;
+        if (rank < k) {
+            const int at = (int)~(unsigned)key;
+            g.top_idx[row * k + rank] = at;
+            g.top_lp[row * k + rank] = row_lp(r, to_f32(x[at]), g.inv_t);
+        }
+    }
+}
+
+// ---- few classes: a team of G lanes holds the row, R pieces per lane --------------------------------------------------------
+template <int G> __device__ __forceinline__ unsigned lanes_max_u32(unsigned v) {
+    auto step = [&](unsigned w) { v = w > v ? w : v; };
+    step(__builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
+    if constexpr (G >= 32) step(__shfl_xor(v, 16, 64));
+    if constexpr (G >= 64) step(__shfl_xor(v, 32, 64));
+    return v;
+}
+template <class T, int G, int R> __global__ __launch_bounds__(256) void scores_few_kernel(Scores g) {
+    constexpr int E = Pack<T>::N, TEAMS = 256 / G;
+    const int t = threadIdx.x % G, V = g.V;
+    const long row = (long)blockIdx.x * TEAMS + threadIdx.x / G;
+    if (row >= g.M) return;                                   // whole teams
+    const T* x = (const T*)g.X + row * g.ld;
+    const int y = g.labels ? g.labels[row] : -1;
+    const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
+    const float c = g.inv_t * LOG2E;
+    float f[R * E];
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i0 = (r * G + t) * E;
+        Raw16 d;
+        if (i0 < V) d = load_piece(x, i0, V, -INFINITY);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            f[r * E + e] = i0 < V ? elem<T>(d, e) : -INFINITY;
+            top = fmaxf(top, f[r * E + e]);
+        }
+    }
+    Stat a{LOWEST, 0.f, 0.f};
+    stat_add(a, f, fmaxf(lanes_max<G>(top), LOWEST), c);
+    a.s = lanes_sum<G>(a.s);
+    a.u = lanes_sum<G>(a.u);
+    const RowEnd r = row_end(a);
+    if (t == 0) row_store(g, row, r, xy, y);
+    // one alternative after another: best of the lane, best of the team, and the winner looks for its next
+    unsigned done = 0;                                        // elements of this lane already given
+    for (int j = 0; j < g.k; ++j) {
+        unsigned best = 0;
+        int at = 0x7fffffff, slot = 0;
+        float val = 0.f;
+#pragma unroll
+        for (int e = 0; e < R * E; ++e) {
+            const int i = ((e / E) * G + t) * E + e % E;
+            const unsigned b = order_bits(f[e]);
+            if (!(done >> e & 1) && i < V && b > best) { best = b; at = i; slot = e; val = f[e]; }
+        }
+        const unsigned m = lanes_max_u32<G>(best);
+        const unsigned who = ~lanes_max_u32<G>(best == m ? ~(unsigned)at : 0u);
+        if (at == (int)who && best == m) {
+            done |= 1u << slot;
+            g.top_idx[row * g.k + j] = at;
+            g.top_lp[row * g.k + j] = row_lp(r, val, g.inv_t);
+        }
+    }
+}
+
+// ---- gradient ---------------------------------------------------------------------------------------------------------------
+// One walk, element-wise once the row's statistics are known: ln p = (x - m) / T - ln s, d = -p (g + h H + h ln p) / T, + g / T at the
+// label.
+struct BwdRow {
+    float m, log_s, q0, q1, dl;      // d = -p (q0 + q1 ln p), + dl at y
+    int y;
+    bool empty;
+};
+__device__ __forceinline__ BwdRow bwd_row(const ScoresBwd& g, long row) {
+    BwdRow r;
+    r.m = g.stat[2 * row];
+    r.log_s = g.stat[2 * row + 1];
+    r.empty = r.m == -INFINITY && r.log_s == 0.f;
+    r.y = g.labels ? g.labels[row] : -1;
+    r.dl = g.d_lp && r.y >= 0 ? g.d_lp[row] * g.inv_t : 0.f;
+    if (r.y >= g.V) r.dl = NAN;
+    r.q1 = g.d_ent ? g.d_ent[row] * g.inv_t : 0.f;
+    r.q0 = g.d_ent ? fmaf(r.q1, g.entropy[row], r.dl) : r.dl;
+    return r;
+}
+template <class T> __device__ __forceinline__ void bwd_piece(const ScoresBwd& g, const BwdRow& r, const Raw16& d, T* o, int i0) {
+    constexpr int E = Pack<T>::N;
+    float f[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float lp = fmaf(elem<T>(d, e) - r.m, g.inv_t, -r.log_s), p = __builtin_amdgcn_exp2f(lp * LOG2E);
+        f[e] = -p * fmaf(r.q1, fmaxf(lp, FAINT), r.q0);
+    }
+    if (r.y >= i0 && r.y < i0 + E)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (i0 + e == r.y) f[e] += r.dl;
+    if (r.empty)
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = 0.f;
+    store_piece(o, i0, g.V, f);
+}
+// rows of many pieces: a workgroup takes U pieces per thread of one row
+template <class T> __global__ __launch_bounds__(256) void scores_bwd_kernel(ScoresBwd g) {
+    constexpr int E = Pack<T>::N, STEP = 256 * U * E;
+    const long row = blockIdx.x / g.chunks;
+    const int base = (int)(blockIdx.x - row * g.chunks) * STEP;
     const T* x = (const T*)g.X + row * g.ld;
     T* o = (T*)g.DX + row * g.lddx;
-    const float m = g.stat[2 * row], log_s = g.stat[2 * row + 1];
-    const bool empty = m == -INFINITY && log_s == 0.f;
-    const int y = g.labels ? g.labels[row] : -1;
-    float dl = g.d_lp && y >= 0 ? g.d_lp[row] : 0.f;
-    if (y >= g.V) dl = NAN;
-    const float dh = g.d_ent ? g.d_ent[row] : 0.f, H = g.d_ent ? g.entropy[row] : 0.f;
-    for (int i = threadIdx.x; i < g.V; i += 256) {
-        const float lp = (to_f32(x[i]) - m) * g.inv_t - log_s, p = __expf(lp);
-        float d = -dl * p - (p != 0.f ? dh * p * (lp + H) : 0.f);
-        if (i == y) d += dl;
-        o[i] = from_f32<T>(empty ? 0.f : d * g.inv_t);
+    Raw16 d[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int i0 = base + (j * 256 + (int)threadIdx.x) * E;
+        if (i0 < g.V) d[j] = load_piece(x, i0, g.V, 0.f);
     }
+    const BwdRow r = bwd_row(g, row);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int i0 = base + (j * 256 + (int)threadIdx.x) * E;
+        if (i0 < g.V) bwd_piece(g, r, d[j], o, i0);
+    }
+}
+// short rows: one thread per piece, all rows' pieces in one run
+template <class T> __global__ __launch_bounds__(256) void scores_bwd_few_kernel(ScoresBwd g) {
+    constexpr int E = Pack<T>::N;
+    const long p = (long)blockIdx.x * 256 + threadIdx.x;
+    const long row = p / g.chunks;
+    if (row >= g.M) return;
+    const int i0 = (int)(p - row * g.chunks) * E;
+    const Raw16 d = load_piece((const T*)g.X + row * g.ld, i0, g.V, 0.f);
+    bwd_piece(g, bwd_row(g, row), d, (T*)g.DX + row * g.lddx, i0);
 }
 
 bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
@@ -129,6 +562,74 @@ bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
     return p && !((uintptr_t)p & align) && (M <= 1 || ld >= V);
 }
 constexpr int MAX_V = 1 << 28, MAX_K = 64;
+int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
+
+// Few classes stay in the registers of a team inside a wave.  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192
+// 16-bit or 4096 fp32 classes); a row is split over workgroups while there are fewer than 1024 of them, and where its group maxima
+// would take more than 32 steps' room in LDS.
+constexpr int FEW = 128;                  // lanes * pieces of the team form: up to 1024 16-bit or 512 fp32 classes
+constexpr int MOST_STEPS = 32;
+struct ScoresShape {
+    int splits, chunk, steps;             // splits = 0: the team form
+};
+ScoresShape scores_shape(int M, int V, int dtype, int k) {
+    const int E = elems_of(dtype);
+    if (V <= FEW * E) return {0, V, 0};
+    const int step = 256 * U * E, steps = cdiv(V, step);
+    int S = M >= 1024 ? 1 : cdiv(1024, M > 0 ? M : 1);
+    if (S > steps) S = steps;
+    if (S > 64) S = 64;
+    if (k > 0 && S * MOST_STEPS < steps) S = cdiv(steps, MOST_STEPS);
+    const int each = cdiv(steps, S);
+    return {cdiv(steps, each), each * step, each};
+}
+
+template <class T> int scores(Scores g, hipStream_t st) {
+    constexpr int E = Pack<T>::N;
+    const int dtype = sizeof(T) == 4 ? WFD_F32 : WFD_BF16;
+    const ScoresShape s = scores_shape(g.M, g.V, dtype, g.k);
+    g.splits = s.splits;
+    g.chunk = s.chunk;
+    if (s.splits == 0) {
+#define WFD_FEW(G, R)                                                                                                    \
+    if (g.V <= G * R * E) {                                                                                              \
+        hipLaunchKernelGGL((scores_few_kernel<T, G, R>), dim3(cdiv(g.M, 256 / G)), dim3(256), 0, st, g);                 \
+        WFD_CHECK_LAUNCH();                                                                                              \
+        return WFD_OK;                                                                                                   \
+    }
+        WFD_FEW(16, 1) WFD_FEW(16, 2) WFD_FEW(64, 1) WFD_FEW(64, 2)
+#undef WFD_FEW
+    }
+    const long parts = (long)g.M * s.splits;
+    if (parts > 0x7fffffffL) return WFD_ERR_ARG;
+    if (g.k > 0)
+        hipLaunchKernelGGL((scores_kernel<T, 256, true>), dim3((unsigned)parts), dim3(256), (size_t)s.steps * 1024, st, g);
+    else
+        hipLaunchKernelGGL((scores_kernel<T, 256, false>), dim3((unsigned)parts), dim3(256), 0, st, g);
+    WFD_CHECK_LAUNCH();
+    if (s.splits > 1) {
+        hipLaunchKernelGGL((scores_join_kernel<T>), dim3(g.M), dim3(256), (size_t)s.splits * g.k * 8, st, g);
+        WFD_CHECK_LAUNCH();
+    }
+    return WFD_OK;
+}
+
+template <class T> int scores_bwd(ScoresBwd g, hipStream_t st) {
+    constexpr int E = Pack<T>::N, STEP = 256 * U * E;
+    if (g.V > STEP / 2) {
+        g.chunks = cdiv(g.V, STEP);
+        const long blocks = (long)g.M * g.chunks;
+        if (blocks > 0x7fffffffL) return WFD_ERR_ARG;
+        hipLaunchKernelGGL(scores_bwd_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, g);
+    } else {
+        g.chunks = cdiv(g.V, E);
+        const long blocks = ((long)g.M * g.chunks + 255) / 256;
+        if (blocks > 0x7fffffffL) return WFD_ERR_ARG;
+        hipLaunchKernelGGL(scores_bwd_few_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, g);
+    }
+    WFD_CHECK_LAUNCH();
+    return WFD_OK;
+}
 
 }  // namespace
 
@@ -136,7 +637,10 @@ extern "C" {
 
 int wfd_label_scores_floats(int M, int V, int dtype, int k) {
     if (!wfd_dtype_ok(dtype) || M < 0 || V <= 0 || V > MAX_V || k < 0 || k > MAX_K || k > V) return -1;
-    return 0;
+    const ScoresShape s = scores_shape(M, V, dtype, k);
+    if (M == 0 || s.splits <= 1) return 0;
+    const long n = (long)M * s.splits * (3 + 2 * k);
+    return n > 0x7fffffffL ? -1 : (int)n;
 }
 
 int wfd_label_scores(const void* logits, int ldl, int dtype, int M, int V, const int* labels, float temperature, int k,
@@ -147,13 +651,10 @@ int wfd_label_scores(const void* logits, int ldl, int dtype, int M, int V, const
     if (M == 0) return WFD_OK;
     if ((k > 0 && (!top_logprob || !top_index)) || (logprob && !labels)) return WFD_ERR_ARG;
     if (!rows_ok(logits, ldl, M, V, dtype)) return WFD_ERR_ARG;
-    Scores g{logits, labels, logprob, entropy, stat, top_logprob, top_index, ldl, M, V, k, 1.f / temperature};
+    Scores g{logits, labels, logprob, entropy, stat, top_logprob, top_index, work, ldl, M, V, k, 1.f / temperature, 0, 0};
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == WFD_F32) hipLaunchKernelGGL(scores_kernel<float>, dim3(M), dim3(256), 0, st, g);
-    else if (dtype == WFD_BF16) hipLaunchKernelGGL(scores_kernel<bf16_t>, dim3(M), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL(scores_kernel<f16_t>, dim3(M), dim3(256), 0, st, g);
-    WFD_CHECK_LAUNCH();
-    return WFD_OK;
+    if (dtype == WFD_F32) return scores<float>(g, st);
+    return dtype == WFD_BF16 ? scores<bf16_t>(g, st) : scores<f16_t>(g, st);
 }
 
 int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, const int* labels, float temperature,
@@ -164,13 +665,10 @@ int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, c
     if (M == 0) return WFD_OK;
     if ((d_logprob && !labels) || (d_entropy && !entropy)) return WFD_ERR_ARG;
     if (!stat || !rows_ok(logits, ldl, M, V, dtype) || !rows_ok(dlogits, lddl, M, V, dtype)) return WFD_ERR_ARG;
-    ScoresBwd g{logits, labels, stat, entropy, d_logprob, d_entropy, dlogits, ldl, lddl, M, V, 1.f / temperature};
+    ScoresBwd g{logits, labels, stat, entropy, d_logprob, d_entropy, dlogits, ldl, lddl, M, V, 1.f / temperature, 0};
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == WFD_F32) hipLaunchKernelGGL(scores_bwd_kernel<float>, dim3(M), dim3(256), 0, st, g);
-    else if (dtype == WFD_BF16) hipLaunchKernelGGL(scores_bwd_kernel<bf16_t>, dim3(M), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL(scores_bwd_kernel<f16_t>, dim3(M), dim3(256), 0, st, g);
-    WFD_CHECK_LAUNCH();
-    return WFD_OK;
+    if (dtype == WFD_F32) return scores_bwd<float>(g, st);
+    return dtype == WFD_BF16 ? scores_bwd<bf16_t>(g, st) : scores_bwd<f16_t>(g, st);
 }
 
 }  // extern "C"
