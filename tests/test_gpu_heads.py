@@ -444,6 +444,16 @@ def test_distill_in_place_equals_out_of_place():
             assert torch.equal(got.loss, want.loss) and torch.equal(x, want.dlogits)
 
 
+def test_distill_teacher_sure_beyond_the_range_of_exponentials():
+    """Entries 60 to 130 below the best one: shares that are tiny, subnormal or zero in fp32 add nothing worth a digit."""
+    for t in TYPES:
+        x, ti, tv, y, rs = distill_inputs(8, 300, 60, t, seed=4)
+        tv = -torch.linspace(0, 130, 60).repeat(8, 1)
+        tv[:, 1:] -= 2.0
+        check_distill(x, ti, tv, y, 1.0, 1.0, 0.0, rs, 1.0, x.to(DEV))
+        check_distill(x, ti, tv, y, 0.9, 0.5, 0.5, rs, 1.0, x.to(DEV))
+
+
 def test_distill_gradient_against_differences():
     x, ti, tv, y, rs = distill_inputs(4, 19, 6, F32, seed=8)
     ti[0, 1] = ti[0, 0]

@@ -5,11 +5,16 @@
 //   d x_i = r (w T (p_i [any entry] - sum_{j: i_j = i} q_j) + u (p1_i - [i = y]))          r = grad_scale * row_scale[row]
 // An index that occurs twice counts twice.  No entry (or none above -inf): the first term is 0; y < 0: the second is 0.
 // A row that holds nothing but -inf has loss +inf and gradient 0; an index or label >= V makes its row NaN.
+// Bound by memory: the row is read once and, with a gradient, written once.  In between it stays packed in the registers of its
+// team (up to 1024 threads x 16 pieces: 131072 16-bit or 65536 fp32 classes), so that maximum, sum and gradient cost one read.  A few
+// long rows are split over workgroups instead: partial sums in a first launch, loss and gradient in a second.
 #include "rowops.h"
 
 namespace {
 
 constexpr int MAX_ENTRIES = 256;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOWEST = -3.402823466e38f;       // floor of a maximum: x - m stays defined for rows of -inf
 
 struct Distill {
     const void* X;
@@ -19,82 +24,335 @@ struct Distill {
     const float* row_scale;
     float* loss;
     void* DX;
+    float* work;            // split form: [M][3 * splits + MAX_ENTRIES + 1]: partial sums, the entries' and the label's logits
     int ld, lddx, ldt, M, V, K;
     float temp, w, u, scale;
+    int splits, chunk;      // split form: parts of a row, their length
 };
 
-template <class T> __global__ __launch_bounds__(256) void distill_kernel(Distill g) {
-    __shared__ float slot[6][8];
-    __shared__ float q[MAX_ENTRIES];
-    __shared__ int at[MAX_ENTRIES];
-    const long row = blockIdx.x;
+__device__ __forceinline__ void wave_sync() {           // LDS traffic between the lanes of one wave
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A row's teacher entries in LDS, worked on by L lanes of one wave: where they point, exp((t - max) / T), the student's logits there.
+struct Entries {
+    int* at;
+    float* e;
+    float* x;
+};
+__device__ __forceinline__ Entries entries_in(float* lds, int K) { return {(int*)lds, lds + K, lds + 2 * K}; }
+
+struct Taught {
+    float max, sum;         // of the entries that are there; sum = 0: none
+    bool wrong;             // an index beyond the classes
+};
+template <int L> __device__ __forceinline__ Taught teacher(const Distill& g, long row, int lane, const Entries& n, float c) {
+    const int K = g.K;
+    Taught r{-INFINITY, 0.f, false};
+    float bad = 0.f;
+    for (int j = lane; j < K; j += L) {
+        int at = g.t_idx[row * g.ldt + j];
+        const float v = g.t_val[row * g.ldt + j];
+        if (at >= g.V) { bad = 1.f; at = -1; }
+        n.at[j] = at;
+        n.e[j] = at < 0 ? -INFINITY : v;
+        r.max = fmaxf(r.max, n.e[j]);
+    }
+    r.max = fmaxf(lanes_max<L>(r.max), LOWEST);
+    for (int j = lane; j < K; j += L) {
+        n.e[j] = __builtin_amdgcn_exp2f((n.e[j] - r.max) * c);
+        r.sum += n.e[j];
+    }
+    r.sum = lanes_sum<L>(r.sum);
+    r.wrong = lanes_max<L>(bad) != 0.f;
+    return r;
+}
+template <class T, int L> __device__ __forceinline__ void entries_gather(const T* x, int K, int lane, const Entries& n) {
+    for (int j = lane; j < K; j += L) n.x[j] = n.at[j] >= 0 ? to_f32(x[n.at[j]]) : 0.f;
+}
+
+struct RowSums {
+    float m, s, s1;         // maximum (floored), sum exp((x - m) / T), sum exp(x - m)
+};
+
+// the row's loss (every lane), from the entries and the sums
+template <int L>
+__device__ __forceinline__ float row_loss(const Distill& g, long row, int lane, const Entries& n, const Taught& t, const RowSums& s,
+                                          float inv_t, int y, float xy, bool wrong) {
+    const bool empty = s.s == 0.f;
+    float kl = 0.f;
+    if (t.sum != 0.f) {
+        const float inv = 1.f / t.sum, log_t = LN2 * __log2f(t.sum), log_s = LN2 * __log2f(s.s);
+        for (int j = lane; j < g.K; j += L) {
+            const float q = n.e[j] * inv;
+            if (!(n.e[j] < 1.17549435e-38f)) {  // below the normal range a share is as good as none, and has no logarithm
+                const float lq = LN2 * __log2f(n.e[j]) - log_t;
+                const float lp = empty ? -INFINITY : (n.x[j] - s.m) * inv_t - log_s;
+                kl = fmaf(q, lq - lp, kl);
+            }
+        }
+    }
+    kl = lanes_sum<L>(kl);
+    float loss = g.K ? g.w * g.temp * g.temp * kl : 0.f;
+    if (y >= 0) loss -= g.u * (empty ? -INFINITY : xy - s.m - LN2 * __log2f(s.s1));
+    return wrong ? NAN : loss;
+}
+
+// what a gradient element is made of: d = cw exp((x - m) / T) + cu exp(x - m), less the targets at the entries and the label
+struct GradRow {
+    float m, cw, cu, r, rt;        // r = grad_scale * row_scale, rt = r w T / (sum of the teacher's exponentials)
+};
+__device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Taught& t, const RowSums& s, int y, bool wrong) {
+    GradRow d;
+    d.m = s.m;
+    d.r = g.scale * (g.row_scale ? g.row_scale[row] : 1.f);
+    if (wrong) d.r = NAN;
+    const bool empty = s.s == 0.f, on = t.sum != 0.f;
+    d.rt = on ? d.r * g.w * g.temp / t.sum : 0.f;
+    d.cw = on ? d.r * g.w * g.temp / s.s : 0.f;
+    d.cu = y >= 0 ? d.r * g.u / s.s1 : 0.f;
+    if (empty) d.cw = d.cu = wrong ? NAN : 0.f;
+    return d;
+}
+template <class T, bool TWO>
+__device__ __forceinline__ void grad_piece(const GradRow& d, const Raw16& p, T* o, int i0, int V, float c) {
+    constexpr int E = Pack<T>::N;
+    float f[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float z = elem<T>(p, e) - d.m;
+        f[e] = d.cw * __builtin_amdgcn_exp2f(z * c);
+        if constexpr (TWO) f[e] = fmaf(d.cu, __builtin_amdgcn_exp2f(z * LOG2E), f[e]);
+    }
+    store_piece(o, i0, V, f);
+}
+// the elements with a target, whole again: the first occurrence of an index subtracts all of its entries, the label its own.
+// Only those of [lo, hi); runs after a barrier behind the stores that it overwrites.
+template <class T, bool TWO, int L>
+__device__ __forceinline__ void grad_targets(const Distill& g, const GradRow& d, const Entries& n, bool empty, int lane, T* o, int lo,
+                                             int hi, int y, float xy, float c) {
+    if (empty) return;
+    auto dense = [&](float x) {
+        const float z = x - d.m;
+        float v = d.cw * __builtin_amdgcn_exp2f(z * c);
+        if constexpr (TWO) v = fmaf(d.cu, __builtin_amdgcn_exp2f(z * LOG2E), v);
+        return v;
+    };
+    bool label_seen = false;
+    for (int j = lane; j < g.K; j += L) {
+        const int at = n.at[j];
+        if (at < lo || at >= hi) continue;
+        float sum = 0.f;
+        bool first = true;
+        for (int i = 0; i < g.K; ++i)
+            if (n.at[i] == at) {
+                sum += n.e[i];
+                first = first && i >= j;
+            }
+        if (at == y) label_seen = true;
+        if (first) {
+            float v = dense(n.x[j]) - d.rt * sum;
+            if (at == y) v -= d.r * g.u;
+            o[at] = from_f32<T>(v);
+        }
+    }
+    const bool seen = lanes_max<L>(label_seen ? 1.f : 0.f) != 0.f;
+    if (lane == 0 && !seen && y >= lo && y < hi && y < g.V) o[y] = from_f32<T>(dense(xy) - d.r * g.u);
+}
+
+// ---- a row in the registers of a team of G threads ----------------------------------------------------------------------------
+// TWO: a label is mixed in at a temperature other than 1, so two sums of exponentials are kept.  Without, every exponential serves both
+// terms and cu joins cw.
+template <class T, int G, int R, bool TWO>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void distill_kernel(Distill g) {
+    constexpr int E = Pack<T>::N, TEAMS = G < 256 ? 256 / G : 1, L = G < 64 ? G : 64;
+    extern __shared__ float lds[];
+    __shared__ float slot[2][2 * (G > 64 ? G / 64 : 1)], told[8];
+    const int t = threadIdx.x % G, team = threadIdx.x / G, V = g.V;
+    const long row = (long)blockIdx.x * TEAMS + team;
+    if (row >= g.M) return;                                   // whole teams, each inside a wave
     const T* x = (const T*)g.X + row * g.ld;
-    const int t = threadIdx.x, V = g.V, K = g.w != 0.f ? g.K : 0;
-    const float it = 1.f / g.temp;
-    const int y = g.u != 0.f && g.labels ? g.labels[row] : -1;
-    float bad = y >= V ? 1.f : 0.f;
-    int e_idx = -1;
-    float e_val = -INFINITY, e_x = 0.f;
-    if (t < K) {
-        e_idx = g.t_idx[row * g.ldt + t];
-        if (e_idx >= V) { bad = 1.f; e_idx = -1; }
-        if (e_idx >= 0) { e_val = g.t_val[row * g.ldt + t]; e_x = to_f32(x[e_idx]); }
-        at[t] = e_idx;
+    const float inv_t = 1.f / g.temp, c = inv_t * LOG2E;
+    Raw16 d[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i0 = (r * G + t) * E;
+        const unsigned none = raw_fill<T>(-INFINITY);
+        d[r] = Raw16{{none, none, none, none}};
+        if (i0 < V) d[r] = load_piece(x, i0, V, -INFINITY);
     }
+    const Entries n = entries_in(lds + team * 3 * g.K, g.K);
+    const int y = g.u != 0.f ? g.labels[row] : -1;
     const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
+    Taught tt{LOWEST, 0.f, false};
+    if (t < L) {
+        tt = teacher<L>(g, row, t, n, c);
+        wave_sync();
+        entries_gather<T, L>(x, g.K, t, n);
+        if constexpr (G > 64)
+            if (t == 0) { told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f; }
+    }
     float m = -INFINITY;
-    for (int i = t; i < V; i += 256) m = fmaxf(m, to_f32(x[i]));
-    m = team_max<256>(m, slot[0]);
-    float s = 0.f, s1 = 0.f;
-    for (int i = t; i < V; i += 256) {
-        const float d = to_f32(x[i]) - m;
-        s += __expf(d * it);
-        s1 += __expf(d);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        keep_packed(d[r]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, elem<T>(d[r], e));
     }
-    const float2 ss = team_sum2<256>(s, s1, slot[1]);
-    int nan_here = 0;
-    if (m == -INFINITY)
-        for (int i = t; i < V; i += 256) nan_here |= isnan(to_f32(x[i]));
-    const bool empty = m == -INFINITY && !__syncthreads_or(nan_here);
-    const float log_s = logf(ss.x), log_s1 = logf(ss.y);
-    // the teacher's softmax
-    const float tm = team_max<256>(e_val, slot[2]);
-    const float e = e_val == -INFINITY ? 0.f : __expf((e_val - tm) * it);
-    const float2 es = team_sum2<256>(e, bad, slot[3]);
-    const bool taught = !(es.x <= 0.f);
-    const float my_q = taught ? e / es.x : 0.f;
-    if (t < K) q[t] = my_q;
-    float term = 0.f;
-    if (my_q != 0.f) {
-        const float lp = empty ? -INFINITY : (e_x - m) * it - log_s;
-        term = my_q * ((e_val - tm) * it - logf(es.x) - lp);
+    RowSums s{fmaxf(team_max<G>(m, slot[0]), LOWEST), 0.f, 0.f};
+    if constexpr (G > 64) tt = Taught{told[0], told[1], told[2] != 0.f};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        keep_packed(d[r]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float z = elem<T>(d[r], e) - s.m;
+            s.s += __builtin_amdgcn_exp2f(z * c);
+            if constexpr (TWO) s.s1 += __builtin_amdgcn_exp2f(z * LOG2E);
+        }
     }
-    const float kl = team_sum<256>(term, slot[4]);
-    const bool wrong = es.y != 0.f;
-    if (t == 0) {
-        float loss = g.w != 0.f ? g.w * g.temp * g.temp * kl : 0.f;
-        if (y >= 0) loss -= g.u * (empty ? -INFINITY : xy - m - log_s1);
-        g.loss[row] = wrong ? NAN : loss;
+    if constexpr (TWO) {
+        const float2 q = team_sum2<G>(s.s, s.s1, slot[1]);
+        s.s = q.x;
+        s.s1 = q.y;
+    } else {
+        s.s1 = s.s = team_sum<G>(s.s, slot[1]);
+    }
+    const bool wrong = tt.wrong || y >= V;
+    if (t < L) {
+        wave_sync();
+        const float loss = row_loss<L>(g, row, t, n, tt, s, inv_t, y, xy, wrong);
+        if (t == 0) g.loss[row] = loss;
     }
     if (!g.DX) return;
+    GradRow k = grad_row(g, row, tt, s, y, wrong);
+    if constexpr (!TWO) k.cw += k.cu;
     T* o = (T*)g.DX + row * g.lddx;
-    float r = g.scale * (g.row_scale ? g.row_scale[row] : 1.f);
-    if (wrong) r = NAN;
-    const float cw = taught ? r * g.w * g.temp / ss.x : 0.f, cu = y >= 0 ? r * g.u / ss.y : 0.f;
-    for (int i = t; i < V; i += 256) {
-        const float d = to_f32(x[i]) - m;
-        float v = 0.f;
-        if (cw != 0.f) v = cw * __expf(d * it);
-        if (cu != 0.f) v = fmaf(cu, __expf(d), v);
-        if (i == y) v -= r * g.u;
-        if (empty) v = wrong ? NAN : 0.f;
-        bool entry = false;
-        float sq = 0.f;
-        for (int j = 0; j < K; ++j)
-            if (at[j] == i) { entry = true; sq += q[j]; }
-        if (entry && !empty) v -= r * g.w * g.temp * sq;
-        o[i] = from_f32<T>(v);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i0 = (r * G + t) * E;
+        keep_packed(d[r]);
+        if (i0 < V) grad_piece<T, TWO>(k, d[r], o, i0, V, c);
     }
+    if constexpr (G > 64) __syncthreads();
+    else wave_sync();
+    if (t < L) grad_targets<T, TWO, L>(g, k, n, s.s == 0.f, t, o, 0, V, y, xy, c);
+}
+
+// ---- rows split over workgroups -------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void sums_to(RowSums& a, float m, float c) {
+    const float d = fmaxf(a.m - m, -1e30f);
+    a.s *= __builtin_amdgcn_exp2f(d * c);
+    a.s1 *= __builtin_amdgcn_exp2f(d * LOG2E);
+    a.m = m;
+}
+constexpr int U = 4;
+template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_part_kernel(Distill g) {
+    constexpr int E = Pack<T>::N, STEP = 256 * U * E;
+    __shared__ float slot[3][8];
+    const long row = blockIdx.x / g.splits;
+    const int sp = (int)(blockIdx.x - row * g.splits), t = threadIdx.x;
+    const int lo = sp * g.chunk, n = min(g.chunk, g.V - lo);
+    const T* x = (const T*)g.X + row * g.ld;
+    float* w = g.work + row * (3L * g.splits + MAX_ENTRIES + 1);
+    const float c = LOG2E / g.temp;
+    RowSums a{LOWEST, 0.f, 0.f};
+    for (long b = 0; b < n; b += STEP) {
+        Raw16 d[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const long i0 = b + (j * 256 + t) * E;
+            const unsigned none = raw_fill<T>(-INFINITY);
+            d[j] = Raw16{{none, none, none, none}};
+            if (i0 < n) d[j] = load_piece(x + lo, (int)i0, n, -INFINITY);
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = fmaxf(top, elem<T>(d[j], e));
+        if (top > a.m) sums_to(a, top, c);
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float z = elem<T>(d[j], e) - a.m;
+                a.s += __builtin_amdgcn_exp2f(z * c);
+                if constexpr (TWO) a.s1 += __builtin_amdgcn_exp2f(z * LOG2E);
+            }
+    }
+    const float m = team_max<256>(a.m, slot[0]);
+    sums_to(a, m, c);
+    const float2 q = team_sum2<256>(a.s, a.s1, slot[1]);
+    if (t == 0) { w[3 * sp] = m; w[3 * sp + 1] = q.x; w[3 * sp + 2] = TWO ? q.y : q.x; }
+    // the logits that the second launch needs by index, before a gradient in place could lie over them
+    if (sp == 0) {
+        if (t < g.K) {
+            const int at = g.t_idx[row * g.ldt + t];
+            w[3 * g.splits + t] = at >= 0 && at < g.V ? to_f32(x[at]) : 0.f;
+        }
+        if (t == 0) {
+            const int y = g.u != 0.f ? g.labels[row] : -1;
+            w[3 * g.splits + MAX_ENTRIES] = y >= 0 && y < g.V ? to_f32(x[y]) : 0.f;
+        }
+    }
+}
+template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_finish_kernel(Distill g) {
+    constexpr int E = Pack<T>::N, STEP = 256 * U * E;
+    extern __shared__ float lds[];
+    __shared__ float told[8];
+    const int parts = g.DX ? cdiv_dev(g.V, STEP) : 1;
+    const long row = blockIdx.x / parts;
+    const int lo = (int)(blockIdx.x - row * parts) * STEP, t = threadIdx.x, V = g.V;
+    const T* x = (const T*)g.X + row * g.ld;
+    const float* w = g.work + row * (3L * g.splits + MAX_ENTRIES + 1);
+    const float inv_t = 1.f / g.temp, c = inv_t * LOG2E;
+    const Entries n = entries_in(lds, g.K);
+    const int y = g.u != 0.f ? g.labels[row] : -1;
+    Raw16 d[U];
+    if (g.DX)
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int i0 = lo + (j * 256 + t) * E;
+            if (i0 < V) d[j] = load_piece(x, i0, V, -INFINITY);
+        }
+    float xy = 0.f;
+    Taught tt{LOWEST, 0.f, false};
+    RowSums s{LOWEST, 0.f, 0.f};
+    if (t < 64) {
+        // splits <= 64: a lane per part, met in a fixed order
+        if (t < g.splits) s = RowSums{w[3 * t], w[3 * t + 1], w[3 * t + 2]};
+        xy = w[3 * g.splits + MAX_ENTRIES];
+        for (int j = t; j < g.K; j += 64) n.x[j] = w[3 * g.splits + j];
+        tt = teacher<64>(g, row, t, n, c);
+        sums_to(s, lanes_max<64>(s.m), c);
+        s.s = lanes_sum<64>(s.s);
+        s.s1 = lanes_sum<64>(s.s1);
+        if (t == 0) {
+            told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f;
+            told[3] = s.m; told[4] = s.s; told[5] = s.s1;
+        }
+        if (lo == 0) {
+            wave_sync();
+            const float loss = row_loss<64>(g, row, t, n, tt, s, inv_t, y, xy, tt.wrong || y >= V);
+            if (t == 0) g.loss[row] = loss;
+        }
+    }
+    if (!g.DX) return;
+    __syncthreads();
+    tt = Taught{told[0], told[1], told[2] != 0.f};
+    s = RowSums{told[3], told[4], told[5]};
+    GradRow k = grad_row(g, row, tt, s, y, tt.wrong || y >= V);
+    if constexpr (!TWO) k.cw += k.cu;
+    T* o = (T*)g.DX + row * g.lddx;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int i0 = lo + (j * 256 + t) * E;
+        if (i0 < V) grad_piece<T, TWO>(k, d[j], o, i0, V, c);
+    }
+    __syncthreads();
+    if (t < 64) grad_targets<T, TWO, 64>(g, k, n, s.s == 0.f, t, o, lo, min(lo + STEP, V), y, xy, c);
 }
 
 bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
@@ -102,6 +360,53 @@ bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
     return p && !((uintptr_t)p & align) && (M <= 1 || ld >= V);
 }
 constexpr int MAX_V = 1 << 28;
+int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
+
+// Rows stay in registers up to 1024 threads x 16 pieces; longer ones are split, and so are long ones of which there are too few to
+// give every CU its own.
+struct DistillShape {
+    int splits, chunk;                // splits = 0: the register form
+};
+DistillShape distill_shape(int M, int V, int dtype) {
+    const int E = elems_of(dtype);
+    if (V <= 1024 * 16 * E && (V <= 256 * 16 * E || M > 96)) return {0, V};
+    const int step = 256 * U * E, steps = cdiv(V, step);
+    int S = M >= 1024 ? 1 : cdiv(1024, M > 0 ? M : 1);
+    if (S > steps) S = steps;
+    if (S > 64) S = 64;
+    const int each = cdiv(steps, S);
+    return {cdiv(steps, each), each * step};
+}
+
+template <class T, bool TWO> int distill(Distill g, hipStream_t st) {
+    constexpr int E = Pack<T>::N;
+    const DistillShape s = distill_shape(g.M, g.V, sizeof(T) == 4 ? WFD_F32 : WFD_BF16);
+    g.splits = s.splits;
+    g.chunk = s.chunk;
+    if (s.splits == 0) {
+#define WFD_GO(G, R)                                                                                                     \
+    if (g.V <= G * R * E) {                                                                                              \
+        constexpr int TEAMS = G < 256 ? 256 / G : 1;                                                                     \
+        hipLaunchKernelGGL((distill_kernel<T, G, R, TWO>), dim3(cdiv(g.M, TEAMS)), dim3(G < 256 ? 256 : G),              \
+                           (size_t)TEAMS * 3 * g.K * 4, st, g);                                                          \
+        WFD_CHECK_LAUNCH();                                                                                              \
+        return WFD_OK;                                                                                                   \
+    }
+        WFD_GO(16, 1) WFD_GO(16, 2) WFD_GO(64, 1) WFD_GO(64, 2) WFD_GO(64, 4) WFD_GO(256, 4) WFD_GO(256, 8) WFD_GO(256, 16)
+        WFD_GO(512, 16) WFD_GO(1024, 16)
+#undef WFD_GO
+    }
+    const int parts = g.DX ? cdiv(g.V, 256 * U * E) : 1;
+    if ((long)g.M * s.splits > 0x7fffffffL || (long)g.M * parts > 0x7fffffffL) return WFD_ERR_ARG;
+    hipLaunchKernelGGL((distill_part_kernel<T, TWO>), dim3(g.M * s.splits), dim3(256), 0, st, g);
+    WFD_CHECK_LAUNCH();
+    hipLaunchKernelGGL((distill_finish_kernel<T, TWO>), dim3(g.M * parts), dim3(256), (size_t)3 * g.K * 4, st, g);
+    WFD_CHECK_LAUNCH();
+    return WFD_OK;
+}
+template <class T> int distill(const Distill& g, hipStream_t st) {
+    return g.temp != 1.f && g.u != 0.f ? distill<T, true>(g, st) : distill<T, false>(g, st);
+}
 
 }  // namespace
 
@@ -109,7 +414,10 @@ extern "C" {
 
 int wfd_distill_floats(int M, int V, int dtype) {
     if (!wfd_dtype_ok(dtype) || M < 0 || V <= 0 || V > MAX_V) return -1;
-    return 0;
+    const DistillShape s = distill_shape(M, V, dtype);
+    if (M == 0 || s.splits == 0) return 0;
+    const long n = (long)M * (3 * s.splits + MAX_ENTRIES + 1);
+    return n > 0x7fffffffL ? -1 : (int)n;
 }
 
 int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int* t_index, const float* t_value, int ldt, int K,
@@ -123,14 +431,14 @@ int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int*
     if (label_weight != 0.f && !labels) return WFD_ERR_ARG;
     if (!loss || !rows_ok(logits, ldl, M, V, dtype) || (dlogits && !rows_ok(dlogits, lddl, M, V, dtype))) return WFD_ERR_ARG;
     if (K > 0 && (!t_index || !t_value || (M > 1 && ldt < K))) return WFD_ERR_ARG;
-    Distill g{logits, t_index, t_value, labels, row_scale, loss, dlogits, ldl, lddl, ldt, M, V, K, temperature, weight,
-              label_weight, grad_scale};
+    // without weight the entries are not read, and the label's term has no temperature
+    if (weight == 0.f) K = 0;
+    if (K == 0) temperature = 1.f;
+    Distill g{logits, t_index, t_value, labels, row_scale, loss, dlogits, work, ldl, lddl, ldt, M, V, K, temperature, weight,
+              label_weight, grad_scale, 0, 0};
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == WFD_F32) hipLaunchKernelGGL(distill_kernel<float>, dim3(M), dim3(256), 0, st, g);
-    else if (dtype == WFD_BF16) hipLaunchKernelGGL(distill_kernel<bf16_t>, dim3(M), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL(distill_kernel<f16_t>, dim3(M), dim3(256), 0, st, g);
-    WFD_CHECK_LAUNCH();
-    return WFD_OK;
+    if (dtype == WFD_F32) return distill<float>(g, st);
+    return dtype == WFD_BF16 ? distill<bf16_t>(g, st) : distill<f16_t>(g, st);
 }
 
 }  // extern "C"

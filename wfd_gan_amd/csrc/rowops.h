@@ -12,6 +12,8 @@ typedef _Float16 f16_t;
 
 static inline bool wfd_dtype_ok(int t) { return t >= WFD_F32 && t <= WFD_F16; }
 
+__device__ __forceinline__ int cdiv_dev(int a, int b) { return (a + b - 1) / b; }
+
 template <class T> struct Pack { static constexpr int N = 16 / (int)sizeof(T); };   // elements of one 16-byte piece
 
 // Rows begin wherever their stride puts them (an odd width of 16-bit values leaves every second row off even a 4-byte border):
@@ -60,6 +62,12 @@ template <class T> __device__ __forceinline__ Raw16 pack(const float* f) {
         }
     }
     return r;
+}
+
+// Hides from the compiler that a packed piece has been unpacked before: it would otherwise keep the unpacked values of one
+// phase alive for the next, at twice the registers (and spills where a thread holds 16 pieces).
+__device__ __forceinline__ void keep_packed(Raw16& r) {
+    asm volatile("" : "+v"(r.v[0]), "+v"(r.v[1]), "+v"(r.v[2]), "+v"(r.v[3]));
 }
 
 // the raw pattern of `fill` in every element

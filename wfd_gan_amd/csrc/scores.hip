@@ -8,8 +8,6 @@
 
 namespace {
 
-__device__ __forceinline__ int cdiv_dev(int a, int b) { return (a + b - 1) / b; }
-
 struct Scores {
     const void* X;
     const int* labels;
