@@ -509,7 +509,7 @@ int wfd_layer_norm_bwd(const void* DY, int lddy, const void* X, int ldx, int dty
                        float* work, void* stream);
 int wfd_layer_norm_bwd_floats(int M, int N, int dtype);
 
-/* Scores over V classes (V <= 2^28) at a temperature > 0, p = softmax(x / T), in one pass over the logits:
+/* Scores over V classes (V <= 2^23) at a temperature > 0, p = softmax(x / T), in one pass over the logits:
  *   logprob[m] = ln p(labels[m]); a label < 0 is none (0), a label >= V a mistake (NaN)
  *   entropy[m] = -sum p ln p
  *   top_logprob / top_index [M][k]: the k (0 .. 64, <= V) largest logits in order, equal ones by lower index, NaN before all

@@ -136,7 +136,7 @@ def test_abi_refusals_and_empty_calls():
                                                    st=0).items()]
     for o in (dict(x=0), dict(ld=8), dict(dt=3), dict(V=0), dict(k=10), dict(k=65, V=100, ld=100), dict(k=-1), dict(T=0.0),
               dict(T=float("inf")), dict(T=float("nan")), dict(tl=0), dict(ti=0), dict(y=0), dict(M=-1), dict(x=P + 1),
-              dict(V=(1 << 28) + 1)):
+              dict(V=(1 << 23) + 1, ld=(1 << 23) + 1)):
         refused(L.label_scores, *sc(**o))
     L.label_scores(*sc(M=0, x=0))
     sb = lambda **o: [o.get(k, d) for k, d in dict(x=P, ld=9, dt=1, M=2, V=9, y=P, T=1.0, s=P, e=P, dl=P, dh=P, dx=P, lddx=9,

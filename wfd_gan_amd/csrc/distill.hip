@@ -76,6 +76,13 @@ struct RowSums {
     float m, s, s1;         // maximum (floored), sum exp((x - m) / T), sum exp(x - m)
 };
 
+template <bool TWO> __device__ __forceinline__ void sums_to(RowSums& a, float m, float c) {      // to a maximum m >= a.m
+    const float d = fmaxf(a.m - m, -1e30f);
+    a.s *= __builtin_amdgcn_exp2f(d * c);
+    if constexpr (TWO) a.s1 *= __builtin_amdgcn_exp2f(d * LOG2E);
+    a.m = m;
+}
+
 // the row's loss (every lane), from the entries and the sums
 template <int L>
 __device__ __forceinline__ float row_loss(const Distill& g, long row, int lane, const Entries& n, const Taught& t, const RowSums& s,
@@ -193,25 +200,32 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void distill_kernel(Distill g) {
         if constexpr (G > 64)
             if (t == 0) { told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f; }
     }
-    float m = -INFINITY;
+    // per thread about its own running maximum, four pieces at a time, while later pieces are still on their way
+    RowSums s{LOWEST, 0.f, 0.f};
+    constexpr int B = R < 4 ? R : 4;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        keep_packed(d[r]);
+    for (int r0 = 0; r0 < R; r0 += B) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; ++e) m = fmaxf(m, elem<T>(d[r], e));
-    }
-    RowSums s{fmaxf(team_max<G>(m, slot[0]), LOWEST), 0.f, 0.f};
-    if constexpr (G > 64) tt = Taught{told[0], told[1], told[2] != 0.f};
+        for (int r = r0; r < r0 + B; ++r) {
+            keep_packed(d[r]);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        keep_packed(d[r]);
+            for (int e = 0; e < E; ++e) top = fmaxf(top, elem<T>(d[r], e));
+        }
+        if (top > s.m) sums_to<TWO>(s, top, c);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float z = elem<T>(d[r], e) - s.m;
-            s.s += __builtin_amdgcn_exp2f(z * c);
-            if constexpr (TWO) s.s1 += __builtin_amdgcn_exp2f(z * LOG2E);
+        for (int r = r0; r < r0 + B; ++r) {
+            keep_packed(d[r]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float z = elem<T>(d[r], e) - s.m;
+                s.s += __builtin_amdgcn_exp2f(z * c);
+                if constexpr (TWO) s.s1 += __builtin_amdgcn_exp2f(z * LOG2E);
+            }
         }
     }
+    sums_to<TWO>(s, team_max<G>(s.m, slot[0]), c);
+    if constexpr (G > 64) tt = Taught{told[0], told[1], told[2] != 0.f};
     if constexpr (TWO) {
         const float2 q = team_sum2<G>(s.s, s.s1, slot[1]);
         s.s = q.x;
@@ -241,12 +255,6 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void distill_kernel(Distill g) {
 }
 
 // ---- rows split over workgroups -------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void sums_to(RowSums& a, float m, float c) {
-    const float d = fmaxf(a.m - m, -1e30f);
-    a.s *= __builtin_amdgcn_exp2f(d * c);
-    a.s1 *= __builtin_amdgcn_exp2f(d * LOG2E);
-    a.m = m;
-}
 constexpr int U = 4;
 template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_part_kernel(Distill g) {
     constexpr int E = Pack<T>::N, STEP = 256 * U * E;
@@ -272,7 +280,7 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_part
         for (int j = 0; j < U; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) top = fmaxf(top, elem<T>(d[j], e));
-        if (top > a.m) sums_to(a, top, c);
+        if (top > a.m) sums_to<TWO>(a, top, c);
 #pragma unroll
         for (int j = 0; j < U; ++j)
 #pragma unroll
@@ -283,7 +291,7 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_part
             }
     }
     const float m = team_max<256>(a.m, slot[0]);
-    sums_to(a, m, c);
+    sums_to<TWO>(a, m, c);
     const float2 q = team_sum2<256>(a.s, a.s1, slot[1]);
     if (t == 0) { w[3 * sp] = m; w[3 * sp + 1] = q.x; w[3 * sp + 2] = TWO ? q.y : q.x; }
     // the logits that the second launch needs by index, before a gradient in place could lie over them
@@ -326,7 +334,7 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_fini
         xy = w[3 * g.splits + MAX_ENTRIES];
         for (int j = t; j < g.K; j += 64) n.x[j] = w[3 * g.splits + j];
         tt = teacher<64>(g, row, t, n, c);
-        sums_to(s, lanes_max<64>(s.m), c);
+        sums_to<true>(s, lanes_max<64>(s.m), c);
         s.s = lanes_sum<64>(s.s);
         s.s1 = lanes_sum<64>(s.s1);
         if (t == 0) {
@@ -359,7 +367,7 @@ bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
     const uintptr_t align = dtype == WFD_F32 ? 3 : 1;
     return p && !((uintptr_t)p & align) && (M <= 1 || ld >= V);
 }
-constexpr int MAX_V = 1 << 28;
+constexpr int MAX_V = 1 << 23;
 int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
 
 // Rows stay in registers up to 1024 threads x 16 pieces; longer ones are split, and so are long ones of which there are too few to

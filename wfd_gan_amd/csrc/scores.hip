@@ -124,18 +124,19 @@ __device__ __forceinline__ void row_store(const Scores& g, long row, const RowEn
 // ---- alternatives of a part of a row --------------------------------------------------------------------------------------
 // Every thread has left the largest value of each group of pieces that it visited in LDS.  The (k / waves)-th largest thread
 // maximum of a wave, the smallest such of all waves, is a value that at least k elements reach (tau).  Only groups whose maximum
-// reaches tau are read again; what reaches tau there goes to a list (expected length: k and a few), whose order is found by
-// counting.  When more elements than the list holds reach tau, they are ties at tau but for a few: those above tau are listed and the
+// reaches tau are read again, an element per thread; what reaches tau there goes to a list (expected length: k and a few), whose
+// order is found by counting.  When more than the lists hold reach tau, they are ties at tau but for a few: those above tau are listed and the
 // rest is filled up by walking the ties in index order.  Rows with NaN, and rows that defeat even this (thousands above
 // tau), take the k largest one after another.
-constexpr int CAND = 1024;
+constexpr int CAND = 1024, GROUPS = 512;
 constexpr int U = 4;                      // pieces per group
 
 template <int NT> struct PickLds {
     unsigned long long key[CAND];
     unsigned long long best[NT / 64 ? NT / 64 : 1];
     float tau[NT / 64 ? NT / 64 : 1];
-    int count, run[NT / 64 ? NT / 64 : 1];
+    int group[GROUPS];
+    int groups, count, run[NT / 64 ? NT / 64 : 1];
 };
 
 template <int NT> __device__ __forceinline__ void team_sync() {
@@ -158,19 +159,24 @@ template <int NT> __device__ __forceinline__ unsigned long long team_max_key(uns
     return v;
 }
 
-// the n-th largest (n >= 1) of the 64 lanes' values (no NaN): how many lanes are above each lane's value
+// the n-th largest (1 <= n <= 64) of the lanes' values (no NaN): a lane's value divides the lanes that are still in question, the
+// masks and counts are scalar work
 __device__ __forceinline__ float lanes_nth(float v, int n) {
-    int above = 0, same = 0;
-    const int me = threadIdx.x & 63;
-#pragma unroll 8
-    for (int i = 0; i < 64; ++i) {
-        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
-        above += w > v;
-        same += (w == v) & (i < me);
+    unsigned long long in = ~0ull;
+    for (;;) {
+        const int src = __ffsll((long long)in) - 1;
+        const float p = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), src));
+        const unsigned long long gt = __ballot(v > p) & in, eq = __ballot(v == p) & in;
+        const int above = __popcll(gt), same = __popcll(eq);
+        if (n <= above) {
+            in = gt;
+        } else if (n <= above + same) {
+            return p;
+        } else {
+            n -= above + same;
+            in &= ~(gt | eq);
+        }
     }
-    const unsigned long long hit = __ballot(above + same == n - 1);
-    const int src = __ffsll((long long)hit) - 1;
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), src));
 }
 
 // Leaves the k best of x[0, n) (indices from `base`) at out_val / out_idx in order, places without an element as index -1.
@@ -184,7 +190,7 @@ __device__ __forceinline__ void pick(const T* x, int n, int base, int k, int nit
     if (!slow) {
         const float mine = lanes_nth(tmax, (k + W - 1) / W);
         if (lane == 0) l.tau[wave] = mine;
-        if (t == 0) l.count = 0;
+        if (t == 0) l.count = l.groups = 0;
         team_sync<NT>();
         float tau = l.tau[0];
 #pragma unroll
@@ -195,29 +201,31 @@ __device__ __forceinline__ void pick(const T* x, int n, int base, int k, int nit
             for (int it = 0; it < niter; ++it) {
                 const float gm = gmax[it * NT + t];
                 if (pass ? gm > tau : gm >= tau) {
-#pragma unroll
-                    for (int j = 0; j < U; ++j) {
-                        const long i0 = ((long)(it * U + j) * NT + t) * E;
-                        if (i0 >= n) continue;
-                        const Raw16 d = load_piece(x, (int)i0, n, -INFINITY);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) {
-                            const float f = elem<T>(d, e);
-                            if ((pass ? f > tau : f >= tau) && i0 + e < n) {
-                                const int at = atomicAdd(&l.count, 1);
-                                if (at < CAND) l.key[at] = order_key(f, base + (int)i0 + e);
-                            }
-                        }
-                    }
+                    const int at = atomicAdd(&l.groups, 1);
+                    if (at < GROUPS) l.group[at] = it * NT + t;
                 }
             }
             team_sync<NT>();
+            const int groups = l.groups;
+            // an element per thread, so that the few groups keep all lanes busy
+            if (groups <= GROUPS)
+                for (int a = t; a < groups * U * E; a += NT) {
+                    const int id = l.group[a / (U * E)], j = a / E % U, e = a % E;
+                    const int i = ((id / NT * U + j) * NT + id % NT) * E + e;
+                    if (i >= n) continue;
+                    const float f = to_f32(x[i]);
+                    if (pass ? f > tau : f >= tau) {
+                        const int at = atomicAdd(&l.count, 1);
+                        if (at < CAND) l.key[at] = order_key(f, base + i);
+                    }
+                }
+            team_sync<NT>();
             total = l.count;
             team_sync<NT>();
-            if (total <= CAND) break;
+            if (groups <= GROUPS && total <= CAND) break;
             if (pass == 0) {
                 ties = true;
-                if (t == 0) l.count = 0;
+                if (t == 0) l.count = l.groups = 0;
                 team_sync<NT>();
             } else {
                 slow = true;
@@ -319,15 +327,28 @@ __device__ __forceinline__ Stat walk(const T* x, int n, float c, float* gmax, fl
         take(d);
     }
     if ((long)it * STEP < n) {
-        Raw16 d[U];
-#pragma unroll
+        // the rest, piece by piece as far as any lane of the wave has one
+        float group = -INFINITY;
+        const int first = (t & ~63) * E;
         for (int j = 0; j < U; ++j) {
             const long i0 = (long)it * STEP + (j * NT + t) * E;
-            const unsigned none = raw_fill<T>(-INFINITY);
-            d[j] = Raw16{{none, none, none, none}};
-            if (i0 < n) d[j] = load_piece(x, (int)i0, n, -INFINITY);
+            if ((long)it * STEP + j * NT * E + first >= n) break;
+            float f[E], top = -INFINITY;
+            if (i0 < n) {
+                const Raw16 d = load_piece(x, (int)i0, n, -INFINITY);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    f[e] = elem<T>(d, e);
+                    top = fmaxf(top, f[e]);
+                }
+                stat_add(a, f, top, c);
+                group = fmaxf(group, top);
+            }
         }
-        take(d);
+        if constexpr (PICK) {
+            gmax[it * NT + t] = group;
+            tmax = fmaxf(tmax, group);
+        }
     }
     return a;
 }
@@ -367,45 +388,43 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
     }
 }
 
-// the parts of a row: statistics in part order, alternatives from the parts' lists
+// the parts of a row: a lane per part for the statistics, alternatives from the parts' lists
+__device__ __forceinline__ float order_value(unsigned b) {
+    return b == 0xffffffffu ? NAN : __uint_as_float((b & 0x80000000u) ? b ^ 0x80000000u : ~b);
+}
 template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Scores g) {
     extern __shared__ unsigned long long keys[];              // splits * k
     __shared__ unsigned long long list[CAND];
     __shared__ unsigned long long slot[4];
     __shared__ int count;
     const long row = blockIdx.x;
-    const int t = threadIdx.x, S = g.splits, k = g.k;
-    const T* x = (const T*)g.X + row * g.ld;
-    const int y = g.labels ? g.labels[row] : -1;
-    const float xy = y >= 0 && y < g.V ? to_f32(x[y]) : 0.f;
-    const float* w = g.work + row * S * (3 + 2 * k);
-    const float c = g.inv_t * LOG2E;
-    Stat a{LOWEST, 0.f, 0.f};
-    for (int i = 0; i < S; ++i) a.m = fmaxf(a.m, w[(long)i * (3 + 2 * k)]);
-    for (int i = 0; i < S; ++i) {
-        const float* p = w + (long)i * (3 + 2 * k);
-        Stat b{p[0], p[1], p[2]};
-        stat_to(b, a.m, c);
-        a.s += b.s;
-        a.u += b.u;
-    }
-    const RowEnd r = row_end(a);
-    if (t == 0) row_store(g, row, r, xy, y);
-    if (k == 0) return;
+    const int t = threadIdx.x, S = g.splits, k = g.k, each = 3 + 2 * k;
+    const float* w = g.work + row * S * each;
     if (t == 0) count = 0;
     // a part's last entry, where its list is full, is reached by k elements: what is below the largest such is out
-    unsigned long long floor_ = 0;
+    unsigned long long least = 0;
     for (int i = t; i < S * k; i += 256) {
         const int s = i / k, j = i - s * k;
-        const float* p = w + (long)s * (3 + 2 * k) + 3;
+        const float* p = w + s * each + 3;
+        const float v = p[j];
         const int at = ((const int*)p)[k + j];
-        const unsigned long long key = at < 0 ? 0ull : order_key(p[j], at);
+        const unsigned long long key = at < 0 ? 0ull : order_key(v, at);
         keys[i] = key;
-        if (j == k - 1 && key > floor_) floor_ = key;
+        if (j == k - 1 && key > least) least = key;
     }
-    floor_ = team_max_key<256>(floor_, slot);
+    const int lane = t & 63;
+    const float c = g.inv_t * LOG2E;
+    Stat a{LOWEST, 0.f, 0.f};
+    if (lane < S) a = Stat{w[lane * each], w[lane * each + 1], w[lane * each + 2]};      // S <= 64
+    const RowEnd r = row_end(stat_team<64>(a, c, nullptr));
+    if (t == 255) {
+        const int y = g.labels ? g.labels[row] : -1;
+        row_store(g, row, r, y >= 0 && y < g.V ? to_f32(((const T*)g.X + row * g.ld)[y]) : 0.f, y);
+    }
+    if (k == 0) return;
+    least = team_max_key<256>(least, slot);
     for (int i = t; i < S * k; i += 256)
-        if (keys[i] >= floor_ && keys[i]) {
+        if (keys[i] >= least && keys[i]) {
             const int at = atomicAdd(&count, 1);
             if (at < CAND) list[at] = keys[i];
         }
@@ -419,9 +438,8 @@ template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Sco
         int rank = 0;
         for (int b = 0; b < n; ++b) rank += from[b] > key;
         if (rank < k) {
-            const int at = (int)~(unsigned)key;
-            g.top_idx[row * k + rank] = at;
-            g.top_lp[row * k + rank] = row_lp(r, to_f32(x[at]), g.inv_t);
+            g.top_idx[row * k + rank] = (int)~(unsigned)key;
+            g.top_lp[row * k + rank] = row_lp(r, order_value((unsigned)(key >> 32)), g.inv_t);
         }
     }
 }
@@ -559,12 +577,12 @@ bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
     const uintptr_t align = dtype == WFD_F32 ? 3 : 1;
     return p && !((uintptr_t)p & align) && (M <= 1 || ld >= V);
 }
-constexpr int MAX_V = 1 << 28, MAX_K = 64;
+constexpr int MAX_V = 1 << 23, MAX_K = 64;   // 64 parts of 32 fp32 steps
 int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
 
 // Few classes stay in the registers of a team inside a wave.  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192
-// 16-bit or 4096 fp32 classes); a row is split over workgroups while there are fewer than 1024 of them, and where its group maxima
-// would take more than 32 steps' room in LDS.
+// 16-bit or 4096 fp32 classes); a row is split over workgroups (64 at most) while there are fewer than 1024 of them, and where its
+// group maxima would take more than 32 steps' room in LDS.
 constexpr int FEW = 128;                  // lanes * pieces of the team form: up to 1024 16-bit or 512 fp32 classes
 constexpr int MOST_STEPS = 32;
 struct ScoresShape {
