@@ -13,8 +13,6 @@
 namespace {
 
 constexpr int MAX_ENTRIES = 256;
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr float LOWEST = -3.402823466e38f;       // floor of a maximum: x - m stays defined for rows of -inf
 
 struct Distill {
     const void* X;
@@ -61,7 +59,7 @@ template <int L> __device__ __forceinline__ Taught teacher(const Distill& g, lon
     }
     r.max = fmaxf(lanes_max<L>(r.max), LOWEST);
     for (int j = lane; j < K; j += L) {
-        n.e[j] = __builtin_amdgcn_exp2f((n.e[j] - r.max) * c);
+        n.e[j] = exp2_of((n.e[j] - r.max) * c);
         r.sum += n.e[j];
     }
     r.sum = lanes_sum<L>(r.sum);
@@ -78,9 +76,34 @@ struct RowSums {
 
 template <bool TWO> __device__ __forceinline__ void sums_to(RowSums& a, float m, float c) {      // to a maximum m >= a.m
     const float d = fmaxf(a.m - m, -1e30f);
-    a.s *= __builtin_amdgcn_exp2f(d * c);
-    if constexpr (TWO) a.s1 *= __builtin_amdgcn_exp2f(d * LOG2E);
+    a.s *= exp2_of(d * c);
+    if constexpr (TWO) a.s1 *= exp2_of(d * LOG2E);
     a.m = m;
+}
+
+// adds N elements whose maximum is `top`
+template <bool TWO, int N> __device__ __forceinline__ void sums_add(RowSums& a, const float (&f)[N], float top, float c) {
+    if (top > a.m) sums_to<TWO>(a, top, c);
+    const float R = a.m * c, R1 = a.m * LOG2E;
+    float s = 0.f, s1 = 0.f;
+    if (fabsf(R) < WIDE && (!TWO || fabsf(R1) < WIDE)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            s += exp2_of(fmaf(f[e], c, -R));
+            if constexpr (TWO) s1 += exp2_of(fmaf(f[e], LOG2E, -R1));
+        }
+        a.s = fmaf(exp2_of(-fmaf(a.m, c, -R)), s, a.s);
+        if constexpr (TWO) a.s1 = fmaf(exp2_of(-fmaf(a.m, LOG2E, -R1)), s1, a.s1);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float z = f[e] - a.m;
+            s += exp2_of(z * c);
+            if constexpr (TWO) s1 += exp2_of(z * LOG2E);
+        }
+        a.s += s;
+        if constexpr (TWO) a.s1 += s1;
+    }
 }
 
 // the row's loss (every lane), from the entries and the sums
@@ -109,8 +132,11 @@ __device__ __forceinline__ float row_loss(const Distill& g, long row, int lane, 
 // what a gradient element is made of: d = cw exp((x - m) / T) + cu exp(x - m), less the targets at the entries and the label
 struct GradRow {
     float m, cw, cu, r, rt;        // r = grad_scale * row_scale, rt = r w T / (sum of the teacher's exponentials)
+    float R, R1, kw, ku;           // m c and m log2(e) rounded, cw and cu with what the rounding left
+    bool wide;                     // m c leaves fp32's range
 };
-__device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Taught& t, const RowSums& s, int y, bool wrong) {
+template <bool TWO>
+__device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Taught& t, const RowSums& s, int y, bool wrong, float c) {
     GradRow d;
     d.m = s.m;
     d.r = g.scale * (g.row_scale ? g.row_scale[row] : 1.f);
@@ -120,19 +146,37 @@ __device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Ta
     d.cw = on ? d.r * g.w * g.temp / s.s : 0.f;
     d.cu = y >= 0 ? d.r * g.u / s.s1 : 0.f;
     if (empty) d.cw = d.cu = wrong ? NAN : 0.f;
+    if constexpr (!TWO) d.cw += d.cu;
+    d.R = d.m * c;
+    d.R1 = d.m * LOG2E;
+    d.wide = !(fabsf(d.R) < WIDE && fabsf(d.R1) < WIDE);
+    d.kw = d.cw * exp2_of(-fmaf(d.m, c, -d.R));
+    d.ku = d.cu * exp2_of(-fmaf(d.m, LOG2E, -d.R1));
     return d;
 }
+template <bool TWO> __device__ __forceinline__ float grad_dense(const GradRow& d, float x, float c) {
+    if (!d.wide) {
+        const float v = d.kw * exp2_of(fmaf(x, c, -d.R));
+        return TWO ? fmaf(d.ku, exp2_of(fmaf(x, LOG2E, -d.R1)), v) : v;
+    }
+    const float v = d.cw * exp2_of((x - d.m) * c);
+    return TWO ? fmaf(d.cu, exp2_of((x - d.m) * LOG2E), v) : v;
+}
 template <class T, bool TWO>
-__device__ __forceinline__ void grad_piece(const GradRow& d, const Raw16& p, T* o, int i0, int V, float c) {
+__device__ __forceinline__ void grad_piece(const GradRow& d, const Raw16& p, T* o, float c) {
     constexpr int E = Pack<T>::N;
     float f[E];
+    if (!d.wide) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float z = elem<T>(p, e) - d.m;
-        f[e] = d.cw * __builtin_amdgcn_exp2f(z * c);
-        if constexpr (TWO) f[e] = fmaf(d.cu, __builtin_amdgcn_exp2f(z * LOG2E), f[e]);
+        for (int e = 0; e < E; ++e) {
+            f[e] = d.kw * exp2_of(fmaf(elem<T>(p, e), c, -d.R));
+            if constexpr (TWO) f[e] = fmaf(d.ku, exp2_of(fmaf(elem<T>(p, e), LOG2E, -d.R1)), f[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = grad_dense<TWO>(d, elem<T>(p, e), c);
     }
-    store_piece(o, i0, V, f);
+    store16(o, pack<T>(f));
 }
 // the elements with a target, whole again: the first occurrence of an index subtracts all of its entries, the label its own.
 // Only those of [lo, hi); runs after a barrier behind the stores that it overwrites.
@@ -140,12 +184,6 @@ template <class T, bool TWO, int L>
 __device__ __forceinline__ void grad_targets(const Distill& g, const GradRow& d, const Entries& n, bool empty, int lane, T* o, int lo,
                                              int hi, int y, float xy, float c) {
     if (empty) return;
-    auto dense = [&](float x) {
-        const float z = x - d.m;
-        float v = d.cw * __builtin_amdgcn_exp2f(z * c);
-        if constexpr (TWO) v = fmaf(d.cu, __builtin_amdgcn_exp2f(z * LOG2E), v);
-        return v;
-    };
     bool label_seen = false;
     for (int j = lane; j < g.K; j += L) {
         const int at = n.at[j];
@@ -159,105 +197,129 @@ __device__ __forceinline__ void grad_targets(const Distill& g, const GradRow& d,
             }
         if (at == y) label_seen = true;
         if (first) {
-            float v = dense(n.x[j]) - d.rt * sum;
+            float v = grad_dense<TWO>(d, n.x[j], c) - d.rt * sum;
             if (at == y) v -= d.r * g.u;
             o[at] = from_f32<T>(v);
         }
     }
     const bool seen = lanes_max<L>(label_seen ? 1.f : 0.f) != 0.f;
-    if (lane == 0 && !seen && y >= lo && y < hi && y < g.V) o[y] = from_f32<T>(dense(xy) - d.r * g.u);
+    if (lane == 0 && !seen && y >= lo && y < hi && y < g.V) o[y] = from_f32<T>(grad_dense<TWO>(d, xy, c) - d.r * g.u);
 }
 
 // ---- a row in the registers of a team of G threads ----------------------------------------------------------------------------
 // TWO: a label is mixed in at a temperature other than 1, so two sums of exponentials are kept.  Without, every exponential serves both
 // terms and cu joins cw.
-template <class T, int G, int R, bool TWO>
+// Workgroups of one row walk rows gridDim.x apart: a piece's registers take the next row's load as soon as its gradient is on its way
+// out, so that memory has work while the arithmetic of a row runs (a long row fills the CU's registers: there is no second workgroup
+// to do that).
+template <class T, int G, int R, bool TWO, bool GRAD>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void distill_kernel(Distill g) {
-    constexpr int E = Pack<T>::N, TEAMS = G < 256 ? 256 / G : 1, L = G < 64 ? G : 64;
+    constexpr int E = Pack<T>::N, TEAMS = G < 256 ? 256 / G : 1, L = G < 64 ? G : 64, B = R < 4 ? R : 4;
     extern __shared__ float lds[];
     __shared__ float slot[2][2 * (G > 64 ? G / 64 : 1)], told[8];
-    const int t = threadIdx.x % G, team = threadIdx.x / G, V = g.V;
-    const long row = (long)blockIdx.x * TEAMS + team;
+    const int t = TEAMS > 1 ? threadIdx.x % G : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / G : 0, V = g.V;
+    int row = blockIdx.x * TEAMS + team;
     if (row >= g.M) return;                                   // whole teams, each inside a wave
-    const T* x = (const T*)g.X + row * g.ld;
     const float inv_t = 1.f / g.temp, c = inv_t * LOG2E;
-    Raw16 d[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int i0 = (r * G + t) * E;
-        const unsigned none = raw_fill<T>(-INFINITY);
-        d[r] = Raw16{{none, none, none, none}};
-        if (i0 < V) d[r] = load_piece(x, i0, V, -INFINITY);
-    }
     const Entries n = entries_in(lds + team * 3 * g.K, g.K);
-    const int y = g.u != 0.f ? g.labels[row] : -1;
-    const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
-    Taught tt{LOWEST, 0.f, false};
-    if (t < L) {
-        tt = teacher<L>(g, row, t, n, c);
-        wave_sync();
-        entries_gather<T, L>(x, g.K, t, n);
-        if constexpr (G > 64)
-            if (t == 0) { told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f; }
-    }
-    // per thread about its own running maximum, four pieces at a time, while later pieces are still on their way
-    RowSums s{LOWEST, 0.f, 0.f};
-    constexpr int B = R < 4 ? R : 4;
+    // piece r * G + t of V / E whole ones; the V % E elements behind them go to the first threads
+    const int P = V / E, rest = V - P * E;
+    const unsigned lane_off = (unsigned)t * E;
+    Raw16 d[R];
+    float tail = -INFINITY;
+    auto fetch = [&](int r, const T* x) {
+        if (r * G + t < P) d[r] = load16(x + r * G * E + lane_off);
+    };
+    const unsigned none = raw_fill<T>(-INFINITY);
+    {
+        const T* x = (const T*)g.X + (long)row * g.ld;
 #pragma unroll
-    for (int r0 = 0; r0 < R; r0 += B) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int r = r0; r < r0 + B; ++r) {
-            keep_packed(d[r]);
-#pragma unroll
-            for (int e = 0; e < E; ++e) top = fmaxf(top, elem<T>(d[r], e));
+        for (int r = 0; r < R; ++r) {
+            d[r] = Raw16{{none, none, none, none}};
+            fetch(r, x);
         }
-        if (top > s.m) sums_to<TWO>(s, top, c);
+        if (t < rest) tail = to_f32(x[P * E + t]);
+    }
+    for (;;) {
+        const T* x = (const T*)g.X + (long)row * g.ld;
+        const long next = (long)row + gridDim.x;
+        const bool more = G > 64 && next < g.M;
+        const T* xn = x + (long)gridDim.x * g.ld;
+        const int y = g.u != 0.f ? g.labels[row] : -1;
+        const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
+        Taught tt{LOWEST, 0.f, false};
+        if (t < L) {
+            tt = teacher<L>(g, row, t, n, c);
+            wave_sync();
+            entries_gather<T, L>(x, g.K, t, n);
+            if constexpr (G > 64)
+                if (t == 0) { told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f; }
+        }
+        // per thread about its own running maximum, four pieces at a time, while later pieces are still on their way
+        RowSums s{LOWEST, 0.f, 0.f};
 #pragma unroll
-        for (int r = r0; r < r0 + B; ++r) {
-            keep_packed(d[r]);
+        for (int r0 = 0; r0 < R; r0 += B) {
+            float f[B * E], top = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float z = elem<T>(d[r], e) - s.m;
-                s.s += __builtin_amdgcn_exp2f(z * c);
-                if constexpr (TWO) s.s1 += __builtin_amdgcn_exp2f(z * LOG2E);
+            for (int r = 0; r < B; ++r) {
+                keep_packed(d[r0 + r]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    f[r * E + e] = elem<T>(d[r0 + r], e);
+                    top = fmaxf(top, f[r * E + e]);
+                }
             }
+            sums_add<TWO>(s, f, top, c);
         }
-    }
-    sums_to<TWO>(s, team_max<G>(s.m, slot[0]), c);
-    if constexpr (G > 64) tt = Taught{told[0], told[1], told[2] != 0.f};
-    if constexpr (TWO) {
-        const float2 q = team_sum2<G>(s.s, s.s1, slot[1]);
-        s.s = q.x;
-        s.s1 = q.y;
-    } else {
-        s.s1 = s.s = team_sum<G>(s.s, slot[1]);
-    }
-    const bool wrong = tt.wrong || y >= V;
-    if (t < L) {
-        wave_sync();
-        const float loss = row_loss<L>(g, row, t, n, tt, s, inv_t, y, xy, wrong);
-        if (t == 0) g.loss[row] = loss;
-    }
-    if (!g.DX) return;
-    GradRow k = grad_row(g, row, tt, s, y, wrong);
-    if constexpr (!TWO) k.cw += k.cu;
-    T* o = (T*)g.DX + row * g.lddx;
+        if (rest) {
+            const float f[1] = {tail};
+            sums_add<TWO>(s, f, tail, c);
+        }
+        sums_to<TWO>(s, team_max<G>(s.m, slot[0]), c);
+        if constexpr (G > 64) tt = Taught{told[0], told[1], told[2] != 0.f};
+        if constexpr (TWO) {
+            const float2 q = team_sum2<G>(s.s, s.s1, slot[1]);
+            s.s = q.x;
+            s.s1 = q.y;
+        } else {
+            s.s1 = s.s = team_sum<G>(s.s, slot[1]);
+        }
+        const bool wrong = tt.wrong || y >= V;
+        if (t < L) {
+            wave_sync();
+            const float loss = row_loss<L>(g, row, t, n, tt, s, inv_t, y, xy, wrong);
+            if (t == 0) g.loss[row] = loss;
+        }
+        if constexpr (GRAD) {
+            const GradRow k = grad_row<TWO>(g, row, tt, s, y, wrong, c);
+            T* o = (T*)g.DX + (long)row * g.lddx;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int i0 = (r * G + t) * E;
-        keep_packed(d[r]);
-        if (i0 < V) grad_piece<T, TWO>(k, d[r], o, i0, V, c);
+            for (int r = 0; r < R; ++r) {
+                keep_packed(d[r]);
+                if (r * G + t < P) grad_piece<T, TWO>(k, d[r], o + r * G * E + lane_off, c);
+                if (more) fetch(r, xn);
+            }
+            if (t < rest) o[P * E + t] = from_f32<T>(grad_dense<TWO>(k, tail, c));
+            if constexpr (G > 64) __syncthreads();
+            else wave_sync();
+            if (t < L) grad_targets<T, TWO, L>(g, k, n, s.s == 0.f, t, o, 0, V, y, xy, c);
+        } else if constexpr (G > 64) {
+            if (more)
+#pragma unroll
+                for (int r = 0; r < R; ++r) fetch(r, xn);
+            __syncthreads();                                  // the next row's entries and sums go where this row's were
+        }
+        if constexpr (G <= 64) return;
+        if (!more) return;
+        if (t < rest) tail = to_f32(xn[P * E + t]);
+        row = (int)next;
     }
-    if constexpr (G > 64) __syncthreads();
-    else wave_sync();
-    if (t < L) grad_targets<T, TWO, L>(g, k, n, s.s == 0.f, t, o, 0, V, y, xy, c);
 }
 
 // ---- rows split over workgroups -------------------------------------------------------------------------------------------------
 constexpr int U = 4;
 template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_part_kernel(Distill g) {
-    constexpr int E = Pack<T>::N, STEP = 256 * U * E;
+    constexpr int E = Pack<T>::N;
     __shared__ float slot[3][8];
     const long row = blockIdx.x / g.splits;
     const int sp = (int)(blockIdx.x - row * g.splits), t = threadIdx.x;
@@ -266,29 +328,28 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_part
     float* w = g.work + row * (3L * g.splits + MAX_ENTRIES + 1);
     const float c = LOG2E / g.temp;
     RowSums a{LOWEST, 0.f, 0.f};
-    for (long b = 0; b < n; b += STEP) {
+    const int P = n / E, rest = n - P * E;
+    const unsigned none = raw_fill<T>(-INFINITY);
+    for (int p0 = 0; p0 < P; p0 += 256 * U) {
         Raw16 d[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const long i0 = b + (j * 256 + t) * E;
-            const unsigned none = raw_fill<T>(-INFINITY);
             d[j] = Raw16{{none, none, none, none}};
-            if (i0 < n) d[j] = load_piece(x + lo, (int)i0, n, -INFINITY);
+            if (p0 + j * 256 + t < P) d[j] = load16(x + lo + (long)(p0 + j * 256 + t) * E);
         }
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-#pragma unroll
-            for (int e = 0; e < E; ++e) top = fmaxf(top, elem<T>(d[j], e));
-        if (top > a.m) sums_to<TWO>(a, top, c);
+        float f[U * E], top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < U; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float z = elem<T>(d[j], e) - a.m;
-                a.s += __builtin_amdgcn_exp2f(z * c);
-                if constexpr (TWO) a.s1 += __builtin_amdgcn_exp2f(z * LOG2E);
+                f[j * E + e] = elem<T>(d[j], e);
+                top = fmaxf(top, f[j * E + e]);
             }
+        sums_add<TWO>(a, f, top, c);
+    }
+    if (t < rest) {
+        const float f[1] = {to_f32(x[lo + P * E + t])};
+        sums_add<TWO>(a, f, f[0], c);
     }
     const float m = team_max<256>(a.m, slot[0]);
     sums_to<TWO>(a, m, c);
@@ -319,12 +380,15 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_fini
     const Entries n = entries_in(lds, g.K);
     const int y = g.u != 0.f ? g.labels[row] : -1;
     Raw16 d[U];
-    if (g.DX)
+    // this workgroup's whole pieces, and one of the elements behind the last of them
+    const int hi = min(lo + STEP, V), P = (hi - lo) / E, rest = hi - lo - P * E;
+    float tail = 0.f;
+    if (g.DX) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int i0 = lo + (j * 256 + t) * E;
-            if (i0 < V) d[j] = load_piece(x, i0, V, -INFINITY);
-        }
+        for (int j = 0; j < U; ++j)
+            if (j * 256 + t < P) d[j] = load16(x + lo + (j * 256 + t) * E);
+        if (t < rest) tail = to_f32(x[lo + P * E + t]);
+    }
     float xy = 0.f;
     Taught tt{LOWEST, 0.f, false};
     RowSums s{LOWEST, 0.f, 0.f};
@@ -351,16 +415,14 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_fini
     __syncthreads();
     tt = Taught{told[0], told[1], told[2] != 0.f};
     s = RowSums{told[3], told[4], told[5]};
-    GradRow k = grad_row(g, row, tt, s, y, tt.wrong || y >= V);
-    if constexpr (!TWO) k.cw += k.cu;
+    const GradRow k = grad_row<TWO>(g, row, tt, s, y, tt.wrong || y >= V, c);
     T* o = (T*)g.DX + row * g.lddx;
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-        const int i0 = lo + (j * 256 + t) * E;
-        if (i0 < V) grad_piece<T, TWO>(k, d[j], o, i0, V, c);
-    }
+    for (int j = 0; j < U; ++j)
+        if (j * 256 + t < P) grad_piece<T, TWO>(k, d[j], o + lo + (j * 256 + t) * E, c);
+    if (t < rest) o[lo + P * E + t] = from_f32<T>(grad_dense<TWO>(k, tail, c));
     __syncthreads();
-    if (t < 64) grad_targets<T, TWO, 64>(g, k, n, s.s == 0.f, t, o, lo, min(lo + STEP, V), y, xy, c);
+    if (t < 64) grad_targets<T, TWO, 64>(g, k, n, s.s == 0.f, t, o, lo, hi, y, xy, c);
 }
 
 bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
@@ -386,7 +448,7 @@ DistillShape distill_shape(int M, int V, int dtype) {
     return {cdiv(steps, each), each * step};
 }
 
-template <class T, bool TWO> int distill(Distill g, hipStream_t st) {
+template <class T, bool TWO, bool GRAD> int distill(Distill g, hipStream_t st) {
     constexpr int E = Pack<T>::N;
     const DistillShape s = distill_shape(g.M, g.V, sizeof(T) == 4 ? WFD_F32 : WFD_BF16);
     g.splits = s.splits;
@@ -395,7 +457,8 @@ template <class T, bool TWO> int distill(Distill g, hipStream_t st) {
 #define WFD_GO(G, R)                                                                                                     \
     if (g.V <= G * R * E) {                                                                                              \
         constexpr int TEAMS = G < 256 ? 256 / G : 1;                                                                     \
-        hipLaunchKernelGGL((distill_kernel<T, G, R, TWO>), dim3(cdiv(g.M, TEAMS)), dim3(G < 256 ? 256 : G),              \
+        const int blocks = cdiv(g.M, TEAMS), most = G > 64 ? 256 * (16 / R) * (1024 / G) : blocks;                       \
+        hipLaunchKernelGGL((distill_kernel<T, G, R, TWO, GRAD>), dim3(blocks < most ? blocks : most), dim3(G < 256 ? 256 : G), \
                            (size_t)TEAMS * 3 * g.K * 4, st, g);                                                          \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
@@ -413,7 +476,8 @@ template <class T, bool TWO> int distill(Distill g, hipStream_t st) {
     return WFD_OK;
 }
 template <class T> int distill(const Distill& g, hipStream_t st) {
-    return g.temp != 1.f && g.u != 0.f ? distill<T, true>(g, st) : distill<T, false>(g, st);
+    if (g.temp != 1.f && g.u != 0.f) return g.DX ? distill<T, true, true>(g, st) : distill<T, true, false>(g, st);
+    return g.DX ? distill<T, false, true>(g, st) : distill<T, false, false>(g, st);
 }
 
 }  // namespace

@@ -17,8 +17,8 @@ __device__ __forceinline__ int cdiv_dev(int a, int b) { return (a + b - 1) / b; 
 template <class T> struct Pack { static constexpr int N = 16 / (int)sizeof(T); };   // elements of one 16-byte piece
 
 // Rows begin wherever their stride puts them (an odd width of 16-bit values leaves every second row off even a 4-byte border):
-// gfx950 serves 16-byte accesses at any address, so pieces are counted from the row's first element, unaligned, and only the
-// last, partial one is taken element by element.
+// gfx950 serves 16-byte accesses at any address, so pieces are counted from the row's first element, unaligned.  The n % N elements
+// behind the last whole piece go one to a thread.
 struct __attribute__((packed, aligned(2))) Raw16u { unsigned v[4]; };
 struct Raw16 { unsigned v[4]; };
 
@@ -42,10 +42,8 @@ template <> __device__ __forceinline__ float elem<bf16_t>(const Raw16& r, int e)
     return __uint_as_float((e & 1) ? (r.v[e >> 1] & 0xffff0000u) : (r.v[e >> 1] << 16));
 }
 template <> __device__ __forceinline__ float elem<f16_t>(const Raw16& r, int e) {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    h2 h;
-    __builtin_memcpy(&h, &r.v[e >> 1], 4);
-    return (float)h[e & 1];
+    const unsigned short h = (unsigned short)((e & 1) ? r.v[e >> 1] >> 16 : r.v[e >> 1] & 0xffffu);
+    return (float)__builtin_bit_cast(_Float16, h);
 }
 
 template <class T> __device__ __forceinline__ Raw16 pack(const float* f) {
@@ -169,3 +167,14 @@ template <int G> __device__ __forceinline__ float team_max(float a, float* slot)
     }
     return a;
 }
+
+// ---- sums of exponentials about a maximum --------------------------------------------------------------------------------
+// exp((x - m) / T) = 2^(x c - m c), c = log2(e) / T.  Per element that is one fused multiply-add with the rounded R = m c and one
+// exp2; what R's rounding leaves (m c - R, exact by fma) is taken out of a whole group's sum at once, so the sums are about the true
+// maximum however large it is.  Where m c leaves fp32's range (rows at the type's lowest value) the difference comes first.
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOWEST = -3.402823466e38f;       // floor of a maximum: x - m stays defined for rows of nothing but -inf
+constexpr float FAINT = -1e4f;                   // an exponent whose exponential is 0: stands in where 0 * -inf would be NaN
+constexpr float WIDE = 1e38f;
+
+__device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }

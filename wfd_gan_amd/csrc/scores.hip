@@ -49,27 +49,38 @@ __device__ __forceinline__ unsigned long long order_key(float v, int i) {
 // c = log2(e) / T.  The floor under m keeps x - m defined for rows of -inf (their s stays 0, which is how they are told) and for
 // rows at the type's lowest value (x - m = 0).  exp2 of -inf is 0, and u takes no exponent below FAINT, so masked classes add
 // nothing; NaN and +inf reach s as NaN.
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr float LOWEST = -3.402823466e38f;
-constexpr float FAINT = -1e4f;            // an exponent whose exponential is 0: stands in where 0 * -inf would be NaN
-
 struct Stat {
     float m, s, u;
 };
 __device__ __forceinline__ void stat_to(Stat& a, float m, float c) {          // moves a to a maximum m >= a.m
-    const float d = fmaxf(a.m - m, -1e30f) * c, w = __builtin_amdgcn_exp2f(d);
+    const float d = fmaxf(a.m - m, -1e30f) * c, w = exp2_of(d);
     a.u = w * fmaf(a.s, d, a.u);
     a.s *= w;
     a.m = m;
 }
 template <int N> __device__ __forceinline__ void stat_add(Stat& a, const float (&f)[N], float top, float c) {
     if (top > a.m) stat_to(a, top, c);
+    const float R = a.m * c;
+    float s = 0.f, u = 0.f, rest = 0.f;
+    if (fabsf(R) < WIDE) {
+        rest = fmaf(a.m, c, -R);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const float d = (f[e] - a.m) * c, w = __builtin_amdgcn_exp2f(d);
-        a.s += w;
-        a.u = fmaf(w, fmaxf(d, FAINT), a.u);
+        for (int e = 0; e < N; ++e) {
+            const float d = fmaf(f[e], c, -R), w = exp2_of(d);
+            s += w;
+            u = fmaf(w, fmaxf(d, FAINT), u);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float d = (f[e] - a.m) * c, w = exp2_of(d);
+            s += w;
+            u = fmaf(w, fmaxf(d, FAINT), u);
+        }
     }
+    const float w = exp2_of(-rest);
+    a.u = fmaf(w, fmaf(-rest, s, u), a.u);
+    a.s = fmaf(w, s, a.s);
 }
 // over a team of G threads; slot: 3 * G / 64 floats of LDS.  Every thread gets the sum, added in a fixed order.
 template <int G> __device__ __forceinline__ Stat stat_team(Stat a, float c, float* slot) {
@@ -530,7 +541,7 @@ template <class T> __device__ __forceinline__ void bwd_piece(const ScoresBwd& g,
     float f[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const float lp = fmaf(elem<T>(d, e) - r.m, g.inv_t, -r.log_s), p = __builtin_amdgcn_exp2f(lp * LOG2E);
+        const float lp = fmaf(elem<T>(d, e) - r.m, g.inv_t, -r.log_s), p = exp2_of(lp * LOG2E);
         f[e] = -p * fmaf(r.q1, fmaxf(lp, FAINT), r.q0);
     }
     if (r.y >= i0 && r.y < i0 + E)
