@@ -26,86 +26,123 @@ struct LnBwd {
     const float* rstd;
     void* DX;
     float* part;       // [blocks][2][N]: each workgroup's sums of dy xh and dy
+    void* dw;          // where a single workgroup leaves them
+    void* db;
     int lddy, ldx, lddx, M, N;
 };
 
-template <class WT, int E> __device__ __forceinline__ void load_weights(float* f, const WT* w, int i0, int n, float none) {
+// E weights from i0 (all inside the row)
+template <class WT, int E> __device__ __forceinline__ void load_weights(float* f, const WT* w, int i0, float none) {
+    constexpr int P = Pack<WT>::N < E ? Pack<WT>::N : E;
+    if (!w) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = none;
-    if (!w) return;
-    constexpr int P = Pack<WT>::N;
-    if (i0 + E <= n) {
-        if constexpr (P >= E) {
-            const Raw16 r = load16(w + i0);
+        for (int e = 0; e < E; ++e) f[e] = none;
+        return;
+    }
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = elem<WT>(r, e);
-        } else {
+    for (int h = 0; h < E / P; ++h) {
+        const Raw16 r = load16(w + i0 + h * P);
 #pragma unroll
-            for (int h = 0; h < E / P; ++h) {
-                const Raw16 r = load16(w + i0 + h * P);
-#pragma unroll
-                for (int e = 0; e < P; ++e) f[h * P + e] = elem<WT>(r, e);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (i0 + e < n) f[e] = to_f32(w[i0 + e]);
+        for (int e = 0; e < P; ++e) f[h * P + e] = elem<WT>(r, e);
     }
 }
 
 // ---- forward: a team of G threads per row, R pieces per thread in registers -----------------------------------------
+// A team takes rows as many apart as there are teams, with the next row's loads behind it and its weights in registers: reading
+// 2 N weights again for every row cost the L1's address path as much as the row itself.
 template <class T, class WT, int G, int R>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void ln_fwd_kernel(LnFwd g) {
     constexpr int E = Pack<T>::N, TEAMS = G < 256 ? 256 / G : 1;
-    __shared__ float slot[2][G > 64 ? G / 64 : 1];
-    const int t = threadIdx.x % G;
-    const long row = (long)blockIdx.x * TEAMS + threadIdx.x / G;
-    if (row >= g.M) return;                              // whole teams; only teams of at most one wave share a workgroup
-    const T* x = (const T*)g.X + row * g.ldx;
-    const int N = g.N;
+    constexpr bool HOLD = G < 1024 || R * E <= 16;        // a full CU of threads has 128 registers each
+    __shared__ float slot[2][2][G > 64 ? G / 64 : 1];
+    const int t = TEAMS > 1 ? threadIdx.x % G : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / G : 0;
+    const int N = g.N, P = N / E, rest = N - P * E;       // whole pieces; the elements behind them go to the first threads
+    const long step = (long)gridDim.x * TEAMS;
+    long row = (long)blockIdx.x * TEAMS + team;
+    if (row >= g.M) return;                               // whole teams; only teams of at most one wave share a workgroup
+    const WT* W = (const WT*)g.W;
+    const WT* B = (const WT*)g.B;
     Raw16 d[R];
+    float last = 0.f;
+    auto fetch = [&](long at) {
+        const T* x = (const T*)g.X + at * g.ldx;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int i0 = (r * G + t) * E;
-        if (i0 < N) d[r] = load_piece(x, i0, N, 0.f);
+        for (int r = 0; r < R; ++r)
+            if (r * G + t < P) d[r] = load16(x + (r * G + t) * E);
+        if (t < rest) last = to_f32(x[P * E + t]);
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) d[r] = Raw16{{0u, 0u, 0u, 0u}};
+    fetch(row);
+    float w[HOLD ? R : 1][E], b[HOLD ? R : 1][E], wl = 1.f, bl = 0.f;
+    if constexpr (HOLD)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r * G + t < P) {
+                load_weights<WT, E>(w[r], W, (r * G + t) * E, 1.f);
+                load_weights<WT, E>(b[r], B, (r * G + t) * E, 0.f);
+            }
+    if (t < rest) {
+        if (W) wl = to_f32(W[P * E + t]);
+        if (B) bl = to_f32(B[P * E + t]);
     }
-    float s = 0.f;
+    for (int par = 0;; par ^= 1) {
+        float s = last;                                   // places without an element hold 0
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-        if ((r * G + t) * E < N)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int e = 0; e < E; ++e) s += elem<T>(d[r], e);
-    const float mean = team_sum<G>(s, slot[0]) / (float)N;
-    float q = 0.f;
+        const float mean = team_sum<G>(s, slot[par][0]) / (float)N;
+        float q = 0.f;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int i0 = (r * G + t) * E;
-        if (i0 < N)
+        for (int r = 0; r < R; ++r)
+            if (r * G + t < P)
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float c = i0 + e < N ? elem<T>(d[r], e) - mean : 0.f;
-                q = fmaf(c, c, q);
-            }
-    }
-    const float rstd = 1.f / sqrtf(team_sum<G>(q, slot[1]) / (float)N + g.eps);
-    if (t == 0) {
-        if (g.mean) g.mean[row] = mean;
-        if (g.rstd) g.rstd[row] = rstd;
-    }
-    T* y = (T*)g.Y + row * g.ldy;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int i0 = (r * G + t) * E;
-        if (i0 < N) {
-            float w[E], b[E], o[E];
-            load_weights<WT, E>(w, (const WT*)g.W, i0, N, 1.f);
-            load_weights<WT, E>(b, (const WT*)g.B, i0, N, 0.f);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf((elem<T>(d[r], e) - mean) * rstd, w[e], b[e]);
-            store_piece(y, i0, N, o);
+                for (int e = 0; e < E; ++e) {
+                    const float c = elem<T>(d[r], e) - mean;
+                    q = fmaf(c, c, q);
+                }
+        if (t < rest) q = fmaf(last - mean, last - mean, q);
+        const float rstd = 1.f / sqrtf(team_sum<G>(q, slot[par][1]) / (float)N + g.eps);
+        if (t == 0) {
+            if (g.mean) g.mean[row] = mean;
+            if (g.rstd) g.rstd[row] = rstd;
         }
+        T* y = (T*)g.Y + row * g.ldy;
+        const long next = row + step;
+        Raw16 c[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) c[r] = d[r];
+        const float cl = last;
+        if (next < g.M) fetch(next);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r * G + t < P) {
+                float o[E];
+                keep_packed(c[r]);
+                if constexpr (!HOLD) {
+                    load_weights<WT, E>(w[0], W, (r * G + t) * E, 1.f);
+                    load_weights<WT, E>(b[0], B, (r * G + t) * E, 0.f);
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    o[e] = fmaf((elem<T>(c[r], e) - mean) * rstd, w[HOLD ? r : 0][e], b[HOLD ? r : 0][e]);
+                store16(y + (r * G + t) * E, pack<T>(o));
+            }
+        if (t < rest) y[P * E + t] = from_f32<T>(fmaf((cl - mean) * rstd, wl, bl));
+        if (next >= g.M) return;
+        row = next;
     }
+}
+
+// weights i0 .. i0 + E - 1 as far as the row has them
+template <class WT, int E> __device__ __forceinline__ void some_weights(float* f, const WT* w, int i0, int n, float none) {
+    if (i0 + E <= n) {
+        load_weights<WT, E>(f, w, i0, none);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = w && i0 + e < n ? to_f32(w[i0 + e]) : none;
 }
 
 // rows longer than a workgroup's registers hold: three walks over the row (the second and third from the caches)
@@ -140,8 +177,8 @@ template <class T, class WT> __global__ __launch_bounds__(1024) void ln_fwd_long
     for (long i0 = (long)t * E; i0 < N; i0 += G * E) {
         const Raw16 d = load_piece(x, (int)i0, N, 0.f);
         float w[E], b[E], o[E];
-        load_weights<WT, E>(w, (const WT*)g.W, (int)i0, N, 1.f);
-        load_weights<WT, E>(b, (const WT*)g.B, (int)i0, N, 0.f);
+        some_weights<WT, E>(w, (const WT*)g.W, (int)i0, N, 1.f);
+        some_weights<WT, E>(b, (const WT*)g.B, (int)i0, N, 0.f);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = fmaf((elem<T>(d, e) - mean) * rstd, w[e], b[e]);
         store_piece(y, (int)i0, N, o);
@@ -150,88 +187,130 @@ template <class T, class WT> __global__ __launch_bounds__(1024) void ln_fwd_long
 
 // ---- backward: a team walks rows, its threads keep the sums of dy xh and dy of their columns in registers ---------------
 template <class T, class WT, int G, int R>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void ln_bwd_kernel(LnBwd g) {
-    constexpr int E = Pack<T>::N, TEAMS = G < 256 ? 256 / G : 1, W = G > 64 ? G / 64 : 1;
+__global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
+    constexpr int E = Pack<T>::N, NT = G < 256 ? 512 : G, TEAMS = NT / G, W = G > 64 ? G / 64 : 1;
+    constexpr bool AHEAD = R * E <= 8;                    // the next row's loads: where its registers cost no occupancy
     __shared__ float slot[2][2 * W];
-    const int t = threadIdx.x % G, team = threadIdx.x / G, N = g.N;
-    float w[R][E], sw[R][E], sb[R][E];
+    const int t = TEAMS > 1 ? threadIdx.x % G : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / G : 0;
+    const int N = g.N, P = N / E, rest = N - P * E;
+    float w[R][E], sw[R][E], sb[R][E], wl = 0.f, swl = 0.f, sbl = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int i0 = (r * G + t) * E;
 #pragma unroll
         for (int e = 0; e < E; ++e) { sw[r][e] = 0.f; sb[r][e] = 0.f; w[r][e] = 0.f; }
-        if (i0 < N) load_weights<WT, E>(w[r], (const WT*)g.W, i0, N, 1.f);
+        if (r * G + t < P) load_weights<WT, E>(w[r], (const WT*)g.W, (r * G + t) * E, 1.f);
     }
+    if (t < rest) wl = g.W ? to_f32(((const WT*)g.W)[P * E + t]) : 1.f;
     const float inv = 1.f / (float)N;
-    int par = 0;
-    for (long row = (long)blockIdx.x * TEAMS + team; row < g.M; row += (long)gridDim.x * TEAMS, par ^= 1) {
+    const long step = (long)gridDim.x * TEAMS;
+    struct Row {
+        Raw16 x[R], dy[R];
+        float xl, dyl, mean, rstd;
+    };
+    auto fetch = [&](Row& k, long row) {
         const T* x = (const T*)g.X + row * g.ldx;
         const T* dy = (const T*)g.DY + row * g.lddy;
-        const float mean = g.mean[row], rstd = g.rstd[row];
-        Raw16 dx_[R], dd[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int i0 = (r * G + t) * E;
-            if (i0 < N) {
-                dx_[r] = load_piece(x, i0, N, 0.f);
-                dd[r] = load_piece(dy, i0, N, 0.f);
+        for (int r = 0; r < R; ++r)
+            if (r * G + t < P) {
+                k.x[r] = load16(x + (r * G + t) * E);
+                k.dy[r] = load16(dy + (r * G + t) * E);
             }
-        }
+        if (t < rest) { k.xl = to_f32(x[P * E + t]); k.dyl = to_f32(dy[P * E + t]); }
+        k.mean = g.mean[row];
+        k.rstd = g.rstd[row];
+    };
+    Row k;
+#pragma unroll
+    for (int r = 0; r < R; ++r) k.x[r] = k.dy[r] = Raw16{{0u, 0u, 0u, 0u}};
+    k.xl = k.dyl = 0.f;                                   // places without an element: dy = 0, so every sum stays
+    long row = (long)blockIdx.x * TEAMS + team;
+    if (row < g.M) fetch(k, row);
+    for (int par = 0; row < g.M; row += step, par ^= 1) {
+        Row n = k;
+        if constexpr (AHEAD)
+            if (row + step < g.M) fetch(n, row + step);
         float a = 0.f, b = 0.f;
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if ((r * G + t) * E < N)
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float d = elem<T>(dd[r], e), xh = (elem<T>(dx_[r], e) - mean) * rstd, v = d * w[r][e];
-                    a += v;                                     // past the row's end dy reads as 0, so all four sums stay
-                    b = fmaf(v, xh, b);
-                    sw[r][e] = fmaf(d, xh, sw[r][e]);
-                    sb[r][e] += d;
-                }
+            for (int e = 0; e < E; ++e) {
+                const float d = elem<T>(k.dy[r], e), xh = (elem<T>(k.x[r], e) - k.mean) * k.rstd, v = d * w[r][e];
+                a += v;
+                b = fmaf(v, xh, b);
+                sw[r][e] = fmaf(d, xh, sw[r][e]);
+                sb[r][e] += d;
+            }
+        const float xhl = (k.xl - k.mean) * k.rstd;
+        if (rest) {
+            a = fmaf(k.dyl, wl, a);
+            b = fmaf(k.dyl * wl, xhl, b);
+            swl = fmaf(k.dyl, xhl, swl);
+            sbl += k.dyl;
+        }
         const float2 c = team_sum2<G>(a, b, slot[par]);
         const float c1 = c.x * inv, c2 = c.y * inv;
         T* o = (T*)g.DX + row * g.lddx;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int i0 = (r * G + t) * E;
-            if (i0 < N) {
+        for (int r = 0; r < R; ++r)
+            if (r * G + t < P) {
                 float f[E];
+                keep_packed(k.dy[r]);
+                keep_packed(k.x[r]);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float d = elem<T>(dd[r], e), xh = (elem<T>(dx_[r], e) - mean) * rstd, v = d * w[r][e];
-                    f[e] = rstd * (v - fmaf(xh, c2, c1));
+                    const float d = elem<T>(k.dy[r], e), xh = (elem<T>(k.x[r], e) - k.mean) * k.rstd, v = d * w[r][e];
+                    f[e] = k.rstd * (v - fmaf(xh, c2, c1));
                 }
-                store_piece(o, i0, N, f);
+                store16(o + (r * G + t) * E, pack<T>(f));
             }
-        }
+        if (t < rest) o[P * E + t] = from_f32<T>(k.rstd * (k.dyl * wl - fmaf(xhl, c2, c1)));
+        if constexpr (!AHEAD)
+            if (row + step < g.M) fetch(n, row + step);
+        k = n;
     }
+    // the workgroup's sums: to its place in `part`, or, if it is the only one, to the gradients
     float* pw = g.part + (long)blockIdx.x * 2 * N;
+    auto out = [&](int h, int col, float v) {
+        if (gridDim.x > 1) {
+            pw[h * N + col] = v;
+        } else {
+            WT* to = (WT*)(h ? g.db : g.dw);
+            if (to) to[col] = from_f32<WT>(v);
+        }
+    };
     if constexpr (TEAMS == 1) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int i0 = (r * G + t) * E;
+        for (int r = 0; r < R; ++r)
+            if (r * G + t < P)
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (i0 + e < N) { pw[i0 + e] = sw[r][e]; pw[N + i0 + e] = sb[r][e]; }
-        }
+                for (int e = 0; e < E; ++e) {
+                    out(0, (r * G + t) * E + e, sw[r][e]);
+                    out(1, (r * G + t) * E + e, sb[r][e]);
+                }
+        if (t < rest) { out(0, P * E + t, swl); out(1, P * E + t, sbl); }
     } else {
-        // the workgroup's teams meet in LDS, added in team order
+        // the teams meet in LDS, added in team order
         __shared__ float meet[TEAMS][G * E];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r <= R; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                const int first = r < R ? r * G * E : P * E, count = r < R ? min(G * E, P * E - first) : rest;
+                if (count <= 0) continue;                 // the same for the whole workgroup
                 __syncthreads();
+                if (r < R) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) meet[team][t * E + e] = h ? sb[r][e] : sw[r][e];
+                    for (int e = 0; e < E; ++e) meet[team][t * E + e] = h ? sb[r < R ? r : 0][e] : sw[r < R ? r : 0][e];
+                } else if (t < rest) {
+                    meet[team][t] = h ? sbl : swl;
+                }
                 __syncthreads();
-                for (int i = threadIdx.x; i < G * E; i += 256) {
+                for (int i = threadIdx.x; i < count; i += NT) {
                     float v = 0.f;
 #pragma unroll
-                    for (int k = 0; k < TEAMS; ++k) v += meet[k][i];
-                    const int col = r * G * E + i;
-                    if (col < N) pw[h * N + col] = v;
+                    for (int j = 0; j < TEAMS; ++j) v += meet[j][i];
+                    out(h, first + i, v);
                 }
             }
     }
@@ -250,7 +329,7 @@ template <class T, class WT> __global__ __launch_bounds__(1024) void ln_bwd_long
     for (long i0 = (long)t * E; i0 < N; i0 += G * E) {
         const Raw16 dx_ = load_piece(x, (int)i0, N, 0.f), dd = load_piece(dy, (int)i0, N, 0.f);
         float w[E];
-        load_weights<WT, E>(w, (const WT*)g.W, (int)i0, N, 1.f);
+        some_weights<WT, E>(w, (const WT*)g.W, (int)i0, N, 1.f);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float v = elem<T>(dd, e) * w[e];
@@ -264,7 +343,7 @@ template <class T, class WT> __global__ __launch_bounds__(1024) void ln_bwd_long
     for (long i0 = (long)t * E; i0 < N; i0 += G * E) {
         const Raw16 dx_ = load_piece(x, (int)i0, N, 0.f), dd = load_piece(dy, (int)i0, N, 0.f);
         float w[E], f[E];
-        load_weights<WT, E>(w, (const WT*)g.W, (int)i0, N, 1.f);
+        some_weights<WT, E>(w, (const WT*)g.W, (int)i0, N, 1.f);
 #pragma unroll
         for (int e = 0; e < E; ++e)
             f[e] = rstd * (elem<T>(dd, e) * w[e] - fmaf((elem<T>(dx_, e) - mean) * rstd, c2, c1));
@@ -293,8 +372,19 @@ __global__ __launch_bounds__(1024) void ln_bwd_reduce_kernel(const float* part, 
     const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
     const long col = (long)blockIdx.x * 32 + c;                      // columns of [dw | db]
     float v = 0.f;
-    if (col < 2L * N)
-        for (int b = k; b < blocks; b += 32) v += part[(long)b * 2 * N + col];
+    if (col < 2L * N) {
+        const float* p = part + (long)k * 2 * N + col;
+        const long step = 64L * N;
+        int b = k;
+        for (; b + 7 * 32 < blocks; b += 8 * 32, p += 8 * step) {        // eight loads in flight
+            float q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = p[i * step];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v += q[i];
+        }
+        for (; b < blocks; b += 32, p += step) v += *p;
+    }
     meet[k][c] = v;
     __syncthreads();
     if (k == 0 && col < 2L * N) {
@@ -309,21 +399,28 @@ __global__ __launch_bounds__(1024) void ln_bwd_reduce_kernel(const float* part, 
     }
 }
 
-// The team of a row: the smallest whose registers hold it at R pieces per thread.
-template <class T> int ln_fwd_cap(int G, int R) { return G * R * Pack<T>::N; }
-
+// The team of a row: the smallest whose registers hold it, from what was measured at 200 MB of rows (us; a large copy takes 37):
+// 16-bit 1401 wide in 64 x 3 pieces 45.7 (64 x 4: 59.8, 256 x 1: 69.6), 2048 in 256 x 1 40.7 (64 x 4: 51.4), 8192 in 1024 x 1 43.1
+// (256 x 4: 54.7); fp32 4096 in 256 x 4 39.6 (1024 x 1: 50.7).  Workgroups: enough for 16 waves on each of 256 CUs, 32 where the
+// team is small and holds little.
 template <class T, class WT> int ln_fwd(const LnFwd& g, hipStream_t st) {
-    const int N = g.N, M = g.M;
+    constexpr int E = Pack<T>::N;
 #define LN_GO(G, R)                                                                                                      \
-    if (N <= ln_fwd_cap<T>(G, R)) {                                                                                      \
+    if (g.N <= G * R * E) {                                                                                              \
         constexpr int TEAMS = G < 256 ? 256 / G : 1, NT = G < 256 ? 256 : G;                                             \
-        hipLaunchKernelGGL((ln_fwd_kernel<T, WT, G, R>), dim3(cdiv(M, TEAMS)), dim3(NT), 0, st, g);                      \
+        const int all = cdiv(g.M, TEAMS), most = NT == 1024 ? 512 : G == 256 && R == 1 ? 2048 : 1024;                                                        \
+        hipLaunchKernelGGL((ln_fwd_kernel<T, WT, G, R>), dim3(all < most ? all : most), dim3(NT), 0, st, g);             \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
     }
-    LN_GO(16, 1) LN_GO(16, 2) LN_GO(64, 1) LN_GO(64, 2) LN_GO(64, 4) LN_GO(256, 2) LN_GO(256, 4) LN_GO(1024, 2) LN_GO(1024, 4)
+    LN_GO(16, 1) LN_GO(16, 2) LN_GO(64, 1) LN_GO(64, 2)
+    LN_GO(64, 3)
+    if constexpr (E == 4) { LN_GO(64, 4) } else { LN_GO(256, 1) }
+    LN_GO(256, 2) LN_GO(256, 3)
+    if constexpr (E == 4) { LN_GO(256, 4) } else { LN_GO(1024, 1) }
+    LN_GO(1024, 2) LN_GO(1024, 4)
 #undef LN_GO
-    hipLaunchKernelGGL((ln_fwd_long_kernel<T, WT>), dim3(M), dim3(1024), 0, st, g);
+    hipLaunchKernelGGL((ln_fwd_long_kernel<T, WT>), dim3(g.M), dim3(1024), 0, st, g);
     WFD_CHECK_LAUNCH();
     return WFD_OK;
 }
@@ -331,26 +428,36 @@ template <class T, class WT> int ln_fwd(const LnFwd& g, hipStream_t st) {
 struct LnBwdShape {
     int G, R, blocks;      // R = 0: the long form
 };
+// Teams as in the forward, with fewer pieces: a column costs three registers more.  More workgroups hide more latency and cost 8 N
+// bytes of partial sums each, written and read: at 1401 .. 2048 columns (16-bit) 1024 of them are best (69.5 us; 512: 80.9), at
+// 4096 512 (68.4; 768: 77.3, 1024: 93.1), above that one per CU.  16-bit 1401 wide: 64 x 3 pieces 70.4, 256 x 1 92.7; 5000: 256 x 3
+// 75.5, 1024 x 1 84.9.
 LnBwdShape ln_bwd_shape(int M, int N, int E) {
-    const int forms[][2] = {{16, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1}, {1024, 2}};
+    const int forms[][2] = {{16, 1}, {64, 1}, {64, 2}, {64, 3}, {256, 1}, {256, 2}, {256, 3}, {1024, 1}, {1024, 2}, {1024, 4}};
     for (auto& f : forms)
-        if (N <= f[0] * f[1] * E) {
-            const int teams = f[0] < 256 ? 256 / f[0] : 1;
-            const int most = f[0] == 1024 ? 256 : 512;
+        if (N <= f[0] * f[1] * E && (f[1] * E <= 16 || f[1] == 3)) {
+            const int teams = f[0] < 256 ? 512 / f[0] : 1;
+            const int most = f[0] == 1024 ? 256 : f[0] == 256 && f[1] == 1 ? 1024 : 512;
             const int b = cdiv(M, teams);
             return {f[0], f[1], b < most ? b : most};
         }
     return {0, 0, M < 64 ? M : 64};
 }
 
-template <class T, class WT> int ln_bwd(const LnBwd& g, WT* dw, WT* db, hipStream_t st) {
+template <class T, class WT> int ln_bwd(LnBwd g, WT* dw, WT* db, hipStream_t st) {
+    g.dw = dw;
+    g.db = db;
     const LnBwdShape s = ln_bwd_shape(g.M, g.N, Pack<T>::N);
     switch (s.G * 16 + s.R) {
 #define LN_GO(G, R)                                                                                                      \
     case G * 16 + R:                                                                                                     \
-        hipLaunchKernelGGL((ln_bwd_kernel<T, WT, G, R>), dim3(s.blocks), dim3(G < 256 ? 256 : G), 0, st, g);             \
+        hipLaunchKernelGGL((ln_bwd_kernel<T, WT, G, R>), dim3(s.blocks), dim3(G < 256 ? 512 : G), 0, st, g);             \
         break;
-        LN_GO(16, 1) LN_GO(64, 1) LN_GO(64, 2) LN_GO(256, 1) LN_GO(256, 2) LN_GO(1024, 1) LN_GO(1024, 2)
+        LN_GO(16, 1) LN_GO(64, 1) LN_GO(64, 2) LN_GO(64, 3) LN_GO(256, 1) LN_GO(256, 2) LN_GO(256, 3) LN_GO(1024, 1) LN_GO(1024, 2)
+        case 1024 * 16 + 4:
+            if constexpr (sizeof(T) == 4)                 // the shape's rule gives 16-bit rows at most 2 pieces
+                hipLaunchKernelGGL((ln_bwd_kernel<T, WT, 1024, 4>), dim3(s.blocks), dim3(1024), 0, st, g);
+            break;
 #undef LN_GO
         default:
             // the columns first: dx may lie over dy or x
@@ -358,7 +465,7 @@ template <class T, class WT> int ln_bwd(const LnBwd& g, WT* dw, WT* db, hipStrea
             hipLaunchKernelGGL((ln_bwd_long_kernel<T, WT>), dim3(g.M), dim3(1024), 0, st, g);
     }
     WFD_CHECK_LAUNCH();
-    if (dw || db) {
+    if ((dw || db) && (s.G == 0 || s.blocks > 1)) {
         hipLaunchKernelGGL((ln_bwd_reduce_kernel<WT>), dim3(cdiv(2L * g.N, 32)), dim3(1024), 0, st, g.part, s.blocks, g.N, dw,
                            db);
         WFD_CHECK_LAUNCH();
@@ -405,7 +512,7 @@ int wfd_layer_norm_bwd(const void* DY, int lddy, const void* X, int ldx, int dty
     if (M > 0 && (!mean || !rstd || !rows_ok(DY, lddy, M, N, dtype) || !rows_ok(X, ldx, M, N, dtype) ||
                   !rows_ok(DX, lddx, M, N, dtype)))
         return WFD_ERR_ARG;
-    LnBwd g{DY, X, weight, mean, rstd, DX, part, lddy, ldx, lddx, M, N};
+    LnBwd g{DY, X, weight, mean, rstd, DX, part, nullptr, nullptr, lddy, ldx, lddx, M, N};
     hipStream_t st = (hipStream_t)stream;
     if (M == 0) {                                        // no rows: the weights' gradients are sums of nothing
         if (wdtype == WFD_F32)
