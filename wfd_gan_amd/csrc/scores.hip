@@ -44,6 +44,10 @@ __device__ __forceinline__ unsigned long long order_key(float v, int i) {
     return ((unsigned long long)order_bits(v) << 32) | (unsigned)~i;
 }
 
+__device__ __forceinline__ float order_value(unsigned b) {
+    return b == 0xffffffffu ? NAN : __uint_as_float((b & 0x80000000u) ? b ^ 0x80000000u : ~b);
+}
+
 // ---- what one workgroup knows of its part of a row -----------------------------------------------------------------------
 // Running statistics: m = max(largest so far, -FLT_MAX), s = sum exp2((x - m) c), u = sum exp2((x - m) c) (x - m) c with
 // c = log2(e) / T.  The floor under m keeps x - m defined for rows of -inf (their s stays 0, which is how they are told) and for
@@ -134,7 +138,8 @@ __device__ __forceinline__ void row_store(const Scores& g, long row, const RowEn
 
 // ---- alternatives of a part of a row --------------------------------------------------------------------------------------
 // Every thread has left the largest value of each group of pieces that it visited in LDS.  The (k / waves)-th largest thread
-// maximum of a wave, the smallest such of all waves, is a value that at least k elements reach (tau).  Only groups whose maximum
+// maximum of a wave, the smallest such of all waves, is a value that at least k elements reach; so is any wave's k-th largest (a
+// part may be so short that the last waves have none).  The larger of the two is tau.  Only groups whose maximum
 // reaches tau are read again, an element per thread; what reaches tau there goes to a list (expected length: k and a few), whose
 // order is found by counting.  When more than the lists hold reach tau, they are ties at tau but for a few: those above tau are listed and the
 // rest is filled up by walking the ties in index order.  Rows with NaN, and rows that defeat even this (thousands above
@@ -145,7 +150,7 @@ constexpr int U = 4;                      // pieces per group
 template <int NT> struct PickLds {
     unsigned long long key[CAND];
     unsigned long long best[NT / 64 ? NT / 64 : 1];
-    float tau[NT / 64 ? NT / 64 : 1];
+    float tau[NT / 64 ? NT / 64 : 1], own[NT / 64 ? NT / 64 : 1];
     int group[GROUPS];
     int groups, count, run[NT / 64 ? NT / 64 : 1];
 };
@@ -172,11 +177,11 @@ template <int NT> __device__ __forceinline__ unsigned long long team_max_key(uns
 
 // the n-th largest (1 <= n <= 64) of the lanes' values (no NaN): a lane's value divides the lanes that are still in question, the
 // masks and counts are scalar work
-__device__ __forceinline__ float lanes_nth(float v, int n) {
+template <class V> __device__ __forceinline__ V lanes_nth(V v, int n) {
     unsigned long long in = ~0ull;
     for (;;) {
         const int src = __ffsll((long long)in) - 1;
-        const float p = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), src));
+        const V p = __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), src));
         const unsigned long long gt = __ballot(v > p) & in, eq = __ballot(v == p) & in;
         const int above = __popcll(gt), same = __popcll(eq);
         if (n <= above) {
@@ -186,6 +191,28 @@ __device__ __forceinline__ float lanes_nth(float v, int n) {
         } else {
             n -= above + same;
             in &= ~(gt | eq);
+        }
+    }
+}
+// the n-th largest (1 <= n <= 128) of two values per lane
+__device__ __forceinline__ float lanes_nth2(float a, float b, int n) {
+    unsigned long long in_a = ~0ull, in_b = ~0ull;
+    for (;;) {
+        const float v = in_a ? a : b;
+        const int src = __ffsll((long long)(in_a ? in_a : in_b)) - 1;
+        const float p = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), src));
+        const unsigned long long gt_a = __ballot(a > p) & in_a, gt_b = __ballot(b > p) & in_b;
+        const unsigned long long eq_a = __ballot(a == p) & in_a, eq_b = __ballot(b == p) & in_b;
+        const int above = __popcll(gt_a) + __popcll(gt_b), same = __popcll(eq_a) + __popcll(eq_b);
+        if (n <= above) {
+            in_a = gt_a;
+            in_b = gt_b;
+        } else if (n <= above + same) {
+            return p;
+        } else {
+            n -= above + same;
+            in_a &= ~(gt_a | eq_a);
+            in_b &= ~(gt_b | eq_b);
         }
     }
 }
@@ -199,13 +226,17 @@ __device__ __forceinline__ void pick(const T* x, int n, int base, int k, int nit
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     bool slow = sum != sum;
     if (!slow) {
-        const float mine = lanes_nth(tmax, (k + W - 1) / W);
-        if (lane == 0) l.tau[wave] = mine;
+        const float share = lanes_nth(tmax, (k + W - 1) / W), own = n < NT * E ? lanes_nth(tmax, k) : -INFINITY;
+        if (lane == 0) { l.tau[wave] = share; l.own[wave] = own; }
         if (t == 0) l.count = l.groups = 0;
         team_sync<NT>();
-        float tau = l.tau[0];
+        float tau = l.tau[0], best = l.own[0];
 #pragma unroll
-        for (int i = 1; i < W; ++i) tau = fminf(tau, l.tau[i]);
+        for (int i = 1; i < W; ++i) {
+            tau = fminf(tau, l.tau[i]);
+            best = fmaxf(best, l.own[i]);
+        }
+        tau = fmaxf(tau, best);
         int total = 0;
         bool ties = false;
         for (int pass = 0; pass < 2; ++pass) {
@@ -400,30 +431,30 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
 }
 
 // the parts of a row: a lane per part for the statistics, alternatives from the parts' lists
-__device__ __forceinline__ float order_value(unsigned b) {
-    return b == 0xffffffffu ? NAN : __uint_as_float((b & 0x80000000u) ? b ^ 0x80000000u : ~b);
-}
 template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Scores g) {
     extern __shared__ unsigned long long keys[];              // splits * k
     __shared__ unsigned long long list[CAND];
-    __shared__ unsigned long long slot[4];
     __shared__ int count;
     const long row = blockIdx.x;
     const int t = threadIdx.x, S = g.splits, k = g.k, each = 3 + 2 * k;
     const float* w = g.work + row * S * each;
     if (t == 0) count = 0;
-    // a part's last entry, where its list is full, is reached by k elements: what is below the largest such is out
-    unsigned long long least = 0;
-    for (int i = t; i < S * k; i += 256) {
-        const int s = i / k, j = i - s * k;
-        const float* p = w + s * each + 3;
-        const float v = p[j];
-        const int at = ((const int*)p)[k + j];
-        const unsigned long long key = at < 0 ? 0ull : order_key(v, at);
-        keys[i] = key;
-        if (j == k - 1 && key > least) least = key;
-    }
     const int lane = t & 63;
+    // If n parts have a j-th entry that reaches a value, n j elements do: the ceil(k / j)-th largest of the parts' j-th entries, with
+    // about half of the parts in it.  A lane per part (at most 64); a place without an entry counts as 0, below every number.
+    const int j = min(k, cdiv_dev(2 * k, S));
+    unsigned jth = 0;
+    if (k > 0 && lane < S) {
+        const float* p = w + lane * each + 3;
+        if (((const int*)p)[k + j - 1] >= 0) jth = order_bits(p[j - 1]);
+    }
+    for (int i = t; i < S * k; i += 256) {
+        const int s = i / k, e = i - s * k;
+        const float* p = w + s * each + 3;
+        const float v = p[e];
+        const int at = ((const int*)p)[k + e];
+        keys[i] = at < 0 ? 0ull : order_key(v, at);
+    }
     const float c = g.inv_t * LOG2E;
     Stat a{LOWEST, 0.f, 0.f};
     if (lane < S) a = Stat{w[lane * each], w[lane * each + 1], w[lane * each + 2]};      // S <= 64
@@ -433,12 +464,15 @@ template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Sco
         row_store(g, row, r, y >= 0 && y < g.V ? to_f32(((const T*)g.X + row * g.ld)[y]) : 0.f, y);
     }
     if (k == 0) return;
-    least = team_max_key<256>(least, slot);
-    for (int i = t; i < S * k; i += 256)
-        if (keys[i] >= least && keys[i]) {
+    const unsigned least = lanes_nth(jth, cdiv_dev(k, j));
+    __syncthreads();
+    for (int i = t; i < S * k; i += 256) {
+        const unsigned long long key = keys[i];
+        if ((unsigned)(key >> 32) >= least && key) {
             const int at = atomicAdd(&count, 1);
-            if (at < CAND) list[at] = keys[i];
+            if (at < CAND) list[at] = key;
         }
+    }
     __syncthreads();
     const bool all = count > CAND;
     const unsigned long long* from = all ? keys : list;
@@ -455,7 +489,7 @@ template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Sco
     }
 }
 
-// ---- few classes: a team of G lanes holds the row, R pieces per lane --------------------------------------------------------
+// ---- few classes: a team of G lanes holds the row, R pieces per lane and at most one element behind the last whole piece --------
 template <int G> __device__ __forceinline__ unsigned lanes_max_u32(unsigned v) {
     auto step = [&](unsigned w) { v = w > v ? w : v; };
     step(__builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));
@@ -466,52 +500,130 @@ template <int G> __device__ __forceinline__ unsigned lanes_max_u32(unsigned v) {
     if constexpr (G >= 64) step(__shfl_xor(v, 32, 64));
     return v;
 }
+constexpr int LIST = 192;                 // candidates of a wave's row
 template <class T, int G, int R> __global__ __launch_bounds__(256) void scores_few_kernel(Scores g) {
-    constexpr int E = Pack<T>::N, TEAMS = 256 / G;
-    const int t = threadIdx.x % G, V = g.V;
+    constexpr int E = Pack<T>::N, TEAMS = 256 / G, N = R * E + 1;
+    __shared__ unsigned long long lists[G == 64 ? 4 : 1][G == 64 ? LIST : 1];
+    const int t = threadIdx.x % G, V = g.V, P = V / E, rest = V - P * E;
     const long row = (long)blockIdx.x * TEAMS + threadIdx.x / G;
     if (row >= g.M) return;                                   // whole teams
     const T* x = (const T*)g.X + row * g.ld;
+    float f[N];
+    auto have = [&](int e) { return e < R * E ? (e / E) * G + t < P : t < rest; };
+    auto index = [&](int e) { return e < R * E ? ((e / E) * G + t) * E + e % E : P * E + t; };
+    {
+        Raw16 d[R];
+        const unsigned none = raw_fill<T>(-INFINITY);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            d[r] = Raw16{{none, none, none, none}};
+            if (r * G + t < P) d[r] = load16(x + (r * G + t) * E);
+        }
+        f[R * E] = t < rest ? to_f32(x[P * E + t]) : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < R * E; ++e) f[e] = elem<T>(d[e / E], e % E);
+    }
     const int y = g.labels ? g.labels[row] : -1;
     const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
     const float c = g.inv_t * LOG2E;
-    float f[R * E];
-    float top = -INFINITY;
+    // the lane's two largest; a NaN is in neither, and in every sum
+    float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int i0 = (r * G + t) * E;
-        Raw16 d;
-        if (i0 < V) d = load_piece(x, i0, V, -INFINITY);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            f[r * E + e] = i0 < V ? elem<T>(d, e) : -INFINITY;
-            top = fmaxf(top, f[r * E + e]);
-        }
+    for (int e = 0; e < N; ++e) {
+        b2 = fmaxf(b2, fminf(b1, f[e]));
+        b1 = fmaxf(b1, f[e]);
     }
     Stat a{LOWEST, 0.f, 0.f};
-    stat_add(a, f, fmaxf(lanes_max<G>(top), LOWEST), c);
+    stat_add(a, f, fmaxf(lanes_max<G>(b1), LOWEST), c);
     a.s = lanes_sum<G>(a.s);
     a.u = lanes_sum<G>(a.u);
     const RowEnd r = row_end(a);
     if (t == 0) row_store(g, row, r, xy, y);
+    if (g.k == 0) return;
+    if constexpr (G == 64) {
+        // as in pick(): a value that k elements reach, a list of what reaches it, its order by counting
+        if (a.s == a.s) {
+            unsigned long long* list = lists[threadIdx.x >> 6];
+            const float tau = lanes_nth2(b1, b2, g.k);
+            const unsigned long long below = (1ull << t) - 1;
+            int n = 0;
+            auto gather = [&](bool strict) {
+                n = 0;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const bool hit = (strict ? f[e] > tau : f[e] >= tau) && have(e);
+                    const unsigned long long who = __ballot(hit);
+                    if (who == 0) continue;
+                    const int at = n + __popcll(who & below);
+                    if (hit && at < LIST) list[at] = order_key(f[e], index(e));
+                    n += __popcll(who);
+                }
+            };
+            gather(false);
+            const bool ties = n > LIST;
+            if (ties) gather(true);
+            if (n <= LIST) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                for (int i = t; i < n; i += 64) {
+                    const unsigned long long key = list[i];
+                    int rank = 0;
+#pragma unroll 4
+                    for (int b = 0; b < n; ++b) rank += list[b] > key;
+                    if (rank < g.k) {
+                        g.top_idx[row * g.k + rank] = (int)~(unsigned)key;
+                        g.top_lp[row * g.k + rank] = row_lp(r, order_value((unsigned)(key >> 32)), g.inv_t);
+                    }
+                }
+                // what is left are ties at tau, in the order of their indices: by piece, lane and element
+                if (ties)
+#pragma unroll
+                    for (int r0 = 0; r0 <= R; ++r0) {
+                        if (n >= g.k) continue;
+                        unsigned long long who[E];
+                        int before = 0, all = 0;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            who[e] = 0;
+                            if (r0 == R && e > 0) continue;
+                            who[e] = __ballot(f[r0 * E + e] == tau && have(r0 * E + e));
+                            before += __popcll(who[e] & below);
+                            all += __popcll(who[e]);
+                        }
+                        int at = n + before;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            if (r0 == R && e > 0) continue;
+                            if (who[e] >> t & 1) {
+                                if (at < g.k) {
+                                    g.top_idx[row * g.k + at] = index(r0 * E + e);
+                                    g.top_lp[row * g.k + at] = row_lp(r, tau, g.inv_t);
+                                }
+                                ++at;
+                            }
+                        }
+                        n += all;
+                    }
+                return;
+            }
+        }
+    }
     // one alternative after another: best of the lane, best of the team, and the winner looks for its next
-    unsigned done = 0;                                        // elements of this lane already given
+    unsigned long long done = 0;                              // elements of this lane already given
     for (int j = 0; j < g.k; ++j) {
         unsigned best = 0;
         int at = 0x7fffffff, slot = 0;
-        float val = 0.f;
 #pragma unroll
-        for (int e = 0; e < R * E; ++e) {
-            const int i = ((e / E) * G + t) * E + e % E;
+        for (int e = 0; e < N; ++e) {
             const unsigned b = order_bits(f[e]);
-            if (!(done >> e & 1) && i < V && b > best) { best = b; at = i; slot = e; val = f[e]; }
+            if (!(done >> e & 1) && have(e) && b > best) { best = b; at = index(e); slot = e; }    // indices rise with e
         }
         const unsigned m = lanes_max_u32<G>(best);
-        const unsigned who = ~lanes_max_u32<G>(best == m ? ~(unsigned)at : 0u);
-        if (at == (int)who && best == m) {
-            done |= 1u << slot;
+        const int who = (int)~lanes_max_u32<G>(best == m ? ~(unsigned)at : 0u);
+        if (best == m && at == who) {
+            done |= 1ull << slot;
             g.top_idx[row * g.k + j] = at;
-            g.top_lp[row * g.k + j] = row_lp(r, val, g.inv_t);
+            g.top_lp[row * g.k + j] = row_lp(r, order_value(m), g.inv_t);
         }
     }
 }
@@ -591,10 +703,11 @@ bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
 constexpr int MAX_V = 1 << 23, MAX_K = 64;   // 64 parts of 32 fp32 steps
 int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
 
-// Few classes stay in the registers of a team inside a wave.  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192
+// Few classes stay in the registers of a team inside a wave: 16 lanes where they hold the row and a round per alternative is
+// cheap (16384 x 100, top 64: 38.1 us in rounds of 16 lanes, 28 in the whole wave's list; top 5: 11.5 and 14.5).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192
 // 16-bit or 4096 fp32 classes); a row is split over workgroups (64 at most) while there are fewer than 1024 of them, and where its
 // group maxima would take more than 32 steps' room in LDS.
-constexpr int FEW = 128;                  // lanes * pieces of the team form: up to 1024 16-bit or 512 fp32 classes
+constexpr int FEW = 256;                  // lanes * pieces of the team form: up to 2048 16-bit or 1024 fp32 classes
 constexpr int MOST_STEPS = 32;
 struct ScoresShape {
     int splits, chunk, steps;             // splits = 0: the team form
@@ -619,12 +732,12 @@ template <class T> int scores(Scores g, hipStream_t st) {
     g.chunk = s.chunk;
     if (s.splits == 0) {
 #define WFD_FEW(G, R)                                                                                                    \
-    if (g.V <= G * R * E) {                                                                                              \
+    if (g.V <= G * R * E && (G == 64 || g.k <= 16)) {                                                                    \
         hipLaunchKernelGGL((scores_few_kernel<T, G, R>), dim3(cdiv(g.M, 256 / G)), dim3(256), 0, st, g);                 \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
     }
-        WFD_FEW(16, 1) WFD_FEW(16, 2) WFD_FEW(64, 1) WFD_FEW(64, 2)
+        WFD_FEW(16, 1) WFD_FEW(16, 2) WFD_FEW(64, 1) WFD_FEW(64, 2) WFD_FEW(64, 4)
 #undef WFD_FEW
     }
     const long parts = (long)g.M * s.splits;
