@@ -138,22 +138,26 @@ __device__ __forceinline__ void row_store(const Scores& g, long row, const RowEn
 
 // ---- alternatives of a part of a row --------------------------------------------------------------------------------------
 // Every thread has left the largest value of each group of pieces that it visited in LDS.  The (k / waves)-th largest thread
-// maximum of a wave, the smallest such of all waves, is a value that at least k elements reach; so is any wave's k-th largest (a
+// maximum of a wave (alone in its workgroup, a wave counts each thread's two largest), the smallest such of all waves, is a value that at least k elements reach; so is any wave's k-th largest (a
 // part may be so short that the last waves have none).  The larger of the two is tau.  Only groups whose maximum
 // reaches tau are read again, an element per thread; what reaches tau there goes to a list (expected length: k and a few), whose
 // order is found by counting.  When more than the lists hold reach tau, they are ties at tau but for a few: those above tau are listed and the
 // rest is filled up by walking the ties in index order.  Rows with NaN, and rows that defeat even this (thousands above
 // tau), take the k largest one after another.
-constexpr int CAND = 1024, GROUPS = 512;
 constexpr int U = 4;                      // pieces per group
 
 template <int NT> struct PickLds {
+    static constexpr int CAND = 4 * NT, GROUPS = 2 * NT;
     unsigned long long key[CAND];
     unsigned long long best[NT / 64 ? NT / 64 : 1];
     float tau[NT / 64 ? NT / 64 : 1], own[NT / 64 ? NT / 64 : 1];
     int group[GROUPS];
     int groups, count, run[NT / 64 ? NT / 64 : 1];
 };
+
+struct NoLds {};
+template <bool PICK, int NT> struct Cond { typedef PickLds<NT> type; };
+template <int NT> struct Cond<false, NT> { typedef NoLds type; };
 
 template <int NT> __device__ __forceinline__ void team_sync() {
     if constexpr (NT > 64) __syncthreads();
@@ -220,13 +224,14 @@ __device__ __forceinline__ float lanes_nth2(float a, float b, int n) {
 // Leaves the k best of x[0, n) (indices from `base`) at out_val / out_idx in order, places without an element as index -1.
 // gmax[it * NT + t]: the group maxima.  sum: the part's s (NaN tells of NaN or +inf).
 template <class T, int NT>
-__device__ __forceinline__ void pick(const T* x, int n, int base, int k, int niter, const float* gmax, float tmax, float sum, PickLds<NT>& l,
+__device__ __forceinline__ void pick(const T* x, int n, int base, int k, int niter, const float* gmax, float tmax, float next, float sum, PickLds<NT>& l,
                      float* out_val, int* out_idx) {
-    constexpr int E = Pack<T>::N, W = NT / 64;
+    constexpr int E = Pack<T>::N, W = NT / 64, CAND = PickLds<NT>::CAND, GROUPS = PickLds<NT>::GROUPS;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     bool slow = sum != sum;
     if (!slow) {
-        const float share = lanes_nth(tmax, (k + W - 1) / W), own = n < NT * E ? lanes_nth(tmax, k) : -INFINITY;
+        const float share = W == 1 ? lanes_nth2(tmax, next, k) : lanes_nth(tmax, (k + W - 1) / W);
+        const float own = W > 1 && n < NT * E ? lanes_nth(tmax, k) : -INFINITY;
         if (lane == 0) { l.tau[wave] = share; l.own[wave] = own; }
         if (t == 0) l.count = l.groups = 0;
         team_sync<NT>();
@@ -278,6 +283,7 @@ __device__ __forceinline__ void pick(const T* x, int n, int base, int k, int nit
             for (int a = t; a < total; a += NT) {
                 const unsigned long long key = l.key[a];
                 int rank = 0;
+#pragma unroll 8
                 for (int b = 0; b < total; ++b) rank += l.key[b] > key;
                 if (rank < k) {
                     const int i = (int)~(unsigned)key;
@@ -341,11 +347,11 @@ __device__ __forceinline__ void pick(const T* x, int n, int base, int k, int nit
 
 // ---- one walk over a part of a row ----------------------------------------------------------------------------------------
 template <class T, int NT, bool PICK>
-__device__ __forceinline__ Stat walk(const T* x, int n, float c, float* gmax, float& tmax) {
+__device__ __forceinline__ Stat walk(const T* x, int n, float c, float* gmax, float& tmax, float& next) {
     constexpr int E = Pack<T>::N, STEP = NT * U * E;
     const int t = threadIdx.x;
     Stat a{LOWEST, 0.f, 0.f};
-    tmax = -INFINITY;
+    tmax = next = -INFINITY;                                  // the thread's two largest group maxima
     int it = 0;
     auto take = [&](const Raw16 (&d)[U]) {
         float f[U * E];
@@ -358,6 +364,7 @@ __device__ __forceinline__ Stat walk(const T* x, int n, float c, float* gmax, fl
         for (int e = 1; e < U * E; ++e) top = fmaxf(top, f[e]);
         if constexpr (PICK) {
             gmax[it * NT + t] = top;
+            if constexpr (NT == 64) next = fmaxf(next, fminf(tmax, top));
             tmax = fmaxf(tmax, top);
         }
         stat_add(a, f, top, c);
@@ -389,6 +396,7 @@ __device__ __forceinline__ Stat walk(const T* x, int n, float c, float* gmax, fl
         }
         if constexpr (PICK) {
             gmax[it * NT + t] = group;
+            if constexpr (NT == 64) next = fmaxf(next, fminf(tmax, group));
             tmax = fmaxf(tmax, group);
         }
     }
@@ -399,7 +407,7 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
     constexpr int E = Pack<T>::N, STEP = NT * U * E;
     extern __shared__ float gmax[];
     __shared__ float slot[3 * (NT / 64)];
-    __shared__ PickLds<PICK ? NT : 64> l;
+    __shared__ typename Cond<PICK, NT>::type l;
     const long part = blockIdx.x, row = part / g.splits;
     const int sp = (int)(part - row * g.splits);
     const int lo = sp * g.chunk, n = min(g.chunk, g.V - lo);
@@ -407,8 +415,8 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
     const int y = g.labels ? g.labels[row] : -1;
     const float xy = g.splits == 1 && y >= 0 && y < g.V ? to_f32(x[y]) : 0.f;
     const float c = g.inv_t * LOG2E;
-    float tmax;
-    Stat a = walk<T, NT, PICK>(x, n, c, gmax, tmax);
+    float tmax, next;
+    Stat a = walk<T, NT, PICK>(x, n, c, gmax, tmax, next);
     a = stat_team<NT>(a, c, slot);
     float* w = g.work + part * (3 + 2 * g.k);
     const bool whole = g.splits == 1;
@@ -422,7 +430,7 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
     if constexpr (PICK) {
         float* val = whole ? g.top_lp + row * g.k : w + 3;
         int* idx = whole ? g.top_idx + row * g.k : (int*)(w + 3 + g.k);
-        pick<T, NT>(x, n, lo, g.k, cdiv_dev(n, STEP), gmax, tmax, a.s, l, val, idx);
+        pick<T, NT>(x, n, lo, g.k, cdiv_dev(n, STEP), gmax, tmax, next, a.s, l, val, idx);
         if (whole) {
             team_sync<NT>();
             for (int j = threadIdx.x; j < g.k; j += NT) val[j] = row_lp(r, val[j], g.inv_t);
@@ -433,6 +441,7 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
 // the parts of a row: a lane per part for the statistics, alternatives from the parts' lists
 template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Scores g) {
     extern __shared__ unsigned long long keys[];              // splits * k
+    constexpr int CAND = 1024;
     __shared__ unsigned long long list[CAND];
     __shared__ int count;
     const long row = blockIdx.x;
@@ -481,6 +490,7 @@ template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Sco
         const unsigned long long key = from[i];
         if (!key) continue;
         int rank = 0;
+#pragma unroll 8
         for (int b = 0; b < n; ++b) rank += from[b] > key;
         if (rank < k) {
             g.top_idx[row * k + rank] = (int)~(unsigned)key;
@@ -568,7 +578,7 @@ template <class T, int G, int R> __global__ __launch_bounds__(256) void scores_f
                 for (int i = t; i < n; i += 64) {
                     const unsigned long long key = list[i];
                     int rank = 0;
-#pragma unroll 4
+#pragma unroll 8
                     for (int b = 0; b < n; ++b) rank += list[b] > key;
                     if (rank < g.k) {
                         g.top_idx[row * g.k + rank] = (int)~(unsigned)key;
@@ -704,17 +714,21 @@ constexpr int MAX_V = 1 << 23, MAX_K = 64;   // 64 parts of 32 fp32 steps
 int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
 
 // Few classes stay in the registers of a team inside a wave: 16 lanes where they hold the row and a round per alternative is
-// cheap (16384 x 100, top 64: 38.1 us in rounds of 16 lanes, 28 in the whole wave's list; top 5: 11.5 and 14.5).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192
+// cheap (16384 x 100, top 64: 38.1 us in rounds of 16 lanes, 28 in the whole wave's list; top 5: 11.5 and 14.5).  Many
+// rows up to 16384 (8192) classes take a wave each: no barriers, four times the rows in flight (16384 x 4000 bf16, top 5: 38.5 us
+// instead of 65.7).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192
 // 16-bit or 4096 fp32 classes); a row is split over workgroups (64 at most) while there are fewer than 1024 of them, and where its
 // group maxima would take more than 32 steps' room in LDS.
 constexpr int FEW = 256;                  // lanes * pieces of the team form: up to 2048 16-bit or 1024 fp32 classes
 constexpr int MOST_STEPS = 32;
+constexpr int NARROW = 8, MANY = 2048;    // a wave per row: up to 8 of its steps, where there are rows enough for all CUs
 struct ScoresShape {
-    int splits, chunk, steps;             // splits = 0: the team form
+    int splits, chunk, steps;             // splits = 0: the team form; -1: a wave per row
 };
 ScoresShape scores_shape(int M, int V, int dtype, int k) {
     const int E = elems_of(dtype);
     if (V <= FEW * E) return {0, V, 0};
+    if (V <= NARROW * 64 * U * E && M >= MANY) return {-1, V, cdiv(V, 64 * U * E)};
     const int step = 256 * U * E, steps = cdiv(V, step);
     int S = M >= 1024 ? 1 : cdiv(1024, M > 0 ? M : 1);
     if (S > steps) S = steps;
@@ -739,6 +753,15 @@ template <class T> int scores(Scores g, hipStream_t st) {
     }
         WFD_FEW(16, 1) WFD_FEW(16, 2) WFD_FEW(64, 1) WFD_FEW(64, 2) WFD_FEW(64, 4)
 #undef WFD_FEW
+    }
+    if (s.splits < 0) {
+        g.splits = 1;
+        if (g.k > 0)
+            hipLaunchKernelGGL((scores_kernel<T, 64, true>), dim3(g.M), dim3(64), (size_t)s.steps * 256, st, g);
+        else
+            hipLaunchKernelGGL((scores_kernel<T, 64, false>), dim3(g.M), dim3(64), 0, st, g);
+        WFD_CHECK_LAUNCH();
+        return WFD_OK;
     }
     const long parts = (long)g.M * s.splits;
     if (parts > 0x7fffffffL) return WFD_ERR_ARG;
