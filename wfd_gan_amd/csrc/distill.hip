@@ -185,16 +185,26 @@ __device__ __forceinline__ void grad_targets(const Distill& g, const GradRow& d,
                                              int hi, int y, float xy, float c) {
     if (empty) return;
     bool label_seen = false;
+    // does any index occur twice?  An entry per lane answers with scalar work; more entries are compared one by one
+    bool twice = L < 64 || g.K > 64;
+    if (!twice) {
+        const int mine = lane < g.K ? n.at[lane] : -1;
+        for (int i = 0; i < g.K && !twice; ++i) {
+            const int at = __builtin_amdgcn_readlane(mine, i);
+            twice = at >= 0 && __popcll(__ballot(mine == at)) > 1;
+        }
+    }
     for (int j = lane; j < g.K; j += L) {
         const int at = n.at[j];
         if (at < lo || at >= hi) continue;
-        float sum = 0.f;
+        float sum = twice ? 0.f : n.e[j];
         bool first = true;
-        for (int i = 0; i < g.K; ++i)
-            if (n.at[i] == at) {
-                sum += n.e[i];
-                first = first && i >= j;
-            }
+        if (twice)
+            for (int i = 0; i < g.K; ++i)
+                if (n.at[i] == at) {
+                    sum += n.e[i];
+                    first = first && i >= j;
+                }
         if (at == y) label_seen = true;
         if (first) {
             float v = grad_dense<TWO>(d, n.x[j], c) - d.rt * sum;
@@ -213,7 +223,7 @@ __device__ __forceinline__ void grad_targets(const Distill& g, const GradRow& d,
 // out, so that memory has work while the arithmetic of a row runs (a long row fills the CU's registers: there is no second workgroup
 // to do that).
 template <class T, int G, int R, bool TWO, bool GRAD>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void distill_kernel(Distill g) {
+__global__ __launch_bounds__(G < 256 ? 256 : G, R == 16 ? 4 : 1) void distill_kernel(Distill g) {
     constexpr int E = Pack<T>::N, TEAMS = G < 256 ? 256 / G : 1, L = G < 64 ? G : 64, B = R < 4 ? R : 4;
     extern __shared__ float lds[];
     __shared__ float slot[2][2 * (G > 64 ? G / 64 : 1)], told[8];
@@ -221,39 +231,50 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void distill_kernel(Distill g) {
     int row = blockIdx.x * TEAMS + team;
     if (row >= g.M) return;                                   // whole teams, each inside a wave
     const float inv_t = 1.f / g.temp, c = inv_t * LOG2E;
-    const Entries n = entries_in(lds + team * 3 * g.K, g.K);
-    // piece r * G + t of V / E whole ones; the V % E elements behind them go to the first threads
-    const int P = V / E, rest = V - P * E;
+    // piece r * G + t of the whole ones; the elements around them go to the first threads
     const unsigned lane_off = (unsigned)t * E;
     Raw16 d[R];
     float tail = -INFINITY;
-    auto fetch = [&](int r, const T* x) {
-        if (r * G + t < P) d[r] = load16(x + r * G * E + lane_off);
+    auto fetch = [&](int r, const T* x, int h, int pieces) {
+        if (r * G + t < pieces) d[r] = load16(x + h + r * G * E + lane_off);
+    };
+    auto fetch_tail = [&](const T* x, int h, int pieces) {
+        tail = -INFINITY;
+        if (t < V - pieces * E) tail = to_f32(x[t < h ? 0 : pieces * E + t]);
     };
     const unsigned none = raw_fill<T>(-INFINITY);
+    int head, P;
     {
         const T* x = (const T*)g.X + (long)row * g.ld;
+        head = G > 64 ? off_border(x) : 0;
+        P = (V - head) / E;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             d[r] = Raw16{{none, none, none, none}};
-            fetch(r, x);
+            fetch(r, x, head, P);
         }
-        if (t < rest) tail = to_f32(x[P * E + t]);
+        fetch_tail(x, head, P);
     }
-    for (;;) {
+    for (int par = 0;; par ^= 1) {
+        // one set of entries per row in turn: the wave of the row before may still be at its targets
+        const Entries n = entries_in(lds + (G > 64 ? par : team) * 3 * g.K, g.K);
         const T* x = (const T*)g.X + (long)row * g.ld;
         const long next = (long)row + gridDim.x;
         const bool more = G > 64 && next < g.M;
         const T* xn = x + (long)gridDim.x * g.ld;
+        const int rest = V - P * E, head_n = G > 64 ? off_border(xn) : 0, P_n = (V - head_n) / E;
+        // the wave that works the entries changes from row to row: a workgroup's first wave always sits on the same SIMD
+        const int lane = G > 64 ? t & 63 : t;
+        const bool boss = G <= 64 || (t >> 6) == (row & (G / 64 - 1));
         const int y = g.u != 0.f ? g.labels[row] : -1;
         const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
         Taught tt{LOWEST, 0.f, false};
-        if (t < L) {
-            tt = teacher<L>(g, row, t, n, c);
+        if (boss) {
+            tt = teacher<L>(g, row, lane, n, c);
             wave_sync();
-            entries_gather<T, L>(x, g.K, t, n);
+            entries_gather<T, L>(x, g.K, lane, n);
             if constexpr (G > 64)
-                if (t == 0) { told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f; }
+                if (lane == 0) { told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f; }
         }
         // per thread about its own running maximum, four pieces at a time, while later pieces are still on their way
         RowSums s{LOWEST, 0.f, 0.f};
@@ -285,10 +306,10 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void distill_kernel(Distill g) {
             s.s1 = s.s = team_sum<G>(s.s, slot[1]);
         }
         const bool wrong = tt.wrong || y >= V;
-        if (t < L) {
+        if (boss) {
             wave_sync();
-            const float loss = row_loss<L>(g, row, t, n, tt, s, inv_t, y, xy, wrong);
-            if (t == 0) g.loss[row] = loss;
+            const float loss = row_loss<L>(g, row, lane, n, tt, s, inv_t, y, xy, wrong);
+            if (lane == 0) g.loss[row] = loss;
         }
         if constexpr (GRAD) {
             const GradRow k = grad_row<TWO>(g, row, tt, s, y, wrong, c);
@@ -296,22 +317,24 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void distill_kernel(Distill g) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 keep_packed(d[r]);
-                if (r * G + t < P) grad_piece<T, TWO>(k, d[r], o + r * G * E + lane_off, c);
-                if (more) fetch(r, xn);
+                if (r * G + t < P) grad_piece<T, TWO>(k, d[r], o + head + r * G * E + lane_off, c);
+                if (more) fetch(r, xn, head_n, P_n);
             }
-            if (t < rest) o[P * E + t] = from_f32<T>(grad_dense<TWO>(k, tail, c));
+            if (t < rest) o[t < head ? 0 : P * E + t] = from_f32<T>(grad_dense<TWO>(k, tail, c));
             if constexpr (G > 64) __syncthreads();
             else wave_sync();
-            if (t < L) grad_targets<T, TWO, L>(g, k, n, s.s == 0.f, t, o, 0, V, y, xy, c);
+            if (boss) grad_targets<T, TWO, L>(g, k, n, s.s == 0.f, lane, o, 0, V, y, xy, c);
         } else if constexpr (G > 64) {
             if (more)
 #pragma unroll
-                for (int r = 0; r < R; ++r) fetch(r, xn);
+                for (int r = 0; r < R; ++r) fetch(r, xn, head_n, P_n);
             __syncthreads();                                  // the next row's entries and sums go where this row's were
         }
         if constexpr (G <= 64) return;
         if (!more) return;
-        if (t < rest) tail = to_f32(xn[P * E + t]);
+        fetch_tail(xn, head_n, P_n);
+        head = head_n;
+        P = P_n;
         row = (int)next;
     }
 }
@@ -459,11 +482,11 @@ template <class T, bool TWO, bool GRAD> int distill(Distill g, hipStream_t st) {
         constexpr int TEAMS = G < 256 ? 256 / G : 1;                                                                     \
         const int blocks = cdiv(g.M, TEAMS), most = G > 64 ? 256 * (16 / R) * (1024 / G) : blocks;                       \
         hipLaunchKernelGGL((distill_kernel<T, G, R, TWO, GRAD>), dim3(blocks < most ? blocks : most), dim3(G < 256 ? 256 : G), \
-                           (size_t)TEAMS * 3 * g.K * 4, st, g);                                                          \
+                           (size_t)(TEAMS > 1 ? TEAMS : 2) * 3 * g.K * 4, st, g);                                                          \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
     }
-        WFD_GO(16, 1) WFD_GO(16, 2) WFD_GO(64, 1) WFD_GO(64, 2) WFD_GO(64, 4) WFD_GO(256, 4) WFD_GO(256, 8) WFD_GO(256, 16)
+        WFD_GO(16, 1) WFD_GO(16, 2) WFD_GO(64, 1) WFD_GO(64, 2) WFD_GO(64, 4) WFD_GO(256, 2) WFD_GO(256, 4) WFD_GO(256, 8) WFD_GO(256, 16)
         WFD_GO(512, 16) WFD_GO(1024, 16)
 #undef WFD_GO
     }

@@ -222,12 +222,15 @@ __device__ __forceinline__ float lanes_nth2(float a, float b, int n) {
 }
 
 // Leaves the k best of x[0, n) (indices from `base`) at out_val / out_idx in order, places without an element as index -1.
-// gmax[it * NT + t]: the group maxima.  sum: the part's s (NaN tells of NaN or +inf).
+// gmax[it * NT + t]: the group maxima of x[head, n); head (0 or 1) elements in front are in no group.  sum: the part's s (NaN tells of NaN or +inf).
 template <class T, int NT>
-__device__ __forceinline__ void pick(const T* x, int n, int base, int k, int niter, const float* gmax, float tmax, float next, float sum, PickLds<NT>& l,
+__device__ __forceinline__ void pick(const T* x0, int n0, int base0, int head, int k, int niter, const float* gmax, float tmax, float next, float sum, PickLds<NT>& l,
                      float* out_val, int* out_idx) {
     constexpr int E = Pack<T>::N, W = NT / 64, CAND = PickLds<NT>::CAND, GROUPS = PickLds<NT>::GROUPS;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const T* x = x0 + head;
+    const int n = n0 - head, base = base0 + head;
+    const float front = head ? to_f32(x0[0]) : 0.f;
     bool slow = sum != sum;
     if (!slow) {
         const float share = W == 1 ? lanes_nth2(tmax, next, k) : lanes_nth(tmax, (k + W - 1) / W);
@@ -251,6 +254,10 @@ __device__ __forceinline__ void pick(const T* x, int n, int base, int k, int nit
                     const int at = atomicAdd(&l.groups, 1);
                     if (at < GROUPS) l.group[at] = it * NT + t;
                 }
+            }
+            if (head && t == 0 && (pass ? front > tau : front >= tau)) {
+                const int at = atomicAdd(&l.count, 1);
+                if (at < CAND) l.key[at] = order_key(front, base0);
             }
             team_sync<NT>();
             const int groups = l.groups;
@@ -287,13 +294,17 @@ __device__ __forceinline__ void pick(const T* x, int n, int base, int k, int nit
                 for (int b = 0; b < total; ++b) rank += l.key[b] > key;
                 if (rank < k) {
                     const int i = (int)~(unsigned)key;
-                    out_val[rank] = to_f32(x[i - base]);
+                    out_val[rank] = to_f32(x0[i - base0]);
                     out_idx[rank] = i;
                 }
             }
             int have = total;
             if (ties && have < k) {
                 // ties at tau in index order, E elements per thread at a time, until there are enough
+                if (head && front == tau) {
+                    if (t == 0) { out_val[have] = tau; out_idx[have] = base0; }
+                    ++have;
+                }
                 for (long p0 = 0; p0 * E < n && have < k; p0 += NT) {
                     const long i0 = (p0 + t) * E;
                     unsigned hit = 0;
@@ -332,14 +343,14 @@ __device__ __forceinline__ void pick(const T* x, int n, int base, int k, int nit
     unsigned long long last = ~0ull;
     for (int j = 0; j < k; ++j) {
         unsigned long long best = 0;
-        for (int i = t; i < n; i += NT) {
-            const unsigned long long key = order_key(to_f32(x[i]), base + i);
+        for (int i = t; i < n0; i += NT) {
+            const unsigned long long key = order_key(to_f32(x0[i]), base0 + i);
             if (key < last && key > best) best = key;
         }
         last = team_max_key<NT>(best, l.best);
         if (t == 0) {
             const int i = (int)~(unsigned)last;
-            out_val[j] = last ? to_f32(x[i - base]) : -INFINITY;
+            out_val[j] = last ? to_f32(x0[i - base0]) : -INFINITY;
             out_idx[j] = last ? i : -1;
         }
     }
@@ -416,7 +427,12 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
     const float xy = g.splits == 1 && y >= 0 && y < g.V ? to_f32(x[y]) : 0.f;
     const float c = g.inv_t * LOG2E;
     float tmax, next;
-    Stat a = walk<T, NT, PICK>(x, n, c, gmax, tmax, next);
+    const int head = off_border(x);
+    Stat a = walk<T, NT, PICK>(x + head, n - head, c, gmax, tmax, next);
+    if (head && threadIdx.x == 0) {
+        const float f[1] = {to_f32(x[0])};
+        stat_add(a, f, f[0], c);
+    }
     a = stat_team<NT>(a, c, slot);
     float* w = g.work + part * (3 + 2 * g.k);
     const bool whole = g.splits == 1;
@@ -430,7 +446,7 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
     if constexpr (PICK) {
         float* val = whole ? g.top_lp + row * g.k : w + 3;
         int* idx = whole ? g.top_idx + row * g.k : (int*)(w + 3 + g.k);
-        pick<T, NT>(x, n, lo, g.k, cdiv_dev(n, STEP), gmax, tmax, next, a.s, l, val, idx);
+        pick<T, NT>(x, n, lo, head, g.k, cdiv_dev(n - head, STEP), gmax, tmax, next, a.s, l, val, idx);
         if (whole) {
             team_sync<NT>();
             for (int j = threadIdx.x; j < g.k; j += NT) val[j] = row_lp(r, val[j], g.inv_t);
