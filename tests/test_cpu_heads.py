@@ -97,9 +97,9 @@ def test_distill_refusals():
         heads.distill_loss(X, TI.long(), TV)
     with pytest.raises(TypeError, match="teacher_value must be"):
         heads.distill_loss(X, TI, TV.to(BF16))
-    with pytest.raises(ValueError, match="does not go with"):
+    with pytest.raises(ValueError, match="go with"):
         heads.distill_loss(X, TI[:3], TV[:3])
-    with pytest.raises(ValueError, match="does not go with"):
+    with pytest.raises(ValueError, match="go with"):
         heads.distill_loss(X, TI, TV[:, :2])
     with pytest.raises(ValueError, match="at most 256"):
         heads.distill_loss(X, torch.zeros(4, 257, dtype=torch.int32), torch.zeros(4, 257))

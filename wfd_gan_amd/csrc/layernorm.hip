@@ -282,16 +282,26 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
     if constexpr (TEAMS == 1) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (r * G + t < P)
+            if (r * G + t < P) {
+                const int col = (r * G + t) * E;
+                if (gridDim.x > 1) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    out(0, (r * G + t) * E + e, sw[r][e]);
-                    out(1, (r * G + t) * E + e, sb[r][e]);
+                    for (int e = 0; e < E; e += 4) {
+                        store16(pw + col + e, pack<float>(sw[r] + e));
+                        store16(pw + N + col + e, pack<float>(sb[r] + e));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        out(0, col + e, sw[r][e]);
+                        out(1, col + e, sb[r][e]);
+                    }
                 }
+            }
         if (t < rest) { out(0, P * E + t, swl); out(1, P * E + t, sbl); }
     } else {
         // the teams meet in LDS, added in team order
-        __shared__ float meet[TEAMS][G * E];
+        __shared__ __attribute__((aligned(16))) float meet[TEAMS][G * E];
 #pragma unroll
         for (int r = 0; r <= R; ++r)
 #pragma unroll
@@ -429,15 +439,15 @@ struct LnBwdShape {
     int G, R, blocks;      // R = 0: the long form
 };
 // Teams as in the forward, with fewer pieces: a column costs three registers more.  More workgroups hide more latency and cost 8 N
-// bytes of partial sums each, written and read: at 1401 .. 2048 columns (16-bit) 1024 of them are best (69.5 us; 512: 80.9), at
-// 4096 512 (68.4; 768: 77.3, 1024: 93.1), above that one per CU.  16-bit 1401 wide: 64 x 3 pieces 70.4, 256 x 1 92.7; 5000: 256 x 3
-// 75.5, 1024 x 1 84.9.
+// bytes of partial sums each, written and read.  Measured at 200 MB of rows (us): 32768 x 1024 bf16 with 256 workgroups of 8 teams
+// 43.0 (384: 52.4, 512: 47.2), 24000 x 2048 with 1024 of one team 64.2 (768: 68.0, 512: 83.6), 12000 x 4096 with 512 62.1 (768: 67.0,
+// 256: 84.0), 6103 x 8192 with 256 71.5 (512: 78.2).  1401 wide: 64 x 3 pieces 66.0 (256 x 1: 92.7); 5000: 256 x 3 67.2 (1024 x 1: 84.9).
 LnBwdShape ln_bwd_shape(int M, int N, int E) {
     const int forms[][2] = {{16, 1}, {64, 1}, {64, 2}, {64, 3}, {256, 1}, {256, 2}, {256, 3}, {1024, 1}, {1024, 2}, {1024, 4}};
     for (auto& f : forms)
         if (N <= f[0] * f[1] * E && (f[1] * E <= 16 || f[1] == 3)) {
             const int teams = f[0] < 256 ? 512 / f[0] : 1;
-            const int most = f[0] == 1024 ? 256 : f[0] == 256 && f[1] == 1 ? 1024 : 512;
+            const int most = f[0] == 1024 || f[0] == 64 ? 256 : f[0] == 256 && f[1] == 1 ? 1024 : 512;
             const int b = cdiv(M, teams);
             return {f[0], f[1], b < most ? b : most};
         }
