@@ -162,3 +162,14 @@ def test_scratch_sizes():
                 assert L.label_scores_floats(m, n, dt, k) >= 0
     assert L.layer_norm_bwd_floats(4, 0, 0) < 0 and L.layer_norm_bwd_floats(4, 8, 7) < 0
     assert L.label_scores_floats(4, 8, 0, 9) < 0 and L.distill_floats(-1, 8, 0) < 0
+
+
+def test_train_df_flags():
+    from wfd_gan_amd import train_df
+    ns = train_df.parse_args(["X.npz"])
+    assert ns.teacher is None and ns.top_k == 0
+    ns = train_df.parse_args(["X.npz", "--teacher", "t.ckpt", "--teacher_k", "5", "--teacher_weight", "0.5", "--temperature", "3"])
+    assert (ns.teacher, ns.teacher_k, ns.teacher_weight, ns.temperature) == ("t.ckpt", 5, 0.5, 3.0)
+    for bad in (["--teacher_weight", "1.5"], ["--temperature", "0"], ["--teacher_k", "0"], ["--teacher_k", "65"], ["--top_k", "-1"]):
+        with pytest.raises(SystemExit):
+            train_df.parse_args(["X.npz"] + bad)

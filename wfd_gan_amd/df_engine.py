@@ -14,10 +14,11 @@ into its epilogue).  The Linear + BatchNorm1d + ReLU + Dropout head reuses the g
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, NamedTuple, Optional, Sequence
 
 import torch
 
+from . import heads
 from ._lib import lib
 from .engine import DF_CONVS, FlatParams, ObserverDF, observer_buffers, observer_forward
 from .plan import ACT_ELU, ACT_NONE, DM_ELU, DM_MUL, DM_RELU, NN, NT, TN, Plan, ptr, rup
@@ -43,14 +44,60 @@ def _df_specs(length: int, C: int):
     return specs, Ls
 
 
+class Distill(NamedTuple):
+    """Training from a teacher's ``k`` top logits per row (``set_teacher``): the loss is weight * T^2 * KL(teacher || student) at
+    temperature T plus (1 - weight) * cross entropy of the label (wfd_distill).  No counterpart in the reference."""
+    k: int
+    temperature: float = 2.0
+    weight: float = 0.7
+
+
+def observer_logits(df: ObserverDF, X: torch.Tensor, ws: torch.Tensor, bs: int):
+    """(first row, logits of rows [first, first + n)) of an eval-mode observer over device-resident X (N, L), in batches of
+    ``bs``; the logits are a view of a buffer that the next batch of that size writes again."""
+    N, dev, plans = X.shape[0], X.device, {}
+    for a in range(0, N, bs):
+        n = min(bs, N - a)
+        if n not in plans:
+            ob = observer_buffers(df, n, dev)
+            xin = torch.zeros(n, df.L, dtype=torch.float32, device=dev)
+            pl = Plan(ws)
+            observer_forward(pl, df, xin, df.L, 0, n, ob["Y"], ob["PO"], ob["F1"], ob["F2"], ob["LOG"], ob["ldc"])
+            plans[n] = (pl, xin, ob)
+        pl, xin, ob = plans[n]
+        xin.copy_(X[a:a + n].reshape(n, df.L))
+        pl.run()
+        yield a, ob["LOG"][:, :df.C]
+
+
+def teacher_alternatives(state: Dict[str, torch.Tensor], length: int, num_classes: int, X: torch.Tensor, k: int,
+                         workspace_mb: int = 256, bs: int = 2048):
+    """(index (N, k) int32, log probability (N, k) fp32) of a trained observer's k best classes for every row of X."""
+    df = ObserverDF(state, length, num_classes, X.device)
+    ws = torch.empty(workspace_mb * (1 << 18), dtype=torch.float32, device=X.device)
+    index = torch.empty(X.shape[0], k, dtype=torch.int32, device=X.device)
+    value = torch.empty(X.shape[0], k, dtype=torch.float32, device=X.device)
+    for a, logits in observer_logits(df, X, ws, bs):
+        top = heads.label_logprobs(logits, None, k)
+        index[a:a + logits.shape[0]] = top.top_index
+        value[a:a + logits.shape[0]] = top.top_logprob
+    return index, value
+
+
 class DFTrainEngine:
     def __init__(self, length: int, num_classes: int, batch: int, state: Dict[str, torch.Tensor], lr: float = 2e-3,
                  betas=(0.9, 0.999), eps: float = 1e-8, device="cuda:0", seed: int = 0, workspace_mb: int = 256,
-                 share: Optional["DFTrainEngine"] = None):
+                 share: Optional["DFTrainEngine"] = None, distill: Optional[Distill] = None):
         if not torch.cuda.is_available():
             raise RuntimeError("wfd_gan_amd.DFTrainEngine needs a HIP device: there is no CPU path")
         if batch < 2:
             raise ValueError("BatchNorm in training mode needs more than one row")
+        if distill is not None:
+            if not 1 <= distill.k <= min(num_classes, heads.MAX_ALTERNATIVES):
+                raise ValueError(f"distill.k must be 1 .. {min(num_classes, heads.MAX_ALTERNATIVES)}, got {distill.k}")
+            if not (0.0 <= distill.weight <= 1.0 and 0.0 < distill.temperature < float("inf")):
+                raise ValueError(f"distill needs a weight in [0, 1] and a positive finite temperature, got {distill}")
+        self.distill = distill
         self.L = lib()
         self.dev = dev = torch.device(device)
         self.length, self.C, self.B = length, num_classes, batch
@@ -101,6 +148,10 @@ class DFTrainEngine:
         b["ones"], b["nsel"], b["invb"] = torch.ones(max(B, 256), **f32), torch.full((1,), float(B), **f32), \
             torch.full((B,), 1.0 / B, **f32)
         b["loss"] = z(1)
+        if distill is not None:
+            b["t_index"] = torch.full((B, distill.k), -1, dtype=torch.int32, device=dev)
+            b["t_value"] = z(B, distill.k)
+            b["t_work"] = z(max(1, self.L.distill_floats(B, C, 0)))
         b["WT"] = [None] + [z(DF_CONVS[k][2], 8 * DF_CONVS[k][3]) for k in range(1, 7)]
         self.rpc = max(64, (B * Ls[0] + 1023) // 1024)                   # rows per chunk of the tall reductions
         nchunk = (B * Ls[0] + self.rpc - 1) // self.rpc
@@ -212,8 +263,13 @@ class DFTrainEngine:
             p.add(L.conv_wflip, ptr(w[f"{conv}.conv.weight"]), cout, cin, ptr(WT[k]))
         self._build_forward(p)
         # ---- CrossEntropyLoss (mean) and its gradient --------------------------------------------------------
-        p.add(L.masked_ce, ptr(b["LOG"]), self.ldc, B, C, ptr(b["labels"]), ptr(b["ones"]), ptr(b["nsel"]), 1.0,
-              ptr(b["CE"]), ptr(b["DLOG"]), self.ldc)
+        if self.distill is None:
+            p.add(L.masked_ce, ptr(b["LOG"]), self.ldc, B, C, ptr(b["labels"]), ptr(b["ones"]), ptr(b["nsel"]), 1.0,
+                  ptr(b["CE"]), ptr(b["DLOG"]), self.ldc)
+        else:
+            d = self.distill
+            p.add(L.distill, ptr(b["LOG"]), self.ldc, 0, B, C, ptr(b["t_index"]), ptr(b["t_value"]), d.k, d.k, ptr(b["labels"]),
+                  d.temperature, d.weight, 1.0 - d.weight, 0, 1.0 / B, ptr(b["CE"]), ptr(b["DLOG"]), self.ldc, ptr(b["t_work"]))
         p.add(L.colsum, ptr(b["CE"]), 1, B, 1, ptr(b["invb"]), ptr(b["loss"]), 0)
         # ---- backward: head --------------------------------------------------------------------------------
         p.gemm(TN, b["DLOG"], self.ldc, b["Hd2"], 512, C, 512, B, out=g["fc.weight"], ldp=512)
@@ -272,6 +328,13 @@ class DFTrainEngine:
         self.buf["X"].copy_(x.reshape(self.B, self.length).to(self.dev, torch.float32))
         self.buf["labels"].copy_(y.to(self.dev).to(torch.int32))
 
+    def set_teacher(self, index: torch.Tensor, value: torch.Tensor):
+        """The batch's rows of ``teacher_alternatives``: index (B, k), value (B, k)."""
+        if self.distill is None:
+            raise RuntimeError("set_teacher: the engine was built without distill")
+        self.buf["t_index"].copy_(index)
+        self.buf["t_value"].copy_(value)
+
     def set_masks(self, masks: Sequence[torch.Tensor]):
         """Explicit dropout keep-masks in the reference's layouts ((B, C, L) x4, (B, 512) x2), values {0, 1/(1-p)}."""
         for i, m in enumerate(masks):
@@ -318,18 +381,24 @@ class DFTrainEngine:
         correct = torch.zeros(1, dtype=torch.int32, device=self.dev)
         st = torch.cuda.current_stream().cuda_stream
         N = X.shape[0]
-        plans = {}
         y32 = y.to(self.dev).to(torch.int32).contiguous()
-        for a in range(0, N, bs):
-            n = min(bs, N - a)
-            if n not in plans:
-                ob = observer_buffers(df, n, self.dev)
-                xin = torch.zeros(n, self.length, dtype=torch.float32, device=self.dev)
-                pl = Plan(self.buf["ws"])
-                observer_forward(pl, df, xin, self.length, 0, n, ob["Y"], ob["PO"], ob["F1"], ob["F2"], ob["LOG"], ob["ldc"])
-                plans[n] = (pl, xin, ob)
-            pl, xin, ob = plans[n]
-            xin.copy_(X[a:a + n].reshape(n, self.length))
-            pl.run()
-            self.L.argmax_correct(ob["LOG"].data_ptr(), ob["ldc"], n, self.C, y32[a:a + n].data_ptr(), correct.data_ptr(), st)
+        for a, logits in observer_logits(df, X, self.buf["ws"], bs):
+            n = logits.shape[0]
+            self.L.argmax_correct(logits.data_ptr(), self.ldc, n, self.C, y32[a:a + n].data_ptr(), correct.data_ptr(), st)
         return int(correct.item()) / max(1, N)
+
+    def evaluate(self, X: torch.Tensor, y: torch.Tensor, k: int = 5, bs: int = 2048) -> Dict[str, float]:
+        """Eval-mode quality of the current parameters on device-resident X (N, L) / y (N,): ``top1`` and ``top_k`` accuracy,
+        mean ``logprob`` of the label and mean ``entropy`` of the prediction."""
+        k = min(k, self.C)
+        df = ObserverDF(self.state_dict(), self.length, self.C, self.dev)
+        y32 = y.to(self.dev).to(torch.int32).contiguous()
+        sums = torch.zeros(4, dtype=torch.float64, device=self.dev)
+        for a, logits in observer_logits(df, X, self.buf["ws"], bs):
+            lab = y32[a:a + logits.shape[0]]
+            r = heads.label_logprobs(logits, lab, k)
+            hit = r.top_index == lab[:, None]
+            sums += torch.stack([hit[:, 0].sum(), hit.sum(), r.logprob.sum(dtype=torch.float64),
+                                 r.entropy.sum(dtype=torch.float64)]).to(torch.float64)
+        top1, topk, lp, ent = (sums / max(1, X.shape[0])).tolist()
+        return {"top1": top1, "top_k": topk, "logprob": lp, "entropy": ent}

@@ -6,7 +6,9 @@ features without the burst-count column, stratified 90/10 split with random_stat
 
     python -m wfd_gan_amd.train_df <...>/feature/raw_feature_x.npz [--verbose] [--cuda_id 0]
 
-Additive flags: --num_epochs, --batch_size, --seed, --out.  The training set is resident in HBM; every step is one
+Additive flags: --num_epochs, --batch_size, --seed, --out; --teacher CKPT trains from another observer's top logits
+(--teacher_k of them per trace, --teacher_weight, --temperature), --top_k N logs the top-N accuracy, mean log probability and
+entropy on the validation traces.  The training set is resident in HBM; every step is one
 launch plan (wfd_gan_amd/df_engine.py); the only host syncs are the per-epoch accuracy read-outs.
 """
 import argparse
@@ -22,7 +24,7 @@ from sklearn.model_selection import train_test_split
 
 from . import common as cm
 from . import utils
-from .df_engine import DFTrainEngine
+from .df_engine import DFTrainEngine, Distill, teacher_alternatives
 from .model import DF
 
 num_epochs = 30          # src/train_df.py:19-20
@@ -49,7 +51,17 @@ def parse_args(argv=None):
     p.add_argument("--batch_size", type=int, default=batch_size)
     p.add_argument("--seed", type=int, default=None, help="seed for init / shuffling / dropout")
     p.add_argument("--out", default=None, help="checkpoint path (default <dModelDir>/df_<dataset name>.ckpt)")
-    return p.parse_args(argv)
+    p.add_argument("--teacher", default=None, help="checkpoint of a trained observer of the same length and classes to learn from")
+    p.add_argument("--teacher_k", type=int, default=10, help="top logits of the teacher kept per trace (at most 64)")
+    p.add_argument("--teacher_weight", type=float, default=0.7, help="share of the teacher's term, the rest is the labels'")
+    p.add_argument("--temperature", type=float, default=2.0, help="temperature of the teacher's term")
+    p.add_argument("--top_k", type=int, default=0, help="log top-k accuracy, log probability and entropy on the validation traces")
+    args = p.parse_args(argv)
+    if not 0.0 <= args.teacher_weight <= 1.0 or not 0.0 < args.temperature < float("inf"):
+        p.error("--teacher_weight must be in [0, 1] and --temperature positive")
+    if not 1 <= args.teacher_k <= 64 or not 0 <= args.top_k <= 64:
+        p.error("--teacher_k must be 1 .. 64 and --top_k 0 .. 64")
+    return args
 
 
 def main(argv=None):
@@ -88,9 +100,16 @@ def main(argv=None):
     seed = args.seed if args.seed is not None else int(torch.initial_seed() & 0x7FFFFFFF)
     N = Xtr.shape[0]
     B = min(args.batch_size, N)
-    eng = DFTrainEngine(seq_len, class_dim, B, model.state_dict(), device=device, seed=seed)
+    distill = None
+    if args.teacher is not None:
+        distill = Distill(min(args.teacher_k, class_dim), args.temperature, args.teacher_weight)
+        state = torch.load(args.teacher, map_location="cpu", weights_only=True)
+        DF(seq_len, class_dim).load_state_dict(state, strict=True)         # another length or class count is refused by name
+        t_index, t_value = teacher_alternatives(state, seq_len, class_dim, Xtr, distill.k)
+        logger.info("Learning from {}: top {} logits, temperature {}, weight {}".format(args.teacher, *distill))
+    eng = DFTrainEngine(seq_len, class_dim, B, model.state_dict(), device=device, seed=seed, distill=distill)
     n_full, tail_rows = N // B, N % B
-    tail = DFTrainEngine(seq_len, class_dim, tail_rows, {}, device=device, seed=seed + 1, share=eng) \
+    tail = DFTrainEngine(seq_len, class_dim, tail_rows, {}, device=device, seed=seed + 1, share=eng, distill=distill) \
         if tail_rows > 1 else None     # the DataLoader's ragged last batch; BatchNorm needs more than one row
     total_step = n_full + (1 if tail is not None else 0)
     gen = torch.Generator(device=device)
@@ -102,6 +121,8 @@ def main(argv=None):
             e = eng if step < n_full else tail
             idx = perm[step * B: step * B + e.B]
             e.set_batch(Xtr[idx], ytr[idx])
+            if distill is not None:
+                e.set_teacher(t_index[idx], t_value[idx])
             e.draw_masks()
             e.train_step()
             if args.verbose and (step + 1) % 50 == 0:
@@ -111,6 +132,10 @@ def main(argv=None):
         acc_train, acc_test = eng.accuracy(Xtr, ytr), eng.accuracy(Xte, yte)
         logger.info("Epoch [{}/{}] train acc: {:.4f} val accuracy: {:.4f}".format(
             epoch + 1, args.num_epochs, acc_train, acc_test))
+        if args.top_k:
+            q = eng.evaluate(Xte, yte, args.top_k)
+            logger.info("Epoch [{}/{}] val top-{}: {:.4f} log probability: {:.4f} entropy: {:.4f}".format(
+                epoch + 1, args.num_epochs, min(args.top_k, class_dim), q["top_k"], q["logprob"], q["entropy"]))
 
     path = args.out
     if path is None:
