@@ -455,14 +455,15 @@ bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
 constexpr int MAX_V = 1 << 23;
 int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
 
-// Rows stay in registers up to 1024 threads x 16 pieces; longer ones are split, and so are long ones of which there are too few to
-// give every CU its own.
+// Rows stay in registers up to 1024 threads x 16 pieces; longer ones are split, and so are the longest of these with a gradient
+// where there are too few to give every CU its own (128000 bf16 classes, us: 1 row 12.7 split, 17.0 whole; 64 rows 15.2, 20.9; 128
+// rows 23.4, 23.0; loss alone of 16 rows 12.0, 9.5; 50000 classes, 16 rows 12.1, 11.8).
 struct DistillShape {
     int splits, chunk;                // splits = 0: the register form
 };
-DistillShape distill_shape(int M, int V, int dtype) {
+DistillShape distill_shape(int M, int V, int dtype, bool grad) {
     const int E = elems_of(dtype);
-    if (V <= 1024 * 16 * E && (V <= 256 * 16 * E || M > 96)) return {0, V};
+    if (V <= 1024 * 16 * E && (V <= 512 * 16 * E || M > 96 || !grad)) return {0, V};
     const int step = 256 * U * E, steps = cdiv(V, step);
     int S = M >= 1024 ? 1 : cdiv(1024, M > 0 ? M : 1);
     if (S > steps) S = steps;
@@ -473,7 +474,7 @@ DistillShape distill_shape(int M, int V, int dtype) {
 
 template <class T, bool TWO, bool GRAD> int distill(Distill g, hipStream_t st) {
     constexpr int E = Pack<T>::N;
-    const DistillShape s = distill_shape(g.M, g.V, sizeof(T) == 4 ? WFD_F32 : WFD_BF16);
+    const DistillShape s = distill_shape(g.M, g.V, sizeof(T) == 4 ? WFD_F32 : WFD_BF16, GRAD);
     g.splits = s.splits;
     g.chunk = s.chunk;
     if (s.splits == 0) {
@@ -509,7 +510,7 @@ extern "C" {
 
 int wfd_distill_floats(int M, int V, int dtype) {
     if (!wfd_dtype_ok(dtype) || M < 0 || V <= 0 || V > MAX_V) return -1;
-    const DistillShape s = distill_shape(M, V, dtype);
+    const DistillShape s = distill_shape(M, V, dtype, true);           // the form without a gradient never needs more
     if (M == 0 || s.splits == 0) return 0;
     const long n = (long)M * (3 * s.splits + MAX_ENTRIES + 1);
     return n > 0x7fffffffL ? -1 : (int)n;

@@ -732,11 +732,12 @@ int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
 // Few classes stay in the registers of a team inside a wave: 16 lanes where they hold the row and a round per alternative is
 // cheap (16384 x 100, top 64: 38.1 us in rounds of 16 lanes, 28 in the whole wave's list; top 5: 11.5 and 14.5).  Many
 // rows up to 16384 (8192) classes take a wave each: no barriers, four times the rows in flight (16384 x 4000 bf16, top 5: 38.5 us
-// instead of 65.7).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192
-// 16-bit or 4096 fp32 classes); a row is split over workgroups (64 at most) while there are fewer than 1024 of them, and where its
-// group maxima would take more than 32 steps' room in LDS.
+// instead of 65.7).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192 16-bit or 4096 fp32 classes).  A row of more
+// than 7 steps is split over workgroups (64 at most) where there are fewer than 512 rows: a join costs a launch (32000 bf16, top 20,
+// us: 1 row 9.4 whole, 11.4 split; 600 rows 17.6, 22.0; 65000: 1 row 12.6, 11.4), and so is one whose group maxima would take
+// more than 32 steps' room in LDS.
 constexpr int FEW = 256;                  // lanes * pieces of the team form: up to 2048 16-bit or 1024 fp32 classes
-constexpr int MOST_STEPS = 32;
+constexpr int MOST_STEPS = 32, ALONE = 7;
 constexpr int NARROW = 8, MANY = 2048;    // a wave per row: up to 8 of its steps, where there are rows enough for all CUs
 struct ScoresShape {
     int splits, chunk, steps;             // splits = 0: the team form; -1: a wave per row
@@ -746,7 +747,7 @@ ScoresShape scores_shape(int M, int V, int dtype, int k) {
     if (V <= FEW * E) return {0, V, 0};
     if (V <= NARROW * 64 * U * E && M >= MANY) return {-1, V, cdiv(V, 64 * U * E)};
     const int step = 256 * U * E, steps = cdiv(V, step);
-    int S = M >= 1024 ? 1 : cdiv(1024, M > 0 ? M : 1);
+    int S = M >= 512 || steps <= ALONE ? 1 : cdiv(1024, M > 0 ? M : 1);
     if (S > steps) S = steps;
     if (S > 64) S = 64;
     if (k > 0 && S * MOST_STEPS < steps) S = cdiv(steps, MOST_STEPS);
