@@ -492,7 +492,8 @@ int wfd_argmax_correct(const float* logits, int ldl, int M, int C, const int* la
  * NO COUNTERPART IN THE REFERENCE; they stand beside its nn.BatchNorm1d (src/model.py:23), nn.CrossEntropyLoss and argmax
  * accuracy (src/train_df.py:111-157) and take rows of fp32, bf16 or fp16: `dtype` 0 fp32, 1 bf16, 2 fp16, leading dimensions
  * in elements, any alignment the type itself has.  Sums, statistics and losses are fp32 whatever the rows' type.  M = 0 is a
- * call with nothing to do.  Rows need no padding, and nothing behind a row's last element is read or written.
+ * call with nothing to do.  Rows need no padding, and nothing behind a row's last element is read or written.  Where an output may be an input (the same
+ * address), their leading dimensions are the same too.
  * `work` (fp32, as many floats as the matching _floats function says, none = may be NULL) is scratch of one call in flight:
  * calls that may overlap -- other streams, graphs that replay side by side -- each need their own.  Every result is
  * deterministic: no atomics order a sum. */
@@ -509,7 +510,7 @@ int wfd_layer_norm_bwd(const void* DY, int lddy, const void* X, int ldx, int dty
                        float* work, void* stream);
 int wfd_layer_norm_bwd_floats(int M, int N, int dtype);
 
-/* Scores over V classes (V <= 2^23) at a temperature > 0, p = softmax(x / T), in one pass over the logits:
+/* Scores over V classes (V <= 2^23) at a temperature T in [1e-6, 1e6], p = softmax(x / T), in one pass over the logits:
  *   logprob[m] = ln p(labels[m]); a label < 0 is none (0), a label >= V a mistake (NaN)
  *   entropy[m] = -sum p ln p
  *   top_logprob / top_index [M][k]: the k (0 .. 64, <= V) largest logits in order, equal ones by lower index, NaN before all
@@ -526,7 +527,7 @@ int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, c
                          const float* stat, const float* entropy, const float* d_logprob, const float* d_entropy,
                          void* dlogits, int lddl, void* stream);
 
-/* Distillation from a teacher's K (0 .. 256) top logits, with a label mixed in.  q = softmax(t_value / T) over the entries of a
+/* Distillation from a teacher's K (0 .. 256) top logits over V <= 2^23 classes, with a label mixed in; T as above.  q = softmax(t_value / T) over the entries of a
  * row of t_index / t_value [M][ldt] whose index is >= 0, p = softmax(x / T), p1 = softmax(x):
  *   loss[m] = weight * T^2 * sum_j q_j (ln q_j - ln p(index_j)) - label_weight * ln p1(labels[m])
  * and, when dlogits is not NULL, its gradient times grad_scale * row_scale[m] (row_scale NULL: 1) in the same call.  An index

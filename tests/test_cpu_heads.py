@@ -75,7 +75,7 @@ def test_label_logprobs_refusals():
         heads.label_logprobs(X, Y.long())
     with pytest.raises(ValueError, match="labels has 3"):
         heads.label_logprobs(X, Y[:3])
-    for t in (0.0, -1.0, float("inf"), float("nan")):
+    for t in (0.0, -1.0, 9e-7, 2e6, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="temperature"):
             heads.label_logprobs(X, Y, temperature=t)
     m, stat = torch.zeros(4), torch.zeros(4, 2)
@@ -124,13 +124,13 @@ def test_abi_refusals_and_empty_calls():
     fwd = lambda **o: [o.get(k, d) for k, d in dict(X=P, ldx=8, dt=1, w=P, b=P, wt=0, M=2, N=8, eps=1e-5, Y=P, ldy=8, mean=P,
                                                     rstd=P, st=0).items()]
     for o in (dict(X=0), dict(Y=0), dict(ldx=7), dict(ldy=7), dict(dt=3), dict(dt=-1), dict(wt=2), dict(M=-1), dict(N=0),
-              dict(N=(1 << 24) + 1), dict(X=P + 1), dict(eps=-1.0), dict(eps=float("nan")), dict(dt=0, Y=P + 2)):
+              dict(N=(1 << 24) + 1), dict(X=P + 1), dict(eps=-1.0), dict(eps=float("nan")), dict(dt=0, Y=P + 2), dict(ldy=9)):
         refused(L.layer_norm_fwd, *fwd(**o))
     L.layer_norm_fwd(*fwd(M=0, X=0, Y=0))
     bwd = lambda **o: [o.get(k, d) for k, d in dict(DY=P, lddy=8, X=P, ldx=8, dt=1, w=P, wt=0, mean=P, rstd=P, M=2, N=8, DX=P,
                                                     lddx=8, dw=P, db=P, work=P, st=0).items()]
     for o in (dict(DY=0), dict(X=0), dict(DX=0), dict(mean=0), dict(rstd=0), dict(work=0), dict(lddy=7), dict(lddx=7), dict(wt=2),
-              dict(N=0), dict(M=-2), dict(dt=5)):
+              dict(N=0), dict(M=-2), dict(dt=5), dict(lddx=9)):
         refused(L.layer_norm_bwd, *bwd(**o))
     sc = lambda **o: [o.get(k, d) for k, d in dict(x=P, ld=9, dt=1, M=2, V=9, y=P, T=1.0, k=3, lp=P, e=P, s=P, tl=P, ti=P, work=P,
                                                    st=0).items()]
@@ -141,13 +141,13 @@ def test_abi_refusals_and_empty_calls():
     L.label_scores(*sc(M=0, x=0))
     sb = lambda **o: [o.get(k, d) for k, d in dict(x=P, ld=9, dt=1, M=2, V=9, y=P, T=1.0, s=P, e=P, dl=P, dh=P, dx=P, lddx=9,
                                                    st=0).items()]
-    for o in (dict(x=0), dict(dx=0), dict(s=0), dict(e=0), dict(y=0), dict(ld=8), dict(lddx=8), dict(T=-1.0), dict(V=0)):
+    for o in (dict(x=0), dict(dx=0), dict(s=0), dict(e=0), dict(y=0), dict(ld=8), dict(lddx=8), dict(T=-1.0), dict(V=0), dict(lddx=10)):
         refused(L.label_scores_bwd, *sb(**o))
     L.label_scores_bwd(*sb(M=0, x=0, dx=0, s=0))
     ds = lambda **o: [o.get(k, d) for k, d in dict(x=P, ld=9, dt=1, M=2, V=9, ti=P, tv=P, ldt=4, K=4, y=P, T=1.0, w=1.0, u=0.5, rs=0,
                                                    gs=1.0, loss=P, dx=P, lddx=9, work=P, st=0).items()]
     for o in (dict(x=0), dict(loss=0), dict(ti=0), dict(tv=0), dict(ldt=3), dict(K=257, ldt=300), dict(K=-1), dict(y=0), dict(T=0.0),
-              dict(w=float("inf")), dict(u=float("nan")), dict(lddx=8), dict(ld=8), dict(dt=3), dict(V=0)):
+              dict(w=float("inf")), dict(u=float("nan")), dict(lddx=8), dict(ld=8), dict(dt=3), dict(V=0), dict(lddx=10), dict(T=1e-7)):
         refused(L.distill, *ds(**o))
     L.distill(*ds(M=0, x=0, loss=0))
 
@@ -160,6 +160,7 @@ def test_scratch_sizes():
             assert L.distill_floats(m, n, dt) >= 0
             for k in (0, 1, min(n, 64)):
                 assert L.label_scores_floats(m, n, dt, k) >= 0
+    assert L.layer_norm_bwd_floats(4096, 1 << 24, 0) == 1 << 30 and L.layer_norm_bwd_floats(4096, (1 << 24) + 1, 0) < 0
     assert L.layer_norm_bwd_floats(4, 0, 0) < 0 and L.layer_norm_bwd_floats(4, 8, 7) < 0
     assert L.label_scores_floats(4, 8, 0, 9) < 0 and L.distill_floats(-1, 8, 0) < 0
 

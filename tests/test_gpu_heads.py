@@ -310,6 +310,19 @@ def test_scores_backward(v, t):
     assert torch.equal(xd, want)
 
 
+def test_scores_of_split_rows_are_the_same_every_time():
+    """Which thread writes an alternative depends on the order of arrival; every thread holds the same statistics."""
+    from wfd_gan_amd import heads
+    for seed in (21, 22, 23):
+        x = logits_of(20, 70001, BF16, seed=seed, spread=2.5).to(DEV)
+        first = heads.label_logprobs(x, None, 9)
+        for _ in range(20):
+            again = heads.label_logprobs(x, None, 9)
+            assert torch.equal(again.top_logprob, first.top_logprob) and torch.equal(again.top_index, first.top_index)
+        # the first alternative is the maximum: its log probability is the one in stat
+        assert torch.equal(first.top_logprob[:, 0], -first.stat[:, 1])
+
+
 def test_scores_gradient_against_differences():
     from wfd_gan_amd import heads
     x = logits_of(4, 23, F32, seed=5)
@@ -384,7 +397,7 @@ def test_distill_sizes(v, t):
 
 @pytest.mark.parametrize("t", TYPES)
 def test_distill_many_rows_and_loss_alone(t):
-    for m, v, k in ((4000, 100, 8), (2500, 33, 33), (900, 1401, 256), (600, 9001, 20)):
+    for m, v, k in ((4000, 100, 8), (2500, 33, 33), (900, 1401, 256), (300, 200, 200), (600, 9001, 20)):
         x, ti, tv, y, rs = distill_inputs(m, v, k, t, seed=m)
         for temp, w, u in ((2.0, 0.5, 0.5), (1.0, 1.0, 0.0)):
             a = check_distill(x, ti, tv, y, temp, w, u, rs, 0.5, x.to(DEV))
@@ -622,3 +635,104 @@ def test_student_step_norm_product_scores_distill():
     for got, want in ((loss.loss, rows), (dW, W64.grad), (back.dx, f64.grad), (back.dweight, nw64.grad), (back.dbias, nb64.grad)):
         want = want.detach()
         assert float((got.cpu().double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Buffers of more than 2^31 elements: the last rows against the definition, in place where a call allows it."""
+    from wfd_gan_amd import heads
+    m, v = 33001, 66001                                       # 2.18e9 elements
+    x = torch.empty(m, v, dtype=BF16, device=DEV)
+    x.fill_(-3.0)
+    last = logits_of(3, v, BF16, seed=1)
+    x[-3:].copy_(last)
+    y = torch.zeros(m, dtype=torch.int32, device=DEV)
+    y[-3:] = torch.tensor([5, v - 1, -1], dtype=torch.int32, device=DEV)
+    got = heads.label_logprobs(x, y, 5)
+    want = R.scores(last, y[-3:].cpu(), 5, 1.0)
+    R.check(got.logprob[-3:], want["logprob"], want["b_logprob"], F32, "logprob")
+    assert torch.equal(got.top_index[-3:].cpu().long(), want["top_index"])
+    assert got.top_index[1000].tolist() == [0, 1, 2, 3, 4]
+    ti = torch.zeros(m, 2, dtype=torch.int32, device=DEV)
+    tv = torch.zeros(m, 2, device=DEV)
+    ti[:, 1] = v - 1
+    one = torch.ones(3, dtype=torch.float64)
+    loss, bl, d, bd = R.distill(last, ti[-3:].cpu(), tv[-3:].cpu(), None, 1.0, 1.0, 0.0, one)
+    out = heads.distill_loss(x, ti, tv, out=heads.DistillOutput(torch.empty(m, device=DEV), x, None))
+    R.check(out.loss[-3:], loss, bl, F32, "loss")
+    R.check(x[-3:], d, bd, BF16, "dlogits")
+    x[-3:].copy_(last)
+    dl = torch.ones(m, device=DEV)
+    d, bd = R.scores_backward(last, y[-3:].cpu(), got.stat[-3:], got.entropy[-3:], torch.ones(3), None, 1.0)
+    heads.label_logprobs_backward(x, y, got, dl, out=x)
+    R.check(x[-3:], d, bd, BF16, "scores gradient")
+    n = 8000                                                  # the same buffer as 272262 rows of 8000
+    rows = x.view(-1)[: (x.numel() // n) * n].view(-1, n)
+    r = rows.shape[0]
+    a, w, b, dy = norm_inputs(3, n, BF16, F32, seed=2)
+    rows.zero_()
+    rows[-3:].copy_(a)
+    wd, bd_ = w.to(DEV), b.to(DEV)
+    g = torch.zeros_like(rows)
+    g[-3:].copy_(dy)
+    got = heads.layer_norm(rows, wd, bd_)
+    yy, mean, rstd, by, bm, br = R.layer_norm(a, w, b, 1e-5)
+    R.check(got.y[-3:], yy, by, BF16, "y")
+    back = heads.layer_norm_backward(g, rows, wd, got.mean, got.rstd)
+    dx, dw, db, bdx, bdw, bdb = R.layer_norm_backward(dy, a, w, got.mean[-3:], got.rstd[-3:])
+    R.check(back.dx[-3:], dx, bdx, BF16, "dx")
+    R.check(back.dweight, dw, bdw, F32, "dweight")            # every other row has a zero gradient
+    assert float(back.dx[:1000].abs().max()) == 0 and r > 2 ** 31 // n
+    torch.cuda.synchronize()
+    del x, rows, g, got, back
+    torch.cuda.empty_cache()
+
+
+def test_captured_with_results_of_its_own():
+    """Calls that make their results inside the capture: fresh memory of the graph's own pool, alive as long as the results."""
+    from wfd_gan_amd import heads
+    s, _ = _state(7, 20, 300, 70001, BF16)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for _ in range(2):
+            heads.label_logprobs(s["logits"], s["y"], 9)
+            heads.distill_loss(s["logits"], s["ti"], s["tv"])
+            heads.layer_norm(s["x"], s["w"], s["b"])
+    torch.cuda.current_stream().wait_stream(st)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        a = heads.label_logprobs(s["logits"], s["y"], 9)
+        b = heads.distill_loss(s["logits"], s["ti"], s["tv"])
+        c = heads.layer_norm(s["x"], s["w"], s["b"])
+        d = heads.layer_norm_backward(s["dy"], s["x"], s["w"], c.mean, c.rstd)
+    for rep in range(3):
+        fresh, _ = _state(20 + rep, 20, 300, 70001, BF16)
+        for key in s:
+            s[key].copy_(fresh[key])
+        gr.replay()
+        ea = heads.label_logprobs(fresh["logits"], fresh["y"], 9)
+        eb = heads.distill_loss(fresh["logits"], fresh["ti"], fresh["tv"])
+        ec = heads.layer_norm(fresh["x"], fresh["w"], fresh["b"])
+        ed = heads.layer_norm_backward(fresh["dy"], fresh["x"], fresh["w"], ec.mean, ec.rstd)
+        torch.cuda.synchronize()
+        for got, want in ((a[:5], ea[:5]), (b[:2], eb[:2]), (c, ec), (d[:3], ed[:3])):
+            assert all(torch.equal(p, q) for p, q in zip(got, want)), rep
+
+
+@pytest.mark.parametrize("temp", [1e-6, 1e-3, 1e3, 1e6])
+def test_extreme_temperatures(temp):
+    """From one class's share to equal shares: differences come before the division."""
+    from wfd_gan_amd import heads
+    for t, v in ((F32, 100), (BF16, 5003)):
+        x = logits_of(4, v, t, seed=6)
+        x[1] = torch.finfo(t).min
+        x[2, ::3] = torch.finfo(t).min
+        y = torch.tensor([0, 1, 2, 3], dtype=torch.int32)
+        got = check_scores(x, y, 5, temp, x.to(DEV))
+        d = heads.label_logprobs_backward(x.to(DEV), y.to(DEV), got, torch.ones(4, device=DEV), temperature=temp)
+        want, bound = R.scores_backward(x, y, got.stat, got.entropy, torch.ones(4), None, temp)
+        R.check(d, want, bound, t, "dlogits")
+        ti = torch.tensor([[0, 1, 2], [1, 2, 3], [4, 5, 7], [9, 8, 7]], dtype=torch.int32)
+        tv = torch.tensor([[0.0, 1.0, 2.0]]).repeat(4, 1)
+        if temp >= 1e-3:                                       # below, T^2 times a difference / T is what is left of fp32's range
+            check_distill(x[[0, 3]], ti[[0, 3]], tv[[0, 3]], y[[0, 3]], temp, 0.5, 0.5, torch.ones(2), 1.0, x[[0, 3]].to(DEV))

@@ -133,7 +133,7 @@ __device__ __forceinline__ float row_loss(const Distill& g, long row, int lane, 
 struct GradRow {
     float m, cw, cu, r, rt;        // r = grad_scale * row_scale, rt = r w T / (sum of the teacher's exponentials)
     float R, R1, kw, ku;           // m c and m log2(e) rounded, cw and cu with what the rounding left
-    bool wide;                     // m c leaves fp32's range
+    bool wide;                     // m c beyond WIDE
 };
 template <bool TWO>
 __device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Taught& t, const RowSums& s, int y, bool wrong, float c) {
@@ -520,12 +520,13 @@ int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int*
                 const int* labels, float temperature, float weight, float label_weight, const float* row_scale,
                 float grad_scale, float* loss, void* dlogits, int lddl, float* work, void* stream) {
     const int need = wfd_distill_floats(M, V, dtype);
-    if (need < 0 || (M > 0 && need > 0 && !work) || K < 0 || K > MAX_ENTRIES || !(temperature > 0.f) || !(temperature < INFINITY))
+    if (need < 0 || (M > 0 && need > 0 && !work) || K < 0 || K > MAX_ENTRIES || !(temperature >= 1e-6f) || !(temperature <= 1e6f))
         return WFD_ERR_ARG;
     if (!(weight - weight == 0.f) || !(label_weight - label_weight == 0.f)) return WFD_ERR_ARG;
     if (M == 0) return WFD_OK;
     if (label_weight != 0.f && !labels) return WFD_ERR_ARG;
     if (!loss || !rows_ok(logits, ldl, M, V, dtype) || (dlogits && !rows_ok(dlogits, lddl, M, V, dtype))) return WFD_ERR_ARG;
+    if (dlogits == logits && lddl != ldl && M > 1) return WFD_ERR_ARG;      // would be written before it is read
     if (K > 0 && (!t_index || !t_value || (M > 1 && ldt < K))) return WFD_ERR_ARG;
     // without weight the entries are not read, and the label's term has no temperature
     if (weight == 0.f) K = 0;

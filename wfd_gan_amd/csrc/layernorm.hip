@@ -451,7 +451,8 @@ LnBwdShape ln_bwd_shape(int M, int N, int E) {
             const int b = cdiv(M, teams);
             return {f[0], f[1], b < most ? b : most};
         }
-    return {0, 0, M < 64 ? M : 64};
+    const int most = N <= 1 << 23 ? 64 : 32;              // the scratch's size stays in 31 bits
+    return {0, 0, M < most ? M : most};
 }
 
 template <class T, class WT> int ln_bwd(LnBwd g, WT* dw, WT* db, hipStream_t st) {
@@ -488,6 +489,8 @@ bool rows_ok(const void* p, int ld, int M, int N, int dtype) {
     const uintptr_t align = dtype == WFD_F32 ? 3 : 1;
     return p && !((uintptr_t)p & align) && (M <= 1 || ld >= N);
 }
+// one buffer under two row strides would be written before it is read
+bool same_rows(const void* out, int ldo, const void* in, int ldi, int M) { return out != in || ldo == ldi || M <= 1; }
 // the longest row: 32-bit column arithmetic inside the kernels keeps 16 * 1024 elements of headroom
 constexpr int LN_MAX_N = 1 << 24;
 
@@ -500,7 +503,7 @@ int wfd_layer_norm_fwd(const void* X, int ldx, int dtype, const void* weight, co
     if (!wfd_dtype_ok(dtype) || (wdtype != dtype && wdtype != WFD_F32) || M < 0 || N <= 0 || N > LN_MAX_N || !(eps >= 0.f))
         return WFD_ERR_ARG;
     if (M == 0) return WFD_OK;
-    if (!rows_ok(X, ldx, M, N, dtype) || !rows_ok(Y, ldy, M, N, dtype)) return WFD_ERR_ARG;
+    if (!rows_ok(X, ldx, M, N, dtype) || !rows_ok(Y, ldy, M, N, dtype) || !same_rows(Y, ldy, X, ldx, M)) return WFD_ERR_ARG;
     LnFwd g{X, weight, bias, Y, mean, rstd, ldx, ldy, M, N, eps};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WFD_F32) return ln_fwd<float, float>(g, st);
@@ -520,7 +523,7 @@ int wfd_layer_norm_bwd(const void* DY, int lddy, const void* X, int ldx, int dty
     if (!wfd_dtype_ok(dtype) || (wdtype != dtype && wdtype != WFD_F32) || M < 0 || N <= 0) return WFD_ERR_ARG;
     if (wfd_layer_norm_bwd_floats(M, N, dtype) < 0 || !part) return WFD_ERR_ARG;
     if (M > 0 && (!mean || !rstd || !rows_ok(DY, lddy, M, N, dtype) || !rows_ok(X, ldx, M, N, dtype) ||
-                  !rows_ok(DX, lddx, M, N, dtype)))
+                  !rows_ok(DX, lddx, M, N, dtype) || !same_rows(DX, lddx, DY, lddy, M) || !same_rows(DX, lddx, X, ldx, M)))
         return WFD_ERR_ARG;
     LnBwd g{DY, X, weight, mean, rstd, DX, part, nullptr, nullptr, lddy, ldx, lddx, M, N};
     hipStream_t st = (hipStream_t)stream;

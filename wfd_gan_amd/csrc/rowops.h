@@ -101,10 +101,13 @@ template <class T> __device__ __forceinline__ void store_piece(T* row, int i0, i
 }
 
 // ---- reductions over the lanes of a wave: DPP inside 16 lanes (no LDS latency), two lane exchanges above ----------------
+// Every step adds a pair in both of its lanes, so all lanes end with the same bits -- as long as neither addition is fused with the
+// product that made the lane's own value: contraction is off in the sums.
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 __device__ __forceinline__ float lanes_sum16(float v) {
+#pragma clang fp contract(off)
     v += dpp<0xB1>(v);      // quad_perm 1,0,3,2
     v += dpp<0x4E>(v);      // quad_perm 2,3,0,1
     v += dpp<0x141>(v);     // row_half_mirror
@@ -119,6 +122,7 @@ __device__ __forceinline__ float lanes_max16(float v) {
     return v;
 }
 template <int G> __device__ __forceinline__ float lanes_sum(float v) {
+#pragma clang fp contract(off)
     v = lanes_sum16(v);
     if constexpr (G >= 32) v += __shfl_xor(v, 16, 64);
     if constexpr (G >= 64) v += __shfl_xor(v, 32, 64);
@@ -177,10 +181,11 @@ template <int G> __device__ __forceinline__ float team_max(float a, float* slot)
 // ---- sums of exponentials about a maximum --------------------------------------------------------------------------------
 // exp((x - m) / T) = 2^(x c - m c), c = log2(e) / T.  Per element that is one fused multiply-add with the rounded R = m c and one
 // exp2; what R's rounding leaves (m c - R, exact by fma) is taken out of a whole group's sum at once, so the sums are about the true
-// maximum however large it is.  Where m c leaves fp32's range (rows at the type's lowest value) the difference comes first.
+// maximum.  Where m c is so large that the remainder would be no small exponent itself (rows at the type's lowest value, whose product
+// may even leave fp32's range) the difference comes first.
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float LOWEST = -3.402823466e38f;       // floor of a maximum: x - m stays defined for rows of nothing but -inf
 constexpr float FAINT = -1e4f;                   // an exponent whose exponential is 0: stands in where 0 * -inf would be NaN
-constexpr float WIDE = 1e38f;
+constexpr float WIDE = 1e6f;                     // m c from which on: the remainder stays below 2^-24 * 1e6 = 0.06
 
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }

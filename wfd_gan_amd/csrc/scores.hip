@@ -827,7 +827,7 @@ int wfd_label_scores(const void* logits, int ldl, int dtype, int M, int V, const
                      float* logprob, float* entropy, float* stat, float* top_logprob, int* top_index, float* work,
                      void* stream) {
     const int need = wfd_label_scores_floats(M, V, dtype, k);
-    if (need < 0 || (M > 0 && need > 0 && !work) || !(temperature > 0.f) || !(temperature < INFINITY)) return WFD_ERR_ARG;
+    if (need < 0 || (M > 0 && need > 0 && !work) || !(temperature >= 1e-6f) || !(temperature <= 1e6f)) return WFD_ERR_ARG;
     if (M == 0) return WFD_OK;
     if ((k > 0 && (!top_logprob || !top_index)) || (logprob && !labels)) return WFD_ERR_ARG;
     if (!rows_ok(logits, ldl, M, V, dtype)) return WFD_ERR_ARG;
@@ -840,11 +840,12 @@ int wfd_label_scores(const void* logits, int ldl, int dtype, int M, int V, const
 int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, const int* labels, float temperature,
                          const float* stat, const float* entropy, const float* d_logprob, const float* d_entropy,
                          void* dlogits, int lddl, void* stream) {
-    if (!wfd_dtype_ok(dtype) || M < 0 || V <= 0 || V > MAX_V || !(temperature > 0.f) || !(temperature < INFINITY))
+    if (!wfd_dtype_ok(dtype) || M < 0 || V <= 0 || V > MAX_V || !(temperature >= 1e-6f) || !(temperature <= 1e6f))
         return WFD_ERR_ARG;
     if (M == 0) return WFD_OK;
     if ((d_logprob && !labels) || (d_entropy && !entropy)) return WFD_ERR_ARG;
     if (!stat || !rows_ok(logits, ldl, M, V, dtype) || !rows_ok(dlogits, lddl, M, V, dtype)) return WFD_ERR_ARG;
+    if (dlogits == logits && lddl != ldl && M > 1) return WFD_ERR_ARG;      // would be written before it is read
     ScoresBwd g{logits, labels, stat, entropy, d_logprob, d_entropy, dlogits, ldl, lddl, M, V, 1.f / temperature, 0};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WFD_F32) return scores_bwd<float>(g, st);

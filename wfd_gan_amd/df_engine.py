@@ -95,8 +95,8 @@ class DFTrainEngine:
         if distill is not None:
             if not 1 <= distill.k <= min(num_classes, heads.MAX_ALTERNATIVES):
                 raise ValueError(f"distill.k must be 1 .. {min(num_classes, heads.MAX_ALTERNATIVES)}, got {distill.k}")
-            if not (0.0 <= distill.weight <= 1.0 and 0.0 < distill.temperature < float("inf")):
-                raise ValueError(f"distill needs a weight in [0, 1] and a positive finite temperature, got {distill}")
+            if not (0.0 <= distill.weight <= 1.0 and 1e-6 <= distill.temperature <= 1e6):
+                raise ValueError(f"distill needs a weight in [0, 1] and a temperature in [1e-6, 1e6], got {distill}")
         self.distill = distill
         self.L = lib()
         self.dev = dev = torch.device(device)

@@ -23,7 +23,6 @@ MAX_ALTERNATIVES = 64
 MAX_TEACHER_ENTRIES = 256
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INT32 = 1 << 31
-_INF = float("inf")
 
 
 class NormOutput(NamedTuple):
@@ -143,8 +142,8 @@ def _launch(dev: int, fn, *args):
 
 def _temperature(t: float, who: str) -> float:
     t = float(t)
-    if not 0.0 < t < _INF:
-        raise ValueError(f"{who}: temperature must be positive and finite, got {t}")
+    if not 1e-6 <= t <= 1e6:
+        raise ValueError(f"{who}: temperature must be in [1e-6, 1e6], got {t}")
     return t
 
 

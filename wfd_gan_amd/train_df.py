@@ -57,8 +57,8 @@ def parse_args(argv=None):
     p.add_argument("--temperature", type=float, default=2.0, help="temperature of the teacher's term")
     p.add_argument("--top_k", type=int, default=0, help="log top-k accuracy, log probability and entropy on the validation traces")
     args = p.parse_args(argv)
-    if not 0.0 <= args.teacher_weight <= 1.0 or not 0.0 < args.temperature < float("inf"):
-        p.error("--teacher_weight must be in [0, 1] and --temperature positive")
+    if not 0.0 <= args.teacher_weight <= 1.0 or not 1e-6 <= args.temperature <= 1e6:
+        p.error("--teacher_weight must be in [0, 1] and --temperature in [1e-6, 1e6]")
     if not 1 <= args.teacher_k <= 64 or not 0 <= args.top_k <= 64:
         p.error("--teacher_k must be 1 .. 64 and --top_k 0 .. 64")
     return args
