@@ -687,6 +687,30 @@ def test_rows_beyond_32_bit_offsets():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_results_beyond_the_caches_have_the_bits_of_smaller_calls(t):
+    """A gradient of 250 MB and more is stored another way, and a workgroup then has many rows: bit for bit the same as the calls on
+    100 of the rows, on rows that begin on both sides of a 4-byte border."""
+    from wfd_gan_amd import heads
+    m, v, k = 2001, 63001, 7
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(m, v, generator=g, device=DEV).to(t)
+    ti = torch.randint(0, v, (m, k), generator=g, device=DEV, dtype=torch.int32)
+    tv = torch.randn(m, k, generator=g, device=DEV)
+    y = torch.randint(0, v, (m,), generator=g, device=DEV, dtype=torch.int32)
+    a = heads.distill_loss(x, ti, tv, y, temperature=2.0, weight=0.7, label_weight=0.3)
+    alone = heads.distill_loss(x, ti, tv, y, temperature=2.0, weight=0.7, label_weight=0.3, grad=False)
+    assert torch.equal(a.loss, alone.loss)
+    got = heads.label_logprobs(x, y)
+    b = heads.label_logprobs_backward(x, y, got, torch.ones(m, device=DEV))
+    for lo in (0, 101, 1901):
+        s = slice(lo, lo + 100)
+        part = heads.distill_loss(x[s], ti[s], tv[s], y[s], temperature=2.0, weight=0.7, label_weight=0.3)
+        assert torch.equal(part.loss, a.loss[s]) and torch.equal(part.dlogits, a.dlogits[s])
+        mine = heads.LabelScores(*[f[s] if f is not None and f.shape[:1] == (m,) else f for f in got])
+        assert torch.equal(heads.label_logprobs_backward(x[s], y[s], mine, torch.ones(100, device=DEV)), b[s])
+
+
 def test_captured_with_results_of_its_own():
     """Calls that make their results inside the capture: fresh memory of the graph's own pool, alive as long as the results."""
     from wfd_gan_amd import heads

@@ -26,6 +26,7 @@ struct Distill {
     int ld, lddx, ldt, M, V, K;
     float temp, w, u, scale;
     int splits, chunk;      // split form: parts of a row, their length
+    bool past;              // the gradient is written past the caches
 };
 
 __device__ __forceinline__ void wave_sync() {           // LDS traffic between the lanes of one wave
@@ -163,7 +164,7 @@ template <bool TWO> __device__ __forceinline__ float grad_dense(const GradRow& d
     return TWO ? fmaf(d.cu, exp2_of((x - d.m) * LOG2E), v) : v;
 }
 template <class T, bool TWO>
-__device__ __forceinline__ void grad_piece(const GradRow& d, const Raw16& p, T* o, float c) {
+__device__ __forceinline__ void grad_piece(const GradRow& d, const Raw16& p, T* o, float c, bool past) {
     constexpr int E = Pack<T>::N;
     float f[E];
     if (!d.wide) {
@@ -176,7 +177,7 @@ __device__ __forceinline__ void grad_piece(const GradRow& d, const Raw16& p, T* 
 #pragma unroll
         for (int e = 0; e < E; ++e) f[e] = grad_dense<TWO>(d, elem<T>(p, e), c);
     }
-    store16(o, pack<T>(f));
+    store16(o, pack<T>(f), past);
 }
 // the elements with a target, whole again: the first occurrence of an index subtracts all of its entries, the label its own.
 // Only those of [lo, hi); runs after a barrier behind the stores that it overwrites.
@@ -231,38 +232,32 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, R == 16 ? 4 : 1) void distill_ke
     int row = blockIdx.x * TEAMS + team;
     if (row >= g.M) return;                                   // whole teams, each inside a wave
     const float inv_t = 1.f / g.temp, c = inv_t * LOG2E;
-    // piece r * G + t of the whole ones; the elements around them go to the first threads
+    // piece r * G + t of the whole ones; the elements around them go to the first threads.  How many there are holds for all rows of
+    // a workgroup: a workgroup with more than one is one of an even number, so its rows lie an even number of elements apart
     const unsigned lane_off = (unsigned)t * E;
+    const T* x = (const T*)g.X + (long)row * g.ld;
+    const int head = G > 64 ? off_border(x) : 0, P = (V - head) / E, rest = V - P * E;
     Raw16 d[R];
     float tail = -INFINITY;
-    auto fetch = [&](int r, const T* x, int h, int pieces) {
-        if (r * G + t < pieces) d[r] = load16(x + h + r * G * E + lane_off);
+    auto fetch = [&](int r, const T* from) {
+        if (r * G + t < P) d[r] = load16(from + head + r * G * E + lane_off);
     };
-    auto fetch_tail = [&](const T* x, int h, int pieces) {
-        tail = -INFINITY;
-        if (t < V - pieces * E) tail = to_f32(x[t < h ? 0 : pieces * E + t]);
+    auto fetch_tail = [&](const T* from) {
+        if (t < rest) tail = to_f32(from[t < head ? 0 : P * E + t]);
     };
     const unsigned none = raw_fill<T>(-INFINITY);
-    int head, P;
-    {
-        const T* x = (const T*)g.X + (long)row * g.ld;
-        head = G > 64 ? off_border(x) : 0;
-        P = (V - head) / E;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            d[r] = Raw16{{none, none, none, none}};
-            fetch(r, x, head, P);
-        }
-        fetch_tail(x, head, P);
+    for (int r = 0; r < R; ++r) {
+        d[r] = Raw16{{none, none, none, none}};
+        fetch(r, x);
     }
+    fetch_tail(x);
     for (int par = 0;; par ^= 1) {
         // one set of entries per row in turn: the wave of the row before may still be at its targets
         const Entries n = entries_in(lds + (G > 64 ? par : team) * 3 * g.K, g.K);
-        const T* x = (const T*)g.X + (long)row * g.ld;
         const long next = (long)row + gridDim.x;
         const bool more = G > 64 && next < g.M;
         const T* xn = x + (long)gridDim.x * g.ld;
-        const int rest = V - P * E, head_n = G > 64 ? off_border(xn) : 0, P_n = (V - head_n) / E;
         // the wave that works the entries changes from row to row: a workgroup's first wave always sits on the same SIMD
         const int lane = G > 64 ? t & 63 : t;
         const bool boss = G <= 64 || (t >> 6) == (row & (G / 64 - 1));
@@ -291,6 +286,12 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, R == 16 ? 4 : 1) void distill_ke
                 }
             }
             sums_add<TWO>(s, f, top, c);
+            // without a gradient a piece's registers are free at once.  Where a row fills the CU that pays (2048 x 128000 bf16: 110 us
+            // before, 98 so); beside other workgroups it does not (4096 x 32000: 49, 53), and the loads follow behind the sums
+            if constexpr (!GRAD && G == 1024)
+                if (more)
+#pragma unroll
+                    for (int r = 0; r < B; ++r) fetch(r0 + r, xn);
         }
         if (rest) {
             const float f[1] = {tail};
@@ -317,25 +318,24 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, R == 16 ? 4 : 1) void distill_ke
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 keep_packed(d[r]);
-                if (r * G + t < P) grad_piece<T, TWO>(k, d[r], o + head + r * G * E + lane_off, c);
-                if (more) fetch(r, xn, head_n, P_n);
+                if (r * G + t < P) grad_piece<T, TWO>(k, d[r], o + head + r * G * E + lane_off, c, g.past);
+                if (more) fetch(r, xn);
             }
             if (t < rest) o[t < head ? 0 : P * E + t] = from_f32<T>(grad_dense<TWO>(k, tail, c));
             if constexpr (G > 64) __syncthreads();
             else wave_sync();
             if (boss) grad_targets<T, TWO, L>(g, k, n, s.s == 0.f, lane, o, 0, V, y, xy, c);
         } else if constexpr (G > 64) {
-            if (more)
+            if (G < 1024 && more)
 #pragma unroll
-                for (int r = 0; r < R; ++r) fetch(r, xn, head_n, P_n);
+                for (int r = 0; r < R; ++r) fetch(r, xn);
             __syncthreads();                                  // the next row's entries and sums go where this row's were
         }
         if constexpr (G <= 64) return;
         if (!more) return;
-        fetch_tail(xn, head_n, P_n);
-        head = head_n;
-        P = P_n;
+        fetch_tail(xn);
         row = (int)next;
+        x = xn;
     }
 }
 
@@ -442,7 +442,7 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_fini
     T* o = (T*)g.DX + row * g.lddx;
 #pragma unroll
     for (int j = 0; j < U; ++j)
-        if (j * 256 + t < P) grad_piece<T, TWO>(k, d[j], o + lo + (j * 256 + t) * E, c);
+        if (j * 256 + t < P) grad_piece<T, TWO>(k, d[j], o + lo + (j * 256 + t) * E, c, g.past);
     if (t < rest) o[lo + P * E + t] = from_f32<T>(grad_dense<TWO>(k, tail, c));
     __syncthreads();
     if (t < 64) grad_targets<T, TWO, 64>(g, k, n, s.s == 0.f, t, o, lo, hi, y, xy, c);
@@ -532,7 +532,7 @@ int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int*
     if (weight == 0.f) K = 0;
     if (K == 0) temperature = 1.f;
     Distill g{logits, t_index, t_value, labels, row_scale, loss, dlogits, work, ldl, lddl, ldt, M, V, K, temperature, weight,
-              label_weight, grad_scale, 0, 0};
+              label_weight, grad_scale, 0, 0, past_caches(M, V, dtype == WFD_F32 ? 4 : 2)};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WFD_F32) return distill<float>(g, st);
     return dtype == WFD_BF16 ? distill<bf16_t>(g, st) : distill<f16_t>(g, st);

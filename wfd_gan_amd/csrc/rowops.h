@@ -31,6 +31,17 @@ template <class T> __device__ __forceinline__ void store16(T* p, const Raw16& r)
     *reinterpret_cast<Raw16u*>(p) = Raw16u{{r.v[0], r.v[1], r.v[2], r.v[3]}};
 }
 
+// A result that the 256 MiB of last-level cache cannot hold until its reader comes is better written past the caches; a smaller one
+// is not.  The gradient of `rows` x 32000 bf16 scores and a sum that reads it, us in the caches / past them: 96 MB 73 / 88, 192 MB
+// 148 / 161, 224 MB 182 / 185, 256 MB 214 / 210, 288 MB 246 / 235 (the gradient alone: 40 / 36, 73 / 70, 85 / 81, 96 / 92, 109 / 104).
+constexpr long LAST_LEVEL = 250000000;
+static inline bool past_caches(long rows, long n, int bytes) { return rows * n * bytes >= LAST_LEVEL; }
+template <class T> __device__ __forceinline__ void store16(T* p, const Raw16& r, bool past) {
+    typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
+    if (past) __builtin_nontemporal_store(u4{r.v[0], r.v[1], r.v[2], r.v[3]}, reinterpret_cast<u4*>(p));
+    else store16(p, r);
+}
+
 // 1 where a row of 16-bit values begins between two 4-byte borders
 template <class T> __device__ __forceinline__ int off_border(const T* p) {
     return sizeof(T) == 2 ? (int)((uintptr_t)p >> 1 & 1) : 0;
@@ -89,10 +100,10 @@ template <class T> __device__ __forceinline__ Raw16 load_piece(const T* row, int
     for (int e = 0; e < E; ++e) f[e] = i0 + e < n ? to_f32(row[i0 + e]) : fill;
     return pack<T>(f);
 }
-template <class T> __device__ __forceinline__ void store_piece(T* row, int i0, int n, const float* f) {
+template <class T> __device__ __forceinline__ void store_piece(T* row, int i0, int n, const float* f, bool past = false) {
     constexpr int E = Pack<T>::N;
     if (i0 + E <= n) {
-        store16(row + i0, pack<T>(f));
+        store16(row + i0, pack<T>(f), past);
         return;
     }
 #pragma unroll

@@ -32,6 +32,7 @@ struct ScoresBwd {
     int ld, lddx, M, V;
     float inv_t;
     int chunks;           // workgroups (long rows) or pieces (short rows) per row
+    bool past;            // the gradient is written past the caches
 };
 
 // order of alternatives: larger value first (NaN before every number, -0 as 0), then the lower index
@@ -689,7 +690,7 @@ template <class T> __device__ __forceinline__ void bwd_piece(const ScoresBwd& g,
     if (r.empty)
 #pragma unroll
         for (int e = 0; e < E; ++e) f[e] = 0.f;
-    store_piece(o, i0, g.V, f);
+    store_piece(o, i0, g.V, f, g.past);
 }
 // rows of many pieces: a workgroup takes U pieces per thread of one row
 template <class T> __global__ __launch_bounds__(256) void scores_bwd_kernel(ScoresBwd g) {
@@ -846,7 +847,8 @@ int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, c
     if ((d_logprob && !labels) || (d_entropy && !entropy)) return WFD_ERR_ARG;
     if (!stat || !rows_ok(logits, ldl, M, V, dtype) || !rows_ok(dlogits, lddl, M, V, dtype)) return WFD_ERR_ARG;
     if (dlogits == logits && lddl != ldl && M > 1) return WFD_ERR_ARG;      // would be written before it is read
-    ScoresBwd g{logits, labels, stat, entropy, d_logprob, d_entropy, dlogits, ldl, lddl, M, V, 1.f / temperature, 0};
+    ScoresBwd g{logits, labels, stat, entropy, d_logprob, d_entropy, dlogits, ldl, lddl, M, V, 1.f / temperature, 0,
+                past_caches(M, V, dtype == WFD_F32 ? 4 : 2)};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WFD_F32) return scores_bwd<float>(g, st);
     return dtype == WFD_BF16 ? scores_bwd<bf16_t>(g, st) : scores_bwd<f16_t>(g, st);
