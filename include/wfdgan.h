@@ -492,8 +492,9 @@ int wfd_argmax_correct(const float* logits, int ldl, int M, int C, const int* la
  * NO COUNTERPART IN THE REFERENCE; they stand beside its nn.BatchNorm1d (src/model.py:23), nn.CrossEntropyLoss and argmax
  * accuracy (src/train_df.py:111-157) and take rows of fp32, bf16 or fp16: `dtype` 0 fp32, 1 bf16, 2 fp16, leading dimensions
  * in elements, any alignment the type itself has.  Sums, statistics and losses are fp32 whatever the rows' type.  M = 0 is a
- * call with nothing to do.  Rows need no padding, and nothing behind a row's last element is read or written.  Where an output may be an input (the same
- * address), their leading dimensions are the same too.
+ * call with nothing to do; one that would take more than 2^32 threads (2^28 rows of few classes) is refused.  Rows need no
+ * padding, and nothing behind a row's last element is read or written.  Where an output may be an input (the same address),
+ * their leading dimensions are the same too; an output that lies over an input in any other way is a mistake.
  * `work` (fp32, as many floats as the matching _floats function says, none = may be NULL) is scratch of one call in flight:
  * calls that may overlap -- other streams, graphs that replay side by side -- each need their own.  Every result is
  * deterministic: no atomics order a sum. */
@@ -527,8 +528,9 @@ int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, c
                          const float* stat, const float* entropy, const float* d_logprob, const float* d_entropy,
                          void* dlogits, int lddl, void* stream);
 
-/* Distillation from a teacher's K (0 .. 256) top logits over V <= 2^23 classes, with a label mixed in; T as above.  q = softmax(t_value / T) over the entries of a
- * row of t_index / t_value [M][ldt] whose index is >= 0, p = softmax(x / T), p1 = softmax(x):
+/* Distillation from a teacher's K (0 .. 256) top logits over V <= 2^23 classes, with a label mixed in; T as above.
+ * q = softmax(t_value / T) over the entries of a row of t_index / t_value [M][ldt] whose index is >= 0, p = softmax(x / T),
+ * p1 = softmax(x) (weight 0: the entries are not looked at):
  *   loss[m] = weight * T^2 * sum_j q_j (ln q_j - ln p(index_j)) - label_weight * ln p1(labels[m])
  * and, when dlogits is not NULL, its gradient times grad_scale * row_scale[m] (row_scale NULL: 1) in the same call.  An index
  * that occurs twice counts twice.  No entry: the first term is 0; a label < 0: the second is 0 (labels may be NULL when

@@ -152,6 +152,20 @@ def test_abi_refusals_and_empty_calls():
     L.distill(*ds(M=0, x=0, loss=0))
 
 
+def test_more_threads_than_a_launch_counts():
+    """A launch counts its threads in 32 bits; calls that would need more are refused, not cut off."""
+    L = lib()
+    P, M = 4096, (1 << 31) - 1
+    calls = ((L.label_scores, lambda m, v: (P, v, 1, m, v, P, 1.0, 1, P, P, P, P, P, P, 0), (9, 4000, 20000)),
+             (L.label_scores_bwd, lambda m, v: (P, v, 1, m, v, P, 1.0, P, P, P, P, P, v, 0), (9, 4000, 20000)),
+             (L.distill, lambda m, v: (P, v, 1, m, v, P, P, 4, 4, P, 1.0, 1.0, 0.5, 0, 1.0, P, P, v, P, 0), (9, 300, 200000)),
+             (L.layer_norm_fwd, lambda m, n: (P, n, 1, P, P, 0, m, n, 1e-5, P, n, P, P, 0), (200000,)))
+    for fn, args, sizes in calls:
+        for v in sizes:
+            with pytest.raises(WfdError, match="bad argument"):
+                fn(*args(M, v))
+
+
 def test_scratch_sizes():
     L = lib()
     for m, n in ((0, 5), (1, 1), (4096, 1024), (100000, 100), (3, 1 << 20)):

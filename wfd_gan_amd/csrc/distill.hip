@@ -448,12 +448,7 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_fini
     if (t < 64) grad_targets<T, TWO, 64>(g, k, n, s.s == 0.f, t, o, lo, hi, y, xy, c);
 }
 
-bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
-    const uintptr_t align = dtype == WFD_F32 ? 3 : 1;
-    return p && !((uintptr_t)p & align) && (M <= 1 || ld >= V);
-}
 constexpr int MAX_V = 1 << 23;
-int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
 
 // Rows stay in registers up to 1024 threads x 16 pieces; longer ones are split, and so are the longest of these with a gradient
 // where there are too few to give every CU its own (128000 bf16 classes, us: 1 row 12.7 split, 17.0 whole; 64 rows 15.2, 20.9; 128
@@ -482,8 +477,9 @@ template <class T, bool TWO, bool GRAD> int distill(Distill g, hipStream_t st) {
     if (g.V <= G * R * E) {                                                                                              \
         constexpr int TEAMS = G < 256 ? 256 / G : 1;                                                                     \
         const int blocks = cdiv(g.M, TEAMS), most = G > 64 ? 256 * (16 / R) * (1024 / G) : blocks;                       \
-        hipLaunchKernelGGL((distill_kernel<T, G, R, TWO, GRAD>), dim3(blocks < most ? blocks : most), dim3(G < 256 ? 256 : G), \
-                           (size_t)(TEAMS > 1 ? TEAMS : 2) * 3 * g.K * 4, st, g);                                                          \
+        if (!launchable(blocks < most ? blocks : most, G < 256 ? 256 : G)) return WFD_ERR_ARG;                           \
+        hipLaunchKernelGGL((distill_kernel<T, G, R, TWO, GRAD>), dim3(blocks < most ? blocks : most),                    \
+                           dim3(G < 256 ? 256 : G), (size_t)(TEAMS > 1 ? TEAMS : 2) * 3 * g.K * 4, st, g);               \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
     }
@@ -492,7 +488,7 @@ template <class T, bool TWO, bool GRAD> int distill(Distill g, hipStream_t st) {
 #undef WFD_GO
     }
     const int parts = g.DX ? cdiv(g.V, 256 * U * E) : 1;
-    if ((long)g.M * s.splits > 0x7fffffffL || (long)g.M * parts > 0x7fffffffL) return WFD_ERR_ARG;
+    if (!launchable((long)g.M * s.splits, 256) || !launchable((long)g.M * parts, 256)) return WFD_ERR_ARG;
     hipLaunchKernelGGL((distill_part_kernel<T, TWO>), dim3(g.M * s.splits), dim3(256), 0, st, g);
     WFD_CHECK_LAUNCH();
     hipLaunchKernelGGL((distill_finish_kernel<T, TWO>), dim3(g.M * parts), dim3(256), (size_t)3 * g.K * 4, st, g);
@@ -526,7 +522,7 @@ int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int*
     if (M == 0) return WFD_OK;
     if (label_weight != 0.f && !labels) return WFD_ERR_ARG;
     if (!loss || !rows_ok(logits, ldl, M, V, dtype) || (dlogits && !rows_ok(dlogits, lddl, M, V, dtype))) return WFD_ERR_ARG;
-    if (dlogits == logits && lddl != ldl && M > 1) return WFD_ERR_ARG;      // would be written before it is read
+    if (!same_rows(dlogits, lddl, logits, ldl, M)) return WFD_ERR_ARG;
     if (K > 0 && (!t_index || !t_value || (M > 1 && ldt < K))) return WFD_ERR_ARG;
     // without weight the entries are not read, and the label's term has no temperature
     if (weight == 0.f) K = 0;

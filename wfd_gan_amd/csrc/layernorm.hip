@@ -418,7 +418,7 @@ template <class T, class WT> int ln_fwd(const LnFwd& g, hipStream_t st) {
 #define LN_GO(G, R)                                                                                                      \
     if (g.N <= G * R * E) {                                                                                              \
         constexpr int TEAMS = G < 256 ? 256 / G : 1, NT = G < 256 ? 256 : G;                                             \
-        const int all = cdiv(g.M, TEAMS), most = NT == 1024 ? 512 : G == 256 && R == 1 ? 2048 : 1024;                                                        \
+        const int all = cdiv(g.M, TEAMS), most = NT == 1024 ? 512 : G == 256 && R == 1 ? 2048 : 1024;                    \
         hipLaunchKernelGGL((ln_fwd_kernel<T, WT, G, R>), dim3(all < most ? all : most), dim3(NT), 0, st, g);             \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
@@ -430,6 +430,7 @@ template <class T, class WT> int ln_fwd(const LnFwd& g, hipStream_t st) {
     if constexpr (E == 4) { LN_GO(256, 4) } else { LN_GO(1024, 1) }
     LN_GO(1024, 2) LN_GO(1024, 4)
 #undef LN_GO
+    if (!launchable(g.M, 1024)) return WFD_ERR_ARG;
     hipLaunchKernelGGL((ln_fwd_long_kernel<T, WT>), dim3(g.M), dim3(1024), 0, st, g);
     WFD_CHECK_LAUNCH();
     return WFD_OK;
@@ -471,6 +472,7 @@ template <class T, class WT> int ln_bwd(LnBwd g, WT* dw, WT* db, hipStream_t st)
             break;
 #undef LN_GO
         default:
+            if (!launchable(g.M, 1024)) return WFD_ERR_ARG;
             // the columns first: dx may lie over dy or x
             hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3(cdiv(g.N, 256), s.blocks), dim3(256), 0, st, g);
             hipLaunchKernelGGL((ln_bwd_long_kernel<T, WT>), dim3(g.M), dim3(1024), 0, st, g);
@@ -484,13 +486,6 @@ template <class T, class WT> int ln_bwd(LnBwd g, WT* dw, WT* db, hipStream_t st)
     return WFD_OK;
 }
 
-int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
-bool rows_ok(const void* p, int ld, int M, int N, int dtype) {
-    const uintptr_t align = dtype == WFD_F32 ? 3 : 1;
-    return p && !((uintptr_t)p & align) && (M <= 1 || ld >= N);
-}
-// one buffer under two row strides would be written before it is read
-bool same_rows(const void* out, int ldo, const void* in, int ldi, int M) { return out != in || ldo == ldi || M <= 1; }
 // the longest row: 32-bit column arithmetic inside the kernels keeps 16 * 1024 elements of headroom
 constexpr int LN_MAX_N = 1 << 24;
 

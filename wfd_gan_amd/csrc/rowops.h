@@ -12,6 +12,16 @@ typedef _Float16 f16_t;
 
 static inline bool wfd_dtype_ok(int t) { return t >= WFD_F32 && t <= WFD_F16; }
 
+static inline int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }     // of one 16-byte piece
+static inline bool rows_ok(const void* p, int ld, int M, int N, int dtype) {
+    const uintptr_t align = dtype == WFD_F32 ? 3 : 1;
+    return p && !((uintptr_t)p & align) && (M <= 1 || ld >= N);
+}
+// one buffer under two row strides would be written before it is read
+static inline bool same_rows(const void* out, int ldo, const void* in, int ldi, int M) { return out != in || ldo == ldi || M <= 1; }
+// a launch counts its threads in 32 bits
+static inline bool launchable(long blocks, int threads) { return blocks * threads <= 0xffffffffL; }
+
 __device__ __forceinline__ int cdiv_dev(int a, int b) { return (a + b - 1) / b; }
 
 template <class T> struct Pack { static constexpr int N = 16 / (int)sizeof(T); };   // elements of one 16-byte piece

@@ -3,6 +3,9 @@
 //   logprob(y) = z_y - ln s,   H = ln s - (sum z exp z) / s,   p = exp z / s
 //   d x_i = (1 / T) (g ([i = y] - p_i) - h p_i (ln p_i + H))
 // Sums are fp32 about the row's own maximum; (m, ln s) stay apart in `stat`, so that differences to the maximum are exact.
+// Bound by memory: the forward reads a row once and writes a few words, the gradient reads and writes it once.  So one walk does all:
+// running maximum and sums, one exponential and four other operations per class, and for the alternatives no more than one maximum per
+// 4 pieces; the few groups that can hold an alternative are read again from the caches.
 // A row that holds nothing but -inf: logprob -inf, entropy 0, gradient 0.  NaN and +inf make the row's numbers NaN.
 #include "rowops.h"
 
@@ -138,13 +141,13 @@ __device__ __forceinline__ void row_store(const Scores& g, long row, const RowEn
 }
 
 // ---- alternatives of a part of a row --------------------------------------------------------------------------------------
-// Every thread has left the largest value of each group of pieces that it visited in LDS.  The (k / waves)-th largest thread
-// maximum of a wave (alone in its workgroup, a wave counts each thread's two largest), the smallest such of all waves, is a value that at least k elements reach; so is any wave's k-th largest (a
-// part may be so short that the last waves have none).  The larger of the two is tau.  Only groups whose maximum
-// reaches tau are read again, an element per thread; what reaches tau there goes to a list (expected length: k and a few), whose
-// order is found by counting.  When more than the lists hold reach tau, they are ties at tau but for a few: those above tau are listed and the
-// rest is filled up by walking the ties in index order.  Rows with NaN, and rows that defeat even this (thousands above
-// tau), take the k largest one after another.
+// Every thread has left the largest value of each group of pieces that it visited in LDS.  The (k / waves)-th largest thread maximum
+// of a wave (alone in its workgroup, a wave counts each thread's two largest), the smallest such of all waves, is a value that at
+// least k elements reach; so is any wave's k-th largest (a part may be so short that the last waves have none).  The larger of the
+// two is tau.  Only groups whose maximum reaches tau are read again, an element per thread; what reaches tau there goes to a list
+// (expected length: k and a few), whose order is found by counting.  When more than the lists hold reach tau, they are ties at tau but
+// for a few: those above tau are listed and the rest is filled up by walking the ties in index order.  Rows with NaN, and rows that
+// defeat even this (thousands above tau), take the k largest one after another.
 constexpr int U = 4;                      // pieces per group
 
 template <int NT> struct PickLds {
@@ -223,10 +226,11 @@ __device__ __forceinline__ float lanes_nth2(float a, float b, int n) {
 }
 
 // Leaves the k best of x[0, n) (indices from `base`) at out_val / out_idx in order, places without an element as index -1.
-// gmax[it * NT + t]: the group maxima of x[head, n); head (0 or 1) elements in front are in no group.  sum: the part's s (NaN tells of NaN or +inf).
+// gmax[it * NT + t]: the group maxima of x[head, n); head (0 or 1) elements in front are in no group.  sum: the part's s (NaN tells
+// of NaN or +inf).
 template <class T, int NT>
-__device__ __forceinline__ void pick(const T* x0, int n0, int base0, int head, int k, int niter, const float* gmax, float tmax, float next, float sum, PickLds<NT>& l,
-                     float* out_val, int* out_idx) {
+__device__ __forceinline__ void pick(const T* x0, int n0, int base0, int head, int k, int niter, const float* gmax, float tmax,
+                                     float next, float sum, PickLds<NT>& l, float* out_val, int* out_idx) {
     constexpr int E = Pack<T>::N, W = NT / 64, CAND = PickLds<NT>::CAND, GROUPS = PickLds<NT>::GROUPS;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const T* x = x0 + head;
@@ -723,20 +727,15 @@ template <class T> __global__ __launch_bounds__(256) void scores_bwd_few_kernel(
     bwd_piece(g, bwd_row(g, row), d, (T*)g.DX + row * g.lddx, i0);
 }
 
-bool rows_ok(const void* p, int ld, int M, int V, int dtype) {
-    const uintptr_t align = dtype == WFD_F32 ? 3 : 1;
-    return p && !((uintptr_t)p & align) && (M <= 1 || ld >= V);
-}
 constexpr int MAX_V = 1 << 23, MAX_K = 64;   // 64 parts of 32 fp32 steps
-int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }
 
 // Few classes stay in the registers of a team inside a wave: 16 lanes where they hold the row and a round per alternative is
 // cheap (16384 x 100, top 64: 38.1 us in rounds of 16 lanes, 28 in the whole wave's list; top 5: 11.5 and 14.5).  Many
 // rows up to 16384 (8192) classes take a wave each: no barriers, four times the rows in flight (16384 x 4000 bf16, top 5: 38.5 us
-// instead of 65.7).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192 16-bit or 4096 fp32 classes).  A row of more
-// than 7 steps is split over workgroups (64 at most) where there are fewer than 512 rows: a join costs a launch (32000 bf16, top 20,
-// us: 1 row 9.4 whole, 11.4 split; 600 rows 17.6, 22.0; 65000: 1 row 12.6, 11.4), and so is one whose group maxima would take
-// more than 32 steps' room in LDS.
+// instead of 65.7).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192 16-bit or 4096 fp32 classes).  A row of
+// more than 7 steps is split over workgroups (64 at most) where there are fewer than 512 rows: a join costs a launch (32000 bf16, top
+// 20, us: 1 row 9.4 whole, 11.4 split; 600 rows 17.6, 22.0; 65000: 1 row 12.6, 11.4), and so is one whose group maxima would
+// take more than 32 steps' room in LDS.
 constexpr int FEW = 256;                  // lanes * pieces of the team form: up to 2048 16-bit or 1024 fp32 classes
 constexpr int MOST_STEPS = 32, ALONE = 7;
 constexpr int NARROW = 8, MANY = 2048;    // a wave per row: up to 8 of its steps, where there are rows enough for all CUs
@@ -765,6 +764,7 @@ template <class T> int scores(Scores g, hipStream_t st) {
     if (s.splits == 0) {
 #define WFD_FEW(G, R)                                                                                                    \
     if (g.V <= G * R * E && (G == 64 || g.k <= 16)) {                                                                    \
+        if (!launchable(cdiv(g.M, 256 / G), 256)) return WFD_ERR_ARG;                                                    \
         hipLaunchKernelGGL((scores_few_kernel<T, G, R>), dim3(cdiv(g.M, 256 / G)), dim3(256), 0, st, g);                 \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
@@ -774,6 +774,7 @@ template <class T> int scores(Scores g, hipStream_t st) {
     }
     if (s.splits < 0) {
         g.splits = 1;
+        if (!launchable(g.M, 64)) return WFD_ERR_ARG;
         if (g.k > 0)
             hipLaunchKernelGGL((scores_kernel<T, 64, true>), dim3(g.M), dim3(64), (size_t)s.steps * 256, st, g);
         else
@@ -782,7 +783,7 @@ template <class T> int scores(Scores g, hipStream_t st) {
         return WFD_OK;
     }
     const long parts = (long)g.M * s.splits;
-    if (parts > 0x7fffffffL) return WFD_ERR_ARG;
+    if (!launchable(parts, 256)) return WFD_ERR_ARG;
     if (g.k > 0)
         hipLaunchKernelGGL((scores_kernel<T, 256, true>), dim3((unsigned)parts), dim3(256), (size_t)s.steps * 1024, st, g);
     else
@@ -800,12 +801,12 @@ template <class T> int scores_bwd(ScoresBwd g, hipStream_t st) {
     if (g.V > STEP / 2) {
         g.chunks = cdiv(g.V, STEP);
         const long blocks = (long)g.M * g.chunks;
-        if (blocks > 0x7fffffffL) return WFD_ERR_ARG;
+        if (!launchable(blocks, 256)) return WFD_ERR_ARG;
         hipLaunchKernelGGL(scores_bwd_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, g);
     } else {
         g.chunks = cdiv(g.V, E);
         const long blocks = ((long)g.M * g.chunks + 255) / 256;
-        if (blocks > 0x7fffffffL) return WFD_ERR_ARG;
+        if (!launchable(blocks, 256)) return WFD_ERR_ARG;
         hipLaunchKernelGGL(scores_bwd_few_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, g);
     }
     WFD_CHECK_LAUNCH();
@@ -846,7 +847,7 @@ int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, c
     if (M == 0) return WFD_OK;
     if ((d_logprob && !labels) || (d_entropy && !entropy)) return WFD_ERR_ARG;
     if (!stat || !rows_ok(logits, ldl, M, V, dtype) || !rows_ok(dlogits, lddl, M, V, dtype)) return WFD_ERR_ARG;
-    if (dlogits == logits && lddl != ldl && M > 1) return WFD_ERR_ARG;      // would be written before it is read
+    if (!same_rows(dlogits, lddl, logits, ldl, M)) return WFD_ERR_ARG;
     ScoresBwd g{logits, labels, stat, entropy, d_logprob, d_entropy, dlogits, ldl, lddl, M, V, 1.f / temperature, 0,
                 past_caches(M, V, dtype == WFD_F32 ? 4 : 2)};
     hipStream_t st = (hipStream_t)stream;
