@@ -66,6 +66,22 @@ def test_without_a_teacher_nothing_changes():
             _engine(200, 10, 16, distill=bad)
 
 
+def test_refusals_of_a_teachers_rows_and_of_k():
+    """A teacher's row for all traces would be spread over the batch without a word; the best alternative is what top1 counts."""
+    from wfd_gan_amd.df_engine import Distill
+    e = _engine(96, 9, 6, distill=Distill(4))
+    for bad in ((1, 4), (4,), (6, 3), (7, 4)):
+        with pytest.raises(ValueError, match="set_teacher"):
+            e.set_teacher(torch.zeros(bad, dtype=torch.int32), torch.zeros(bad))
+    with pytest.raises(ValueError, match="set_teacher"):
+        e.set_teacher(torch.zeros(6, 4, dtype=torch.int32), torch.zeros(1, 4))
+    X, y = torch.rand(5, 96, device=DEV), torch.zeros(5, dtype=torch.int32, device=DEV)
+    for k in (0, -1, 65):
+        with pytest.raises(ValueError, match="evaluate: k"):
+            e.evaluate(X, y, k)
+    assert e.evaluate(X, y, 64).keys() == {"top1", "top_k", "logprob", "entropy"}
+
+
 @pytest.mark.parametrize("C,k", [(7, 3), (100, 5), (3, 5)])
 def test_evaluate_and_teacher_alternatives(C, k):
     from wfd_gan_amd.df_engine import teacher_alternatives

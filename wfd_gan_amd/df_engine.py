@@ -332,6 +332,9 @@ class DFTrainEngine:
         """The batch's rows of ``teacher_alternatives``: index (B, k), value (B, k)."""
         if self.distill is None:
             raise RuntimeError("set_teacher: the engine was built without distill")
+        if index.shape != self.buf["t_index"].shape or value.shape != index.shape:
+            raise ValueError(f"set_teacher: index {tuple(index.shape)} and value {tuple(value.shape)}, expected "
+                             f"{tuple(self.buf['t_index'].shape)} each")
         self.buf["t_index"].copy_(index)
         self.buf["t_value"].copy_(value)
 
@@ -384,12 +387,14 @@ class DFTrainEngine:
         y32 = y.to(self.dev).to(torch.int32).contiguous()
         for a, logits in observer_logits(df, X, self.buf["ws"], bs):
             n = logits.shape[0]
-            self.L.argmax_correct(logits.data_ptr(), self.ldc, n, self.C, y32[a:a + n].data_ptr(), correct.data_ptr(), st)
+            self.L.argmax_correct(logits.data_ptr(), logits.stride(0), n, self.C, y32[a:a + n].data_ptr(), correct.data_ptr(), st)
         return int(correct.item()) / max(1, N)
 
     def evaluate(self, X: torch.Tensor, y: torch.Tensor, k: int = 5, bs: int = 2048) -> Dict[str, float]:
         """Eval-mode quality of the current parameters on device-resident X (N, L) / y (N,): ``top1`` and ``top_k`` accuracy,
         mean ``logprob`` of the label and mean ``entropy`` of the prediction."""
+        if not 1 <= k <= heads.MAX_ALTERNATIVES:
+            raise ValueError(f"evaluate: k must be 1 .. {heads.MAX_ALTERNATIVES}, got {k}")
         k = min(k, self.C)
         df = ObserverDF(self.state_dict(), self.length, self.C, self.dev)
         y32 = y.to(self.dev).to(torch.int32).contiguous()
