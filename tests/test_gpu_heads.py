@@ -83,6 +83,32 @@ def test_norm_many_rows(t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n", [3, 5, 64, 127, 129, 513, 1000, 1401, 2047, 2049, 4096, 4099, 6001, 8192, 8200, 16384])
+def test_norm_backward_on_both_sides_of_few_rows(n, t):
+    """Few rows are done in one launch, more with partial sums: every team's form on both sides of the borders, with strides, in
+    place, and without some of the weights' gradients."""
+    from wfd_gan_amd import heads
+    few = 1024 if t != F32 or n <= 2048 else 512
+    for m in (few, few + 1):
+        x, w, b, dy = norm_inputs(m, n, t, F32, seed=n + m)
+        xd, dyd, wd = strided(x, 3, 1), strided(dy, 2, 1), dev(w)
+        check_norm(x, w, b, dy, 1e-5, xd, dyd)
+        r = heads.layer_norm(xd, wd, dev(b))
+        full = heads.layer_norm_backward(dyd, xd, wd, r.mean, r.rstd)
+        for where in ("dy", "x"):
+            dd, xx = dyd.clone(memory_format=torch.contiguous_format), xd.clone(memory_format=torch.contiguous_format)
+            o = full._replace(dx=dd if where == "dy" else xx, dweight=torch.empty_like(wd), dbias=torch.empty_like(wd))
+            g = heads.layer_norm_backward(dd, xx, wd, r.mean, r.rstd, out=o)
+            assert torch.equal(g.dx, full.dx) and torch.equal(g.dweight, full.dweight) and torch.equal(g.dbias, full.dbias)
+        for dw, db in ((None, full.dbias), (full.dweight, None), (None, None)):
+            o = full._replace(dx=torch.empty_like(full.dx), dweight=None if dw is None else torch.empty_like(dw),
+                              dbias=None if db is None else torch.empty_like(db))
+            g = heads.layer_norm_backward(dyd, xd, wd, r.mean, r.rstd, out=o)
+            assert torch.equal(g.dx, full.dx)
+            assert all(a is None if c is None else torch.equal(a, c) for a, c in ((g.dweight, dw), (g.dbias, db)))
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("n", [3, 64, 1401, 2048, 9000, 33001])
 def test_norm_strides_and_missing_weights(n, t):
     for k, (w, b) in enumerate(((True, False), (False, True), (False, False))):

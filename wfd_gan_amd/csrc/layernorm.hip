@@ -272,7 +272,7 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
             if (row + step < g.M) fetch(n, row + step);
         k = n;
     }
-    // the workgroup's sums: to its place in `part`, or, if it is the only one, to the gradients
+    // the workgroup's sums: to its place in `part`, or, if it is the only one (32 rows of no whole piece), to the gradients
     float* pw = g.part + (long)blockIdx.x * 2 * N;
     auto out = [&](int h, int col, float v) {
         if (gridDim.x > 1) {
@@ -286,22 +286,14 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (r * G + t < P) {
-                const int col = (r * G + t) * E;
-                if (gridDim.x > 1) {
+                const int col = (r * G + t) * E;          // never alone: so few rows have a form of their own
 #pragma unroll
-                    for (int e = 0; e < E; e += 4) {
-                        store16(pw + col + e, pack<float>(sw[r] + e));
-                        store16(pw + N + col + e, pack<float>(sb[r] + e));
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        out(0, col + e, sw[r][e]);
-                        out(1, col + e, sb[r][e]);
-                    }
+                for (int e = 0; e < E; e += 4) {
+                    store16(pw + col + e, pack<float>(sw[r] + e));
+                    store16(pw + N + col + e, pack<float>(sb[r] + e));
                 }
             }
-        if (t < rest) { out(0, P * E + t, swl); out(1, P * E + t, sbl); }
+        if (t < rest) { pw[P * E + t] = swl; pw[N + P * E + t] = sbl; }
     } else {
         // the teams meet in LDS, added in team order
         __shared__ __attribute__((aligned(16))) float meet[TEAMS][G * E];
@@ -327,6 +319,123 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
                 }
             }
     }
+}
+
+// ---- backward of few rows: dx and the column sums in one launch ---------------------------------------------------------
+// The first workgroups take 8 pieces of columns each and walk down all rows, the others take the rows: x and dy are read twice, but
+// there are no partial sums and no second launch (two where dx lies over x or dy).
+template <class T, class WT, int NT> __device__ __forceinline__ void bwd_columns(const LnBwd& g, int block) {
+    constexpr int E = Pack<T>::N, W = NT / 64, STEP = NT / 8, U = 4;
+    __shared__ float meet[W][2][8 * E];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, N = g.N;
+    // the row's last piece ends where the row does: columns that it shares with the piece before are that one's
+    auto column = [&](int p) { return min((block * 8 + p) * E, N - E); };
+    const int col = column(t & 7);
+    float sw[E], sb[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sw[e] = sb[e] = 0.f;
+    if ((block * 8 + (t & 7)) * E < N)
+        for (int r0 = t >> 3; r0 < g.M; r0 += U * STEP) {
+            Raw16 x[U], dy[U];
+            float mean[U], rstd[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const long row = r0 + j * STEP;
+                x[j] = dy[j] = Raw16{{0u, 0u, 0u, 0u}};
+                mean[j] = rstd[j] = 0.f;                  // a row past the last adds 0
+                if (row < g.M) {
+                    x[j] = load16((const T*)g.X + row * g.ldx + col);
+                    dy[j] = load16((const T*)g.DY + row * g.lddy + col);
+                    mean[j] = g.mean[row];
+                    rstd[j] = g.rstd[row];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float d = elem<T>(dy[j], e);
+                    sw[e] = fmaf(d, (elem<T>(x[j], e) - mean[j]) * rstd[j], sw[e]);
+                    sb[e] += d;
+                }
+        }
+    // lanes 8 apart hold the same columns
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int o = 8; o < 64; o <<= 1) {
+            sw[e] += __shfl_xor(sw[e], o, 64);
+            sb[e] += __shfl_xor(sb[e], o, 64);
+        }
+    if (lane < 8)
+#pragma unroll
+        for (int e = 0; e < E; ++e) { meet[wave][0][lane * E + e] = sw[e]; meet[wave][1][lane * E + e] = sb[e]; }
+    __syncthreads();
+    const int h = t / (8 * E), c = t % (8 * E), at = column(c / E) + c % E;
+    WT* to = (WT*)(h ? g.db : g.dw);
+    if (h < 2 && at >= (block * 8 + c / E) * E && to) {   // never true for a piece behind the last
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v += meet[w][h][c];
+        to[at] = from_f32<WT>(v);
+    }
+}
+template <class T, class WT, int G, int R> __device__ __forceinline__ void bwd_row(const LnBwd& g, int block) {
+    constexpr int E = Pack<T>::N, TEAMS = G < 256 ? 256 / G : 1;
+    __shared__ float slot[2 * (G > 64 ? G / 64 : 1)];
+    const int t = TEAMS > 1 ? threadIdx.x % G : threadIdx.x;
+    const int N = g.N, P = N / E, rest = N - P * E;
+    const long row = (long)block * TEAMS + (TEAMS > 1 ? threadIdx.x / G : 0);
+    if (row >= g.M) return;                               // whole teams, each inside a wave
+    const T* x = (const T*)g.X + row * g.ldx;
+    const T* dy = (const T*)g.DY + row * g.lddy;
+    T* o = (T*)g.DX + row * g.lddx;
+    const float mean = g.mean[row], rstd = g.rstd[row], inv = 1.f / (float)N;
+    float xh[R][E], v[R][E], xhl = 0.f, vl = 0.f, a = 0.f, b = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) xh[r][e] = v[r][e] = 0.f;
+        if (r * G + t < P) {
+            const Raw16 dx_ = load16(x + (r * G + t) * E), dd = load16(dy + (r * G + t) * E);
+            load_weights<WT, E>(v[r], (const WT*)g.W, (r * G + t) * E, 1.f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                xh[r][e] = (elem<T>(dx_, e) - mean) * rstd;
+                v[r][e] *= elem<T>(dd, e);
+            }
+        }
+    }
+    if (t < rest) {
+        xhl = (to_f32(x[P * E + t]) - mean) * rstd;
+        vl = to_f32(dy[P * E + t]) * (g.W ? to_f32(((const WT*)g.W)[P * E + t]) : 1.f);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            a += v[r][e];
+            b = fmaf(v[r][e], xh[r][e], b);
+        }
+    a += vl;
+    b = fmaf(vl, xhl, b);
+    const float2 c = team_sum2<G>(a, b, slot);
+    const float c1 = c.x * inv, c2 = c.y * inv;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (r * G + t < P) {
+            float f[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] = rstd * (v[r][e] - fmaf(xh[r][e], c2, c1));
+            store16(o + (r * G + t) * E, pack<T>(f));
+        }
+    if (t < rest) o[P * E + t] = from_f32<T>(rstd * (vl - fmaf(xhl, c2, c1)));
+}
+template <class T, class WT, int G, int R>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void ln_bwd_few_kernel(LnBwd g, int first) {
+    const int block = blockIdx.x + first, columns = cdiv_dev(g.N, 8 * Pack<T>::N);
+    if (block < columns) bwd_columns<T, WT, (G < 256 ? 256 : G)>(g, block);
+    else bwd_row<T, WT, G, R>(g, block - columns);
 }
 
 // rows too long for the registers: dx with two walks over the row ...
@@ -441,29 +550,62 @@ template <class T, class WT> int ln_fwd(const LnFwd& g, hipStream_t st) {
 
 struct LnBwdShape {
     int G, R, blocks;      // R = 0: the long form
+    bool few;              // rows and columns in one launch, no partial sums
 };
 // Teams as in the forward, with fewer pieces: a column costs three registers more.  More workgroups hide more latency and cost 8 N
 // bytes of partial sums each, written and read.  Measured at 200 MB of rows (us): 32768 x 1024 bf16 with 256 workgroups of 8 teams
 // 43.0 (384: 52.4, 512: 47.2), 24000 x 2048 with 1024 of one team 64.2 (768: 68.0, 512: 83.6), 12000 x 4096 with 512 62.1 (768: 67.0,
 // 256: 84.0), 6103 x 8192 with 256 71.5 (512: 78.2).  1401 wide: 64 x 3 pieces 66.0 (256 x 1: 92.7); 5000: 256 x 3 67.2 (1024 x 1:
 // 84.9).
+// Few rows: a second launch costs more than a second reading.  us in one launch / two: 1024 rows x 100 bf16 9.8 / 12.9, x 1024 10.3 /
+// 12.4, x 1401 13.8 / 12.8, x 4096 13.4 / 15.1, x 16384 28.4 / 40.6; 1536 x 1024 15.6 / 12.5; fp32 1024 x 2048 11.7 / 12.6, x 6000
+// 22.9 / 19.6, 512 x 6000 13.6 / 13.9, x 16384 28.5 / 39.2; 512 x 3 bf16 (no whole piece) 13.7 / 13.4.
 LnBwdShape ln_bwd_shape(int M, int N, int E) {
     const int forms[][2] = {{16, 1}, {64, 1}, {64, 2}, {64, 3}, {256, 1}, {256, 2}, {256, 3}, {1024, 1}, {1024, 2}, {1024, 4}};
     for (auto& f : forms)
         if (N <= f[0] * f[1] * E && (f[1] * E <= 16 || f[1] == 3)) {
+            if (N >= E && M <= (E == 8 || N <= 2048 ? 1024 : 512)) return {f[0], f[1], 1, true};
             const int teams = f[0] < 256 ? 512 / f[0] : 1;
             const int most = f[0] == 1024 || f[0] == 64 ? 256 : f[0] == 256 && f[1] == 1 ? 1024 : 512;
             const int b = cdiv(M, teams);
-            return {f[0], f[1], b < most ? b : most};
+            return {f[0], f[1], b < most ? b : most, false};
         }
     const int most = N <= 1 << 23 ? 64 : 32;              // the scratch's size stays in 31 bits
-    return {0, 0, M < most ? M : most};
+    return {0, 0, M < most ? M : most, false};
 }
 
 template <class T, class WT> int ln_bwd(LnBwd g, WT* dw, WT* db, hipStream_t st) {
     g.dw = dw;
     g.db = db;
     const LnBwdShape s = ln_bwd_shape(g.M, g.N, Pack<T>::N);
+    if (s.few) {
+        const int columns = cdiv(g.N, 8 * Pack<T>::N), skip = dw || db ? 0 : columns;
+        const bool over = g.DX == g.X || g.DX == g.DY;    // the columns are read before a row is written over them
+        switch (s.G * 16 + s.R) {
+#define LN_GO(G, R)                                                                                                      \
+    case G * 16 + R: {                                                                                                   \
+        const int rows = cdiv(g.M, G < 256 ? 256 / G : 1);                                                               \
+        if (over && !skip)                                                                                               \
+            hipLaunchKernelGGL((ln_bwd_few_kernel<T, WT, G, R>), dim3(columns), dim3(G < 256 ? 256 : G), 0, st, g, 0);   \
+        hipLaunchKernelGGL((ln_bwd_few_kernel<T, WT, G, R>), dim3(rows + (over ? 0 : columns - skip)),                   \
+                           dim3(G < 256 ? 256 : G), 0, st, g, over ? columns : skip);                                    \
+        break;                                                                                                           \
+    }
+            LN_GO(16, 1) LN_GO(64, 1) LN_GO(64, 2) LN_GO(64, 3) LN_GO(256, 1) LN_GO(256, 2) LN_GO(256, 3) LN_GO(1024, 1)
+            LN_GO(1024, 2)
+            case 1024 * 16 + 4:
+                if constexpr (sizeof(T) == 4) {           // the shape's rule gives 16-bit rows at most 2 pieces
+                    if (over && !skip)
+                        hipLaunchKernelGGL((ln_bwd_few_kernel<T, WT, 1024, 4>), dim3(columns), dim3(1024), 0, st, g, 0);
+                    hipLaunchKernelGGL((ln_bwd_few_kernel<T, WT, 1024, 4>), dim3(g.M + (over ? 0 : columns - skip)), dim3(1024),
+                                       0, st, g, over ? columns : skip);
+                }
+                break;
+#undef LN_GO
+        }
+        WFD_CHECK_LAUNCH();
+        return WFD_OK;
+    }
     switch (s.G * 16 + s.R) {
 #define LN_GO(G, R)                                                                                                      \
     case G * 16 + R:                                                                                                     \
