@@ -737,6 +737,32 @@ def test_results_beyond_the_caches_have_the_bits_of_smaller_calls(t):
         assert torch.equal(heads.label_logprobs_backward(x[s], y[s], mine, torch.ones(100, device=DEV)), b[s])
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,v", [(1100, 20001), (600, 40001), (300, 63000), (300, 100001)])
+def test_distill_of_many_long_rows_has_the_bits_of_fewer(m, v, t):
+    """Workgroups that walk several rows each against calls on 100 of the rows, loss alone against loss with gradient."""
+    from wfd_gan_amd import heads
+    if t == F32 and v > 65536:
+        v = 65535                                             # the longest fp32 row that is not split
+    g = torch.Generator(device=DEV).manual_seed(v)
+    x = torch.randn(m, v, generator=g, device=DEV).to(t)
+    ti = torch.randint(-1, v, (m, 9), generator=g, device=DEV, dtype=torch.int32)
+    tv = torch.randn(m, 9, generator=g, device=DEV)
+    y = torch.randint(-1, v, (m,), generator=g, device=DEV, dtype=torch.int32)
+    for kw in (dict(temperature=2.0, weight=0.7, label_weight=0.3), dict(temperature=1.0)):
+        a = heads.distill_loss(x, ti, tv, y, **kw)
+        assert torch.equal(heads.distill_loss(x, ti, tv, y, grad=False, **kw).loss, a.loss)
+        for lo in (0, m // 2 - 7, m - 100):
+            s = slice(lo, lo + 100)
+            part = heads.distill_loss(x[s], ti[s], tv[s], y[s], **kw)
+            assert torch.equal(part.loss, a.loss[s]) and torch.equal(part.dlogits, a.dlogits[s])
+    rows = [0, 1, m // 2, m - 1]
+    one = torch.ones(len(rows), dtype=torch.float64)
+    loss, bl, d, bd = R.distill(x[rows].cpu(), ti[rows].cpu(), tv[rows].cpu(), None, 1.0, 1.0, 0.0, one)
+    R.check(a.loss[rows], loss, bl, F32, "loss")
+    R.check(a.dlogits[rows], d, bd, t, "dlogits")
+
+
 def test_captured_with_results_of_its_own():
     """Calls that make their results inside the capture: fresh memory of the graph's own pool, alive as long as the results."""
     from wfd_gan_amd import heads

@@ -222,122 +222,91 @@ __device__ __forceinline__ void grad_targets(const Distill& g, const GradRow& d,
 // ---- a row in the registers of a team of G threads ----------------------------------------------------------------------------
 // TWO: a label is mixed in at a temperature other than 1, so two sums of exponentials are kept.  Without, every exponential serves both
 // terms and cu joins cw.
-// Workgroups of one row walk rows gridDim.x apart: a piece's registers take the next row's load as soon as its gradient is on its way
-// out, so that memory has work while the arithmetic of a row runs (a long row fills the CU's registers: there is no second workgroup
-// to do that).
+// One row per team: the other workgroups of a CU, or of the chip where a row fills a CU's registers, keep memory busy while this one
+// computes.  What matters is that all of a thread's loads are on their way before the first is waited for; walking rows with the
+// next one's loads behind each stored piece was no better once that held (2048 x 128000 bf16: 205 us, walking 234; 4096 x 32000:
+// 105, 105; loss alone 46, 47).
 template <class T, int G, int R, bool TWO, bool GRAD>
 __global__ __launch_bounds__(G < 256 ? 256 : G, R == 16 ? 4 : 1) void distill_kernel(Distill g) {
     constexpr int E = Pack<T>::N, TEAMS = G < 256 ? 256 / G : 1, L = G < 64 ? G : 64, B = R < 4 ? R : 4;
     extern __shared__ float lds[];
-    __shared__ float slot[2][2 * (G > 64 ? G / 64 : 1)], told[8];
+    __shared__ float slot[2][2 * (G > 64 ? G / 64 : 1)], told[3];
     const int t = TEAMS > 1 ? threadIdx.x % G : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / G : 0, V = g.V;
-    int row = blockIdx.x * TEAMS + team;
+    const int row = blockIdx.x * TEAMS + team;
     if (row >= g.M) return;                                   // whole teams, each inside a wave
     const float inv_t = 1.f / g.temp, c = inv_t * LOG2E;
-    // piece r * G + t of the whole ones; the elements around them go to the first threads.  How many there are holds for all rows of
-    // a workgroup: a workgroup with more than one is one of an even number, so its rows lie an even number of elements apart
+    // piece r * G + t of the whole ones; the elements around them go to the first threads
     const unsigned lane_off = (unsigned)t * E;
     const T* x = (const T*)g.X + (long)row * g.ld;
     const int head = G > 64 ? off_border(x) : 0, P = (V - head) / E, rest = V - P * E;
     Raw16 d[R];
-    float tail = -INFINITY;
-    auto fetch = [&](int r, const T* from) {
-        if (r * G + t < P) d[r] = load16(from + head + r * G * E + lane_off);
-    };
-    auto fetch_tail = [&](const T* from) {
-        if (t < rest) tail = to_f32(from[t < head ? 0 : P * E + t]);
-    };
-    const unsigned none = raw_fill<T>(-INFINITY);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        d[r] = Raw16{{none, none, none, none}};
-        fetch(r, x);
+    for (int r = 0; r < R; ++r) team_load<T, G == 16 && R == 1>(d[r], x + head, r * G + t, P);
+    const float tail = t < rest ? to_f32(x[t < head ? 0 : P * E + t]) : -INFINITY;
+    // not always the first wave: that one sits on the same SIMD in every workgroup
+    const int lane = G > 64 ? t & 63 : t;
+    const bool boss = G <= 64 || (t >> 6) == (row & (G / 64 - 1));
+    const Entries n = entries_in(lds + team * 3 * g.K, g.K);
+    const int y = g.u != 0.f ? g.labels[row] : -1;
+    const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
+    Taught tt{LOWEST, 0.f, false};
+    if (boss) {
+        tt = teacher<L>(g, row, lane, n, c);
+        wave_sync();
+        entries_gather<T, L>(x, g.K, lane, n);
+        if constexpr (G > 64)
+            if (lane == 0) { told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f; }
     }
-    fetch_tail(x);
-    for (int par = 0;; par ^= 1) {
-        // one set of entries per row in turn: the wave of the row before may still be at its targets
-        const Entries n = entries_in(lds + (G > 64 ? par : team) * 3 * g.K, g.K);
-        const long next = (long)row + gridDim.x;
-        const bool more = G > 64 && next < g.M;
-        const T* xn = x + (long)gridDim.x * g.ld;
-        // the wave that works the entries changes from row to row: a workgroup's first wave always sits on the same SIMD
-        const int lane = G > 64 ? t & 63 : t;
-        const bool boss = G <= 64 || (t >> 6) == (row & (G / 64 - 1));
-        const int y = g.u != 0.f ? g.labels[row] : -1;
-        const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
-        Taught tt{LOWEST, 0.f, false};
-        if (boss) {
-            tt = teacher<L>(g, row, lane, n, c);
-            wave_sync();
-            entries_gather<T, L>(x, g.K, lane, n);
-            if constexpr (G > 64)
-                if (lane == 0) { told[0] = tt.max; told[1] = tt.sum; told[2] = tt.wrong ? 1.f : 0.f; }
-        }
-        // per thread about its own running maximum, four pieces at a time, while later pieces are still on their way
-        RowSums s{LOWEST, 0.f, 0.f};
+    // per thread about its own running maximum, four pieces at a time, while later pieces are still on their way
+    const unsigned none = raw_fill<T>(-INFINITY);
+    RowSums s{LOWEST, 0.f, 0.f};
 #pragma unroll
-        for (int r0 = 0; r0 < R; r0 += B) {
-            float f[B * E], top = -INFINITY;
+    for (int r0 = 0; r0 < R; r0 += B) {
+        float f[B * E], top = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < B; ++r) {
-                keep_packed(d[r0 + r]);
+        for (int r = 0; r < B; ++r) {
+            // every form holds at most twice the classes of the one before, so the first half of its places is full
+            if (R == 1 || r0 + r >= R / 2) only(d[r0 + r], (r0 + r) * G + t < P, none);
+            keep_packed(d[r0 + r]);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    f[r * E + e] = elem<T>(d[r0 + r], e);
-                    top = fmaxf(top, f[r * E + e]);
-                }
+            for (int e = 0; e < E; ++e) {
+                f[r * E + e] = elem<T>(d[r0 + r], e);
+                top = fmaxf(top, f[r * E + e]);
             }
-            sums_add<TWO>(s, f, top, c);
-            // without a gradient a piece's registers are free at once.  Where a row fills the CU that pays (2048 x 128000 bf16: 110 us
-            // before, 98 so); beside other workgroups it does not (4096 x 32000: 49, 53), and the loads follow behind the sums
-            if constexpr (!GRAD && G == 1024)
-                if (more)
+        }
+        sums_add<TWO>(s, f, top, c);
+    }
+    if (rest) {
+        const float f[1] = {tail};
+        sums_add<TWO>(s, f, tail, c);
+    }
+    sums_to<TWO>(s, team_max<G>(s.m, slot[0]), c);
+    if constexpr (G > 64) tt = Taught{told[0], told[1], told[2] != 0.f};
+    if constexpr (TWO) {
+        const float2 q = team_sum2<G>(s.s, s.s1, slot[1]);
+        s.s = q.x;
+        s.s1 = q.y;
+    } else {
+        s.s1 = s.s = team_sum<G>(s.s, slot[1]);
+    }
+    const bool wrong = tt.wrong || y >= V;
+    if (boss) {
+        wave_sync();
+        const float loss = row_loss<L>(g, row, lane, n, tt, s, inv_t, y, xy, wrong);
+        if (lane == 0) g.loss[row] = loss;
+    }
+    if constexpr (GRAD) {
+        const GradRow k = grad_row<TWO>(g, row, tt, s, y, wrong, c);
+        T* o = (T*)g.DX + (long)row * g.lddx;
 #pragma unroll
-                    for (int r = 0; r < B; ++r) fetch(r0 + r, xn);
+        for (int r = 0; r < R; ++r) {
+            keep_packed(d[r]);
+            if (r * G + t < P) grad_piece<T, TWO>(k, d[r], o + head + r * G * E + lane_off, c, g.past);
         }
-        if (rest) {
-            const float f[1] = {tail};
-            sums_add<TWO>(s, f, tail, c);
-        }
-        sums_to<TWO>(s, team_max<G>(s.m, slot[0]), c);
-        if constexpr (G > 64) tt = Taught{told[0], told[1], told[2] != 0.f};
-        if constexpr (TWO) {
-            const float2 q = team_sum2<G>(s.s, s.s1, slot[1]);
-            s.s = q.x;
-            s.s1 = q.y;
-        } else {
-            s.s1 = s.s = team_sum<G>(s.s, slot[1]);
-        }
-        const bool wrong = tt.wrong || y >= V;
-        if (boss) {
-            wave_sync();
-            const float loss = row_loss<L>(g, row, lane, n, tt, s, inv_t, y, xy, wrong);
-            if (lane == 0) g.loss[row] = loss;
-        }
-        if constexpr (GRAD) {
-            const GradRow k = grad_row<TWO>(g, row, tt, s, y, wrong, c);
-            T* o = (T*)g.DX + (long)row * g.lddx;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                keep_packed(d[r]);
-                if (r * G + t < P) grad_piece<T, TWO>(k, d[r], o + head + r * G * E + lane_off, c, g.past);
-                if (more) fetch(r, xn);
-            }
-            if (t < rest) o[t < head ? 0 : P * E + t] = from_f32<T>(grad_dense<TWO>(k, tail, c));
-            if constexpr (G > 64) __syncthreads();
-            else wave_sync();
-            if (boss) grad_targets<T, TWO, L>(g, k, n, s.s == 0.f, lane, o, 0, V, y, xy, c);
-        } else if constexpr (G > 64) {
-            if (G < 1024 && more)
-#pragma unroll
-                for (int r = 0; r < R; ++r) fetch(r, xn);
-            __syncthreads();                                  // the next row's entries and sums go where this row's were
-        }
-        if constexpr (G <= 64) return;
-        if (!more) return;
-        fetch_tail(xn);
-        row = (int)next;
-        x = xn;
+        if (t < rest) o[t < head ? 0 : P * E + t] = from_f32<T>(grad_dense<TWO>(k, tail, c));
+        if constexpr (G > 64) __syncthreads();
+        else wave_sync();
+        if (boss) grad_targets<T, TWO, L>(g, k, n, s.s == 0.f, lane, o, 0, V, y, xy, c);
     }
 }
 
@@ -478,14 +447,14 @@ template <class T, bool TWO, bool GRAD> int distill(Distill g, hipStream_t st) {
 #define WFD_GO(G, R)                                                                                                     \
     if (g.V <= G * R * E) {                                                                                              \
         constexpr int TEAMS = G < 256 ? 256 / G : 1;                                                                     \
-        const int blocks = cdiv(g.M, TEAMS), most = G > 64 ? 256 * (16 / R) * (1024 / G) : blocks;                       \
-        if (!launchable(blocks < most ? blocks : most, G < 256 ? 256 : G)) return WFD_ERR_ARG;                           \
-        hipLaunchKernelGGL((distill_kernel<T, G, R, TWO, GRAD>), dim3(blocks < most ? blocks : most),                    \
-                           dim3(G < 256 ? 256 : G), (size_t)(TEAMS > 1 ? TEAMS : 2) * 3 * g.K * 4, st, g);               \
+        const int blocks = cdiv(g.M, TEAMS);                                                                             \
+        if (!launchable(blocks, G < 256 ? 256 : G)) return WFD_ERR_ARG;                                                  \
+        hipLaunchKernelGGL((distill_kernel<T, G, R, TWO, GRAD>), dim3(blocks), dim3(G < 256 ? 256 : G),                  \
+                           (size_t)TEAMS * 3 * g.K * 4, st, g);                                                          \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
     }
-        WFD_GO(16, 1) WFD_GO(16, 2) WFD_GO(64, 1) WFD_GO(64, 2) WFD_GO(64, 4) WFD_GO(256, 2) WFD_GO(256, 4) WFD_GO(256, 8) WFD_GO(256, 16)
+        WFD_GO(16, 1) WFD_GO(16, 2) WFD_GO(64, 1) WFD_GO(64, 2) WFD_GO(64, 4) WFD_GO(64, 8) WFD_GO(256, 4) WFD_GO(256, 8) WFD_GO(256, 16)
         WFD_GO(512, 16) WFD_GO(1024, 16)
 #undef WFD_GO
     }

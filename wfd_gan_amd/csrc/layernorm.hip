@@ -33,20 +33,23 @@ struct LnBwd {
     int lddy, ldx, lddx, M, N;
 };
 
-// E weights from i0 (all inside the row)
+// E weights from i0 (all inside the row), `none` without weights: those are loaded all the same, from somewhere else, as in team_load
+__device__ const unsigned NO_WEIGHTS[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 template <class WT, int E> __device__ __forceinline__ void load_weights(float* f, const WT* w, int i0, float none) {
     constexpr int P = Pack<WT>::N < E ? Pack<WT>::N : E;
-    if (!w) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = none;
-        return;
-    }
+    const WT* from = w ? w + i0 : (const WT*)NO_WEIGHTS;
 #pragma unroll
     for (int h = 0; h < E / P; ++h) {
-        const Raw16 r = load16(w + i0 + h * P);
+        const Raw16 r = load16(from + h * P);
 #pragma unroll
-        for (int e = 0; e < P; ++e) f[h * P + e] = elem<WT>(r, e);
+        for (int e = 0; e < P; ++e) f[h * P + e] = w ? elem<WT>(r, e) : none;
     }
+}
+
+// those of piece `piece` of P (see team_load)
+template <class WT, int E, bool ONE> __device__ __forceinline__ void team_weights(float* f, const WT* w, int piece, int P, float none) {
+    if (ONE && piece >= P) return;
+    load_weights<WT, E>(f, w, (ONE ? piece : min(piece, P - 1)) * E, none);
 }
 
 // ---- forward: a team of G threads per row, R pieces per thread in registers -----------------------------------------
@@ -64,26 +67,33 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void ln_fwd_kernel(LnFwd g) {
     if (row >= g.M) return;                               // whole teams; only teams of at most one wave share a workgroup
     const WT* W = (const WT*)g.W;
     const WT* B = (const WT*)g.B;
+    // KEEP: a team of a whole CU has many empty places; those hold 0 from the start and load nothing (5000 x 10000 bf16: 51 us, reading
+    // the last piece there 55; backward 75 and 82)
+    constexpr bool ONE = G == 16 && R == 1, KEEP = G == 1024 && R > 1;
     Raw16 d[R];
     float last = 0.f;
     auto fetch = [&](long at) {
         const T* x = (const T*)g.X + at * g.ldx;
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (r * G + t < P) d[r] = load16(x + (r * G + t) * E);
+            if constexpr (KEEP) {
+                if (r * G + t < P) d[r] = load16(x + (r * G + t) * E);
+            } else {
+                team_load<T, ONE>(d[r], x, r * G + t, P);
+            }
         if (t < rest) last = to_f32(x[P * E + t]);
     };
+    if constexpr (KEEP)
 #pragma unroll
-    for (int r = 0; r < R; ++r) d[r] = Raw16{{0u, 0u, 0u, 0u}};
+        for (int r = 0; r < R; ++r) d[r] = Raw16{{0u, 0u, 0u, 0u}};
     fetch(row);
     float w[HOLD ? R : 1][E], b[HOLD ? R : 1][E], wl = 1.f, bl = 0.f;
     if constexpr (HOLD)
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (r * G + t < P) {
-                load_weights<WT, E>(w[r], W, (r * G + t) * E, 1.f);
-                load_weights<WT, E>(b[r], B, (r * G + t) * E, 0.f);
-            }
+        for (int r = 0; r < R; ++r) {
+            team_weights<WT, E, ONE>(w[r], W, r * G + t, P, 1.f);
+            team_weights<WT, E, ONE>(b[r], B, r * G + t, P, 0.f);
+        }
     if (t < rest) {
         if (W) wl = to_f32(W[P * E + t]);
         if (B) bl = to_f32(B[P * E + t]);
@@ -91,9 +101,11 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void ln_fwd_kernel(LnFwd g) {
     for (int par = 0;; par ^= 1) {
         float s = last;                                   // places without an element hold 0
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+            if constexpr (!KEEP) only(d[r], r * G + t < P, 0u);
 #pragma unroll
             for (int e = 0; e < E; ++e) s += elem<T>(d[r], e);
+        }
         const float mean = team_sum<G>(s, slot[par][0]) / (float)N;
         float q = 0.f;
 #pragma unroll
@@ -196,12 +208,13 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
     __shared__ float slot[2][2 * W];
     const int t = TEAMS > 1 ? threadIdx.x % G : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / G : 0;
     const int N = g.N, P = N / E, rest = N - P * E;
+    constexpr bool ONE = G == 16 && R == 1, KEEP = G == 1024 && R > 1;
     float w[R][E], sw[R][E], sb[R][E], wl = 0.f, swl = 0.f, sbl = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
         for (int e = 0; e < E; ++e) { sw[r][e] = 0.f; sb[r][e] = 0.f; w[r][e] = 0.f; }
-        if (r * G + t < P) load_weights<WT, E>(w[r], (const WT*)g.W, (r * G + t) * E, 1.f);
+        team_weights<WT, E, ONE || KEEP>(w[r], (const WT*)g.W, r * G + t, P, 1.f);
     }
     if (t < rest) wl = g.W ? to_f32(((const WT*)g.W)[P * E + t]) : 1.f;
     const float inv = 1.f / (float)N;
@@ -215,17 +228,23 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
         const T* dy = (const T*)g.DY + row * g.lddy;
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (r * G + t < P) {
-                k.x[r] = load16(x + (r * G + t) * E);
-                k.dy[r] = load16(dy + (r * G + t) * E);
+            if constexpr (KEEP) {
+                if (r * G + t < P) {
+                    k.x[r] = load16(x + (r * G + t) * E);
+                    k.dy[r] = load16(dy + (r * G + t) * E);
+                }
+            } else {
+                team_load<T, ONE>(k.x[r], x, r * G + t, P);
+                team_load<T, ONE>(k.dy[r], dy, r * G + t, P);
             }
         if (t < rest) { k.xl = to_f32(x[P * E + t]); k.dyl = to_f32(dy[P * E + t]); }
         k.mean = g.mean[row];
         k.rstd = g.rstd[row];
     };
     Row k;
+    if constexpr (KEEP)
 #pragma unroll
-    for (int r = 0; r < R; ++r) k.x[r] = k.dy[r] = Raw16{{0u, 0u, 0u, 0u}};
+        for (int r = 0; r < R; ++r) k.x[r] = k.dy[r] = Raw16{{0u, 0u, 0u, 0u}};
     k.xl = k.dyl = 0.f;                                   // places without an element: dy = 0, so every sum stays
     long row = (long)blockIdx.x * TEAMS + team;
     if (row < g.M) fetch(k, row);
@@ -235,7 +254,8 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
             if (row + step < g.M) fetch(n, row + step);
         float a = 0.f, b = 0.f;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+            if constexpr (!KEEP) only(k.dy[r], r * G + t < P, 0u);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float d = elem<T>(k.dy[r], e), xh = (elem<T>(k.x[r], e) - k.mean) * k.rstd, v = d * w[r][e];
@@ -244,6 +264,7 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
                 sw[r][e] = fmaf(d, xh, sw[r][e]);
                 sb[r][e] += d;
             }
+        }
         const float xhl = (k.xl - k.mean) * k.rstd;
         if (rest) {
             a = fmaf(k.dyl, wl, a);
@@ -392,18 +413,20 @@ template <class T, class WT, int G, int R> __device__ __forceinline__ void bwd_r
     T* o = (T*)g.DX + row * g.lddx;
     const float mean = g.mean[row], rstd = g.rstd[row], inv = 1.f / (float)N;
     float xh[R][E], v[R][E], xhl = 0.f, vl = 0.f, a = 0.f, b = 0.f;
+    Raw16 xr[R], dr[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {                         // P >= 1: rows shorter than a piece do not come here
+        team_load<T, false>(xr[r], x, r * G + t, P);
+        team_load<T, false>(dr[r], dy, r * G + t, P);
+        team_weights<WT, E, false>(v[r], (const WT*)g.W, r * G + t, P, 1.f);
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+        only(dr[r], r * G + t < P, 0u);
 #pragma unroll
-        for (int e = 0; e < E; ++e) xh[r][e] = v[r][e] = 0.f;
-        if (r * G + t < P) {
-            const Raw16 dx_ = load16(x + (r * G + t) * E), dd = load16(dy + (r * G + t) * E);
-            load_weights<WT, E>(v[r], (const WT*)g.W, (r * G + t) * E, 1.f);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                xh[r][e] = (elem<T>(dx_, e) - mean) * rstd;
-                v[r][e] *= elem<T>(dd, e);
-            }
+        for (int e = 0; e < E; ++e) {
+            xh[r][e] = (elem<T>(xr[r], e) - mean) * rstd;
+            v[r][e] *= elem<T>(dr[r], e);
         }
     }
     if (t < rest) {

@@ -101,6 +101,23 @@ template <class T> __device__ __forceinline__ unsigned raw_fill(float fill) {
     return pack<T>(f).v[0];
 }
 
+// A team's pieces: thread t of G has pieces r * G + t of a row's P whole ones.  A load under a condition with another value beside it
+// makes the compiler wait for each one before the next (it merges registers behind the branch), so a thread without a piece reads
+// the row's last one instead, and `only` puts the value of an empty place where the piece is used.  ONE: the team of the shortest
+// rows, which may have no whole piece at all and only has the one load to wait for.
+template <class T, bool ONE> __device__ __forceinline__ void team_load(Raw16& d, const T* row, int piece, int P) {
+    if constexpr (ONE) {
+        d = Raw16{{0u, 0u, 0u, 0u}};
+        if (piece < P) d = load16(row + piece * Pack<T>::N);
+    } else {
+        d = load16(row + min(piece, P - 1) * Pack<T>::N);
+    }
+}
+__device__ __forceinline__ void only(Raw16& d, bool here, unsigned none) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d.v[i] = here ? d.v[i] : none;
+}
+
 // elements [i0, i0 + Pack<T>::N) of a row of n; those past the end read as `fill`
 template <class T> __device__ __forceinline__ Raw16 load_piece(const T* row, int i0, int n, float fill) {
     constexpr int E = Pack<T>::N;

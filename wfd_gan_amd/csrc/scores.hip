@@ -394,18 +394,26 @@ __device__ __forceinline__ Stat walk(const T* x, int n, float c, float* gmax, fl
         take(d);
     }
     if ((long)it * STEP < n) {
-        // the rest, piece by piece as far as any lane of the wave has one
+        // the rest, as far as any lane of the wave has a piece.  All loads first, and none under a condition (see team_load): a piece that
+        // would reach past the end starts earlier, its elements before i0 are another piece's
         float group = -INFINITY;
-        const int first = (t & ~63) * E;
+        const int first = (t & ~63) * E, i0 = it * STEP + t * E, last = max(n - E, 0);
+        Raw16 d[U];
+        if (n >= E) {
+#pragma unroll
+            for (int j = 0; j < U; ++j) d[j] = load16(x + min(i0 + j * NT * E, last));
+        } else {
+            d[0] = load_piece(x, 0, n, -INFINITY);
+        }
+#pragma unroll
         for (int j = 0; j < U; ++j) {
-            const long i0 = (long)it * STEP + (j * NT + t) * E;
-            if ((long)it * STEP + j * NT * E + first >= n) break;
+            const int i = i0 + j * NT * E, s = min(i, last);
+            if (it * STEP + j * NT * E + first >= n) continue;
             float f[E], top = -INFINITY;
-            if (i0 < n) {
-                const Raw16 d = load_piece(x, (int)i0, n, -INFINITY);
+            if (i < n) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    f[e] = elem<T>(d, e);
+                    f[e] = s + e >= i ? elem<T>(d[j], e) : -INFINITY;
                     top = fmaxf(top, f[e]);
                 }
                 stat_add(a, f, top, c);
