@@ -269,6 +269,23 @@ def test_scores_masks_ties_and_order(v, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("v", [1, 2, 100, 1401, 5000, 40003])
+def test_scores_of_a_class_alone_in_its_row(v, t):
+    """Everything else masked: probability 1 and entropy 0, to the bit, at any value and temperature."""
+    from wfd_gan_amd import heads
+    m = 40
+    g = gen(v)
+    x = torch.full((m, v), -INF, dtype=t)
+    at = torch.randint(0, v, (m,), generator=g)
+    x[torch.arange(m), at] = (randn(g, m) * 20).to(t)
+    for rows in (1, m):
+        for temp in (0.3, 1.0, 7.0):
+            r = heads.label_logprobs(x[:rows].to(DEV), at[:rows].to(torch.int32).to(DEV), 1, temperature=temp)
+            assert float(r.logprob.abs().max()) == 0 and float(r.entropy.abs().max()) == 0
+            assert float(r.top_logprob.abs().max()) == 0 and torch.equal(r.top_index[:, 0].cpu().long(), at[:rows])
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("v", [6, 1401, 40003])
 def test_scores_non_finite_and_wrong_labels(v, t):
     from wfd_gan_amd import heads

@@ -26,7 +26,7 @@ struct Distill {
     void* DX;
     float* work;            // split form: [M][3 * splits + MAX_ENTRIES + 1]: partial sums, the entries' and the label's logits
     int ld, lddx, ldt, M, V, K;
-    float temp, w, u, scale;
+    float temp, c, w, u, scale;     // c = log2(e) / temp
     int splits, chunk;      // split form: parts of a row, their length
     bool past;              // the gradient is written past the caches
 };
@@ -112,24 +112,25 @@ template <bool TWO, int N> __device__ __forceinline__ void sums_add(RowSums& a, 
 // the row's loss (every lane), from the entries and the sums
 template <int L>
 __device__ __forceinline__ float row_loss(const Distill& g, long row, int lane, const Entries& n, const Taught& t, const RowSums& s,
-                                          float inv_t, int y, float xy, bool wrong) {
+                                          int y, float xy, bool wrong) {
+    // ln q_j - ln p_j = ((t_j - max t) - (x_j - max x)) / T + ln(s / sum e): terms of tens whose sum may be small, so they are added
+    // in 64 bits
     const bool empty = s.s == 0.f;
-    float kl = 0.f;
-    if (t.sum != 0.f) {
-        const float inv = 1.f / t.sum, log_t = LN2 * __log2f(t.sum), log_s = LN2 * __log2f(s.s);
-        for (int j = lane; j < g.K; j += L) {
-            const float q = n.e[j] * inv;
-            if (!(n.e[j] < 1.17549435e-38f)) {  // below the normal range a share is as good as none, and has no logarithm
-                const float lq = LN2 * __log2f(n.e[j]) - log_t;
-                const float lp = empty ? -INFINITY : (n.x[j] - s.m) * inv_t - log_s;
-                kl = fmaf(q, lq - lp, kl);
-            }
+    double sum = 0., apart = 0.;
+    for (int j = lane; j < g.K; j += L)
+        if (n.e[j] != 0.f) {
+            sum += n.e[j];
+            apart += n.e[j] * ((double)(g.t_val[row * g.ldt + j] - t.max) - (double)(n.x[j] - s.m));
         }
+    sum = lanes_sum<L>(sum);
+    apart = lanes_sum<L>(apart);
+    double loss = 0.;
+    if (sum != 0.) {
+        const float inv = 1.f / (float)sum;
+        loss = (double)g.w * g.temp * (empty ? INFINITY : (double)g.temp * logf(s.s * inv) + apart * inv);
     }
-    kl = lanes_sum<L>(kl);
-    float loss = g.K ? g.w * g.temp * g.temp * kl : 0.f;
-    if (y >= 0) loss -= g.u * (empty ? -INFINITY : xy - s.m - LN2 * __log2f(s.s1));
-    return wrong ? NAN : loss;
+    if (y >= 0) loss -= g.u * (empty ? -INFINITY : (double)(xy - s.m) - logf(s.s1));
+    return wrong ? NAN : (float)loss;
 }
 
 // what a gradient element is made of: d = cw exp((x - m) / T) + cu exp(x - m), less the targets at the entries and the label
@@ -139,7 +140,8 @@ struct GradRow {
     bool wide;                     // m c beyond WIDE
 };
 template <bool TWO>
-__device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Taught& t, const RowSums& s, int y, bool wrong, float c) {
+__device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Taught& t, const RowSums& s, int y, bool wrong,
+                                            float c) {
     GradRow d;
     d.m = s.m;
     d.r = g.scale * (g.row_scale ? g.row_scale[row] : 1.f);
@@ -234,7 +236,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, R == 16 ? 4 : 1) void distill_ke
     const int t = TEAMS > 1 ? threadIdx.x % G : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / G : 0, V = g.V;
     const int row = blockIdx.x * TEAMS + team;
     if (row >= g.M) return;                                   // whole teams, each inside a wave
-    const float inv_t = 1.f / g.temp, c = inv_t * LOG2E;
+    const float c = g.c;
     // piece r * G + t of the whole ones; the elements around them go to the first threads
     const unsigned lane_off = (unsigned)t * E;
     const T* x = (const T*)g.X + (long)row * g.ld;
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, R == 16 ? 4 : 1) void distill_ke
     const bool wrong = tt.wrong || y >= V;
     if (boss) {
         wave_sync();
-        const float loss = row_loss<L>(g, row, lane, n, tt, s, inv_t, y, xy, wrong);
+        const float loss = row_loss<L>(g, row, lane, n, tt, s, y, xy, wrong);
         if (lane == 0) g.loss[row] = loss;
     }
     if constexpr (GRAD) {
@@ -320,7 +322,7 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_part
     const int lo = sp * g.chunk, n = min(g.chunk, g.V - lo);
     const T* x = (const T*)g.X + row * g.ld;
     float* w = g.work + row * (3L * g.splits + MAX_ENTRIES + 1);
-    const float c = LOG2E / g.temp;
+    const float c = g.c;
     RowSums a{LOWEST, 0.f, 0.f};
     const int P = n / E, rest = n - P * E;
     const unsigned none = raw_fill<T>(-INFINITY);
@@ -370,7 +372,7 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_fini
     const int lo = (int)(blockIdx.x - row * parts) * STEP, t = threadIdx.x, V = g.V;
     const T* x = (const T*)g.X + row * g.ld;
     const float* w = g.work + row * (3L * g.splits + MAX_ENTRIES + 1);
-    const float inv_t = 1.f / g.temp, c = inv_t * LOG2E;
+    const float c = g.c;
     const Entries n = entries_in(lds, g.K);
     const int y = g.u != 0.f ? g.labels[row] : -1;
     Raw16 d[U];
@@ -401,7 +403,7 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_fini
         }
         if (lo == 0) {
             wave_sync();
-            const float loss = row_loss<64>(g, row, t, n, tt, s, inv_t, y, xy, tt.wrong || y >= V);
+            const float loss = row_loss<64>(g, row, t, n, tt, s, y, xy, tt.wrong || y >= V);
             if (t == 0) g.loss[row] = loss;
         }
     }
@@ -498,7 +500,7 @@ int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int*
     // without weight the entries are not read, and the label's term has no temperature
     if (weight == 0.f) K = 0;
     if (K == 0) temperature = 1.f;
-    Distill g{logits, t_index, t_value, labels, row_scale, loss, dlogits, work, ldl, lddl, ldt, M, V, K, temperature, weight,
+    Distill g{logits, t_index, t_value, labels, row_scale, loss, dlogits, work, ldl, lddl, ldt, M, V, K, temperature, log2e_over(temperature), weight,
               label_weight, grad_scale, 0, 0, past_caches(M, V, dtype == WFD_F32 ? 4 : 2)};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WFD_F32) return distill<float>(g, st);

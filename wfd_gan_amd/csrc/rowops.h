@@ -10,6 +10,7 @@ typedef _Float16 f16_t;
 #define WFD_BF16 1
 #define WFD_F16 2
 
+static inline float log2e_over(float t) { return (float)(1.4426950408889634 / (double)t); }
 static inline bool wfd_dtype_ok(int t) { return t >= WFD_F32 && t <= WFD_F16; }
 
 static inline int elems_of(int dtype) { return dtype == WFD_F32 ? 4 : 8; }     // of one 16-byte piece
@@ -152,6 +153,21 @@ __device__ __forceinline__ float lanes_sum16(float v) {
     v += dpp<0x140>(v);     // row_mirror
     return v;
 }
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+    const int2 w = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, int2{__builtin_amdgcn_update_dpp(0, w.x, CTRL, 0xf, 0xf, true),
+                                           __builtin_amdgcn_update_dpp(0, w.y, CTRL, 0xf, 0xf, true)});
+}
+template <int G> __device__ __forceinline__ double lanes_sum(double v) {
+#pragma clang fp contract(off)
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    v += dpp<0x140>(v);
+    if constexpr (G >= 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (G >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
 __device__ __forceinline__ float lanes_max16(float v) {
     v = fmaxf(v, dpp<0xB1>(v));
     v = fmaxf(v, dpp<0x4E>(v));
@@ -217,10 +233,11 @@ template <int G> __device__ __forceinline__ float team_max(float a, float* slot)
 }
 
 // ---- sums of exponentials about a maximum --------------------------------------------------------------------------------
-// exp((x - m) / T) = 2^(x c - m c), c = log2(e) / T.  Per element that is one fused multiply-add with the rounded R = m c and one
-// exp2; what R's rounding leaves (m c - R, exact by fma) is taken out of a whole group's sum at once, so the sums are about the true
-// maximum.  Where m c is so large that the remainder would be no small exponent itself (rows at the type's lowest value, whose product
-// may even leave fp32's range) the difference comes first.
+// exp((x - m) / T) = 2^((x - m) c), c = log2(e) / T.  The scores take the difference first: the maximum itself then gives 1 to the bit,
+// so a class alone in its row has log probability 0.  Distillation, whose gradient has two exponentials per element, takes
+// 2^(x c - m c): one fused multiply-add with the rounded R = m c (3000 x 70000 fp16 197 us, difference first 210), and what R's rounding
+// leaves (m c - R, exact by fma) is taken out of a whole group's sum at once.  Where m c is so large that the remainder would be
+// no small exponent itself (rows at the type's lowest value, whose product may even leave fp32's range) the difference comes first.
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float LOWEST = -3.402823466e38f;       // floor of a maximum: x - m stays defined for rows of nothing but -inf
 constexpr float FAINT = -1e4f;                   // an exponent whose exponential is 0: stands in where 0 * -inf would be NaN

@@ -23,7 +23,7 @@ struct Scores {
     int* top_idx;
     float* work;          // [M][splits][3 + 2 k]: a part's statistics, its alternatives' values and indices
     int ld, M, V, k;
-    float inv_t;
+    float inv_t, c;       // 1 / T and log2(e) / T
     int splits, chunk;    // parts of a row and their length (a multiple of a step)
 };
 struct ScoresBwd {
@@ -70,27 +70,15 @@ __device__ __forceinline__ void stat_to(Stat& a, float m, float c) {          //
 }
 template <int N> __device__ __forceinline__ void stat_add(Stat& a, const float (&f)[N], float top, float c) {
     if (top > a.m) stat_to(a, top, c);
-    const float R = a.m * c;
-    float s = 0.f, u = 0.f, rest = 0.f;
-    if (fabsf(R) < WIDE) {
-        rest = fmaf(a.m, c, -R);
+    float s = 0.f, u = 0.f;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float d = fmaf(f[e], c, -R), w = exp2_of(d);
-            s += w;
-            u = fmaf(w, fmaxf(d, FAINT), u);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float d = (f[e] - a.m) * c, w = exp2_of(d);
-            s += w;
-            u = fmaf(w, fmaxf(d, FAINT), u);
-        }
+    for (int e = 0; e < N; ++e) {
+        const float d = (f[e] - a.m) * c, w = exp2_of(d);     // the difference first: a lone class has s = 1 to the bit
+        s += w;
+        u = fmaf(w, fmaxf(d, FAINT), u);
     }
-    const float w = exp2_of(-rest);
-    a.u = fmaf(w, fmaf(-rest, s, u), a.u);
-    a.s = fmaf(w, s, a.s);
+    a.u += u;
+    a.s += s;
 }
 // over a team of G threads; slot: 3 * G / 64 floats of LDS.  Every thread gets the sum, added in a fixed order.
 template <int G> __device__ __forceinline__ Stat stat_team(Stat a, float c, float* slot) {
@@ -127,10 +115,9 @@ struct RowEnd {
 __device__ __forceinline__ RowEnd row_end(const Stat& a) {
     RowEnd r;
     r.empty = a.s == 0.f;
-    const float l2 = __log2f(a.s);
     r.m = r.empty ? -INFINITY : a.m;
-    r.log_s = r.empty ? 0.f : LN2 * l2;
-    r.entropy = r.empty ? 0.f : LN2 * (l2 - a.u / a.s);
+    r.log_s = r.empty ? 0.f : logf(a.s);
+    r.entropy = r.empty ? 0.f : fmaf(-LN2, a.u / a.s, r.log_s);
     return r;
 }
 __device__ __forceinline__ float row_lp(const RowEnd& r, float x, float inv_t) {
@@ -440,7 +427,7 @@ template <class T, int NT, bool PICK> __global__ __launch_bounds__(NT) void scor
     const T* x = (const T*)g.X + row * g.ld + lo;
     const int y = g.labels ? g.labels[row] : -1;
     const float xy = g.splits == 1 && y >= 0 && y < g.V ? to_f32(x[y]) : 0.f;
-    const float c = g.inv_t * LOG2E;
+    const float c = g.c;
     float tmax, next;
     const int head = off_border(x);
     Stat a = walk<T, NT, PICK>(x + head, n - head, c, gmax, tmax, next);
@@ -495,7 +482,7 @@ template <class T> __global__ __launch_bounds__(256) void scores_join_kernel(Sco
         const int at = ((const int*)p)[k + e];
         keys[i] = at < 0 ? 0ull : order_key(v, at);
     }
-    const float c = g.inv_t * LOG2E;
+    const float c = g.c;
     Stat a{LOWEST, 0.f, 0.f};
     if (lane < S) a = Stat{w[lane * each], w[lane * each + 1], w[lane * each + 2]};      // S <= 64
     const RowEnd r = row_end(stat_team<64>(a, c, nullptr));
@@ -566,7 +553,7 @@ template <class T, int G, int R> __global__ __launch_bounds__(256) void scores_f
     }
     const int y = g.labels ? g.labels[row] : -1;
     const float xy = y >= 0 && y < V ? to_f32(x[y]) : 0.f;
-    const float c = g.inv_t * LOG2E;
+    const float c = g.c;
     // the lane's two largest; a NaN is in neither, and in every sum
     float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
@@ -843,7 +830,8 @@ int wfd_label_scores(const void* logits, int ldl, int dtype, int M, int V, const
     if (M == 0) return WFD_OK;
     if ((k > 0 && (!top_logprob || !top_index)) || (logprob && !labels)) return WFD_ERR_ARG;
     if (!rows_ok(logits, ldl, M, V, dtype)) return WFD_ERR_ARG;
-    Scores g{logits, labels, logprob, entropy, stat, top_logprob, top_index, work, ldl, M, V, k, 1.f / temperature, 0, 0};
+    Scores g{logits, labels, logprob, entropy, stat, top_logprob, top_index, work, ldl, M, V, k, 1.f / temperature,
+             log2e_over(temperature), 0, 0};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WFD_F32) return scores<float>(g, st);
     return dtype == WFD_BF16 ? scores<bf16_t>(g, st) : scores<f16_t>(g, st);
