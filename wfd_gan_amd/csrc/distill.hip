@@ -8,8 +8,8 @@
 // Bound by memory: the row is read once and, with a gradient, written once.  In between it stays packed in the registers of its
 // team (up to 1024 threads x 16 pieces: 131072 16-bit or 65536 fp32 classes), so that maximum, sum and gradient cost one read.  A few
 // long rows are split over workgroups instead: partial sums in a first launch, loss and gradient in a second.
-// Measured (a large copy reaches 5.47 TB/s): 2048 x 128000 bf16 with gradient 246 us = 4.3 TB/s, loss alone 97 us = 5.4 TB/s; 4096 x
-// 32000 bf16 113 us = 4.6 TB/s, loss alone 49 us = 5.3 TB/s; 128 x 100 fp32 5.3 us.
+// Measured (a large copy reaches 5.47 TB/s): 2048 x 128000 bf16 with gradient 210 us = 5.0 TB/s, loss alone 97 us = 5.4 TB/s; 4096 x
+// 32000 bf16 105 us = 5.0 TB/s, loss alone 47 us = 5.6 TB/s; 128 x 100 fp32 5.2 us.
 #include "rowops.h"
 
 namespace {

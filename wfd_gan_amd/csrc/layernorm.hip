@@ -4,8 +4,8 @@
 //             dx = rstd (v - sum v / N - xh sum(v xh) / N),  dw = sum_rows dy xh,  db = sum_rows dy
 // Bound by memory: forward reads and writes a row once, backward reads two and writes one.  A row is held packed in the registers
 // of its team (16 / 64 / 256 / 1024 threads), so the variance is the two-pass one about the true mean and costs no second read.
-// Measured (a large copy reaches 5.47 TB/s): forward 4096 x 2048 fp32 11.9 us = 5.6 TB/s, 8191 x 1401 bf16 11.4 us = 4.0 TB/s;
-// backward 16384 x 4096 bf16 79.9 us = 5.0 TB/s, 5.2 of them the second launch; one row of 2048 2.2 us.
+// Measured (a large copy reaches 5.47 TB/s): forward 4096 x 2048 fp32 11.6 us = 5.8 TB/s, 8191 x 1401 bf16 10.5 us = 4.4 TB/s;
+// backward 16384 x 4096 bf16 78.5 us = 5.1 TB/s, 5.1 of them the second launch; one row of 2048 2.2 us.
 #include "rowops.h"
 
 namespace {
