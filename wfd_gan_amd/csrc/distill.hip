@@ -424,14 +424,15 @@ template <class T, bool TWO> __global__ __launch_bounds__(256) void distill_fini
 constexpr int MAX_V = 1 << 23;
 
 // Rows stay in registers up to 1024 threads x 16 pieces; longer ones are split, and so are the longest of these with a gradient
-// where there are too few to give every CU its own (128000 bf16 classes, us: 1 row 12.7 split, 17.0 whole; 64 rows 15.2, 20.9; 128
-// rows 23.4, 23.0; loss alone of 16 rows 12.0, 9.5; 50000 classes, 16 rows 12.1, 11.8).
+// where there are too few to give every CU its own (us, split and whole: 128000 bf16 classes 1 row 11.9, 16.4; 64 rows 16.1, 18.9; 96
+// rows 20.6, 19.8; 66000 classes 96 rows 15.4, 16.8; 50000 classes 1 row 11.9, 11.4; loss alone of 1 x 128000 11.2, 9.3; fp32 65000
+// classes 32 rows 12.6, 13.5; 64 rows 15.2, 13.9).
 struct DistillShape {
     int splits, chunk;                // splits = 0: the register form
 };
 DistillShape distill_shape(int M, int V, int dtype, bool grad) {
     const int E = elems_of(dtype);
-    if (V <= 1024 * 16 * E && (V <= 512 * 16 * E || M > 96 || !grad)) return {0, V};
+    if (V <= 1024 * 16 * E && (V <= 512 * 16 * E || M > (E == 8 ? 80 : 32) || !grad)) return {0, V};
     const int step = 256 * U * E, steps = cdiv(V, step);
     int S = M >= 1024 ? 1 : cdiv(1024, M > 0 ? M : 1);
     if (S > steps) S = steps;

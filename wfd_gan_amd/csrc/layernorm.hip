@@ -547,13 +547,15 @@ __global__ __launch_bounds__(1024) void ln_bwd_reduce_kernel(const float* part, 
 // The team of a row: the smallest whose registers hold it, from what was measured at 200 MB of rows (us; a large copy takes 37):
 // 16-bit 1401 wide in 64 x 3 pieces 45.7 (64 x 4: 59.8, 256 x 1: 69.6), 2048 in 256 x 1 40.7 (64 x 4: 51.4), 8192 in 1024 x 1 43.1
 // (256 x 4: 54.7); fp32 4096 in 256 x 4 39.6 (1024 x 1: 50.7).  Workgroups: enough for 16 waves on each of 256 CUs, 32 where the
-// team is small and holds little.
+// team is small and holds little; fp32 rows of a wave or less hold so few weights that a team per row is faster (25000 x 1000 36.7, in
+// 1024 workgroups 39.8; 32768 x 300 14.2, 16.1; bf16 1401 wide 44.9, 40.5).
 template <class T, class WT> int ln_fwd(const LnFwd& g, hipStream_t st) {
     constexpr int E = Pack<T>::N;
 #define LN_GO(G, R)                                                                                                      \
     if (g.N <= G * R * E) {                                                                                              \
         constexpr int TEAMS = G < 256 ? 256 / G : 1, NT = G < 256 ? 256 : G;                                             \
-        const int all = cdiv(g.M, TEAMS), most = NT == 1024 ? 512 : G == 256 && R == 1 ? 2048 : 1024;                    \
+        const int all = cdiv(g.M, TEAMS);                                                                                \
+        const int most = NT == 1024 ? 512 : G == 256 && R == 1 ? 2048 : E == 4 && G < 256 ? 1 << 20 : 1024;              \
         hipLaunchKernelGGL((ln_fwd_kernel<T, WT, G, R>), dim3(all < most ? all : most), dim3(NT), 0, st, g);             \
         WFD_CHECK_LAUNCH();                                                                                              \
         return WFD_OK;                                                                                                   \
