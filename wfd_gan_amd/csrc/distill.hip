@@ -501,8 +501,8 @@ int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int*
     // without weight the entries are not read, and the label's term has no temperature
     if (weight == 0.f) K = 0;
     if (K == 0) temperature = 1.f;
-    Distill g{logits, t_index, t_value, labels, row_scale, loss, dlogits, work, ldl, lddl, ldt, M, V, K, temperature, log2e_over(temperature), weight,
-              label_weight, grad_scale, 0, 0, past_caches(M, V, dtype == WFD_F32 ? 4 : 2)};
+    Distill g{logits, t_index, t_value, labels, row_scale, loss, dlogits, work, ldl, lddl, ldt, M, V, K, temperature,
+              log2e_over(temperature), weight, label_weight, grad_scale, 0, 0, past_caches(M, V, dtype == WFD_F32 ? 4 : 2)};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == WFD_F32) return distill<float>(g, st);
     return dtype == WFD_BF16 ? distill<bf16_t>(g, st) : distill<f16_t>(g, st);
