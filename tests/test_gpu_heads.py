@@ -269,6 +269,26 @@ def test_scores_masks_ties_and_order(v, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("k", [1, 48, 49, 64])
+def test_scores_of_many_rows_pick_what_few_rows_pick(k, t):
+    """Around the sizes where a wave takes a row of its own if there are many: the same alternatives as for 40 of the rows."""
+    from wfd_gan_amd import heads
+    g = torch.Generator(device=DEV).manual_seed(k)
+    for v in (1025, 1060, 1151, 1153, 1400, 2049, 2100, 2303, 2305, 4100) + ((8191, 8193) if t == F32 else (16384, 16391)):
+        x = torch.randn(2048, v, generator=g, device=DEV).to(t)
+        x[:, ::7] = -INF
+        y = torch.randint(0, v, (2048,), generator=g, device=DEV, dtype=torch.int32)
+        a = heads.label_logprobs(x, y, k)
+        for lo in (0, 1000, 2008):
+            s = slice(lo, lo + 40)
+            b = heads.label_logprobs(x[s], y[s], k)
+            assert torch.equal(a.top_index[s], b.top_index)
+            want = R.scores(x[s].cpu(), y[s].cpu(), k, 1.0)
+            assert torch.equal(a.top_index[s].cpu().long(), want["top_index"])
+            R.check(a.logprob[s], want["logprob"], want["b_logprob"], F32, "logprob")
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("v", [1, 2, 100, 1401, 5000, 40003])
 def test_scores_of_a_class_alone_in_its_row(v, t):
     """Everything else masked: probability 1 and entropy 0, to the bit, at any value and temperature."""

@@ -729,7 +729,8 @@ constexpr int MAX_V = 1 << 23, MAX_K = 64;   // 64 parts of 32 fp32 steps
 // Few classes stay in the registers of a team inside a wave: 16 lanes where they hold the row and a round per alternative is
 // cheap (16384 x 100, top 64: 38.1 us in rounds of 16 lanes, 28 in the whole wave's list; top 5: 11.5 and 14.5).  Many
 // rows up to 16384 (8192) classes take a wave each: no barriers, four times the rows in flight (16384 x 4000 bf16, top 5: 38.5 us
-// instead of 65.7).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192 16-bit or 4096 fp32 classes).  A row of
+// instead of 65.7) -- unless most of 64 lanes would have only one group to find 64 alternatives in, for then the bound is too low
+// and the list runs over (16384 x 2100, top 64: 346 us, 102 in a workgroup; top 48: 59 in a wave).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192 16-bit or 4096 fp32 classes).  A row of
 // more than 7 steps is split over workgroups (64 at most) where there are fewer than 512 rows: a join costs a launch (32000 bf16, top
 // 20, us: 1 row 9.4 whole, 11.4 split; 600 rows 17.6, 22.0; 65000: 1 row 12.6, 11.4), and so is one whose group maxima would
 // take more than 32 steps' room in LDS.
@@ -742,7 +743,7 @@ struct ScoresShape {
 ScoresShape scores_shape(int M, int V, int dtype, int k) {
     const int E = elems_of(dtype);
     if (V <= FEW * E) return {0, V, 0};
-    if (V <= NARROW * 64 * U * E && M >= MANY) return {-1, V, cdiv(V, 64 * U * E)};
+    if (V <= NARROW * 64 * U * E && M >= MANY && (k <= 48 || V >= 72 * U * E)) return {-1, V, cdiv(V, 64 * U * E)};
     const int step = 256 * U * E, steps = cdiv(V, step);
     int S = M >= 512 || steps <= ALONE ? 1 : cdiv(1024, M > 0 ? M : 1);
     if (S > steps) S = steps;
