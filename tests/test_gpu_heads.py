@@ -269,6 +269,28 @@ def test_scores_masks_ties_and_order(v, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", [3, 2050])
+def test_scores_where_large_values_stand_together(m, t):
+    """Rows that rise, fall, drift, or have one high run: the lists run over and the k-th value itself is looked for."""
+    g = gen(m)
+    for v in (100, 300, 600, 1024, 1401, 2048, 2100, 4000, 16000, 20000) + ((131072,) if m == 3 else ()):
+        rows = min(m, 2050 if v <= 4000 else 3)
+        x = randn(g, rows, v) * 3
+        kind = torch.arange(rows) % 5
+        rise = x.sort(1).values
+        x = torch.where((kind == 0)[:, None], rise, x)
+        x = torch.where((kind == 1)[:, None], rise.flip(1), x)
+        x = torch.where((kind == 2)[:, None], x - torch.arange(v) * (20.0 / v), x)
+        high = torch.zeros(v)
+        high[v // 3: v // 3 + 250] = 30.0
+        x = torch.where((kind == 3)[:, None], x + high, x)
+        x = torch.where((kind == 4)[:, None], (rise * 2).round() / 2, x).to(t)
+        y = torch.randint(0, v, (rows,), generator=g).to(torch.int32)
+        for k in (7, 64):
+            check_scores(x, y, k, 1.0, strided(x, 1, 1) if v == 4000 else x.to(DEV))
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("k", [1, 48, 49, 64])
 def test_scores_of_many_rows_pick_what_few_rows_pick(k, t):
     """Around the sizes where a wave takes a row of its own if there are many: the same alternatives as for 40 of the rows."""

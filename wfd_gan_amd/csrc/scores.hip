@@ -135,8 +135,9 @@ __device__ __forceinline__ void row_store(const Scores& g, long row, const RowEn
 // least k elements reach; so is any wave's k-th largest (a part may be so short that the last waves have none).  The larger of the
 // two is tau.  Only groups whose maximum reaches tau are read again, an element per thread; what reaches tau there goes to a list
 // (expected length: k and a few), whose order is found by counting.  When more than the lists hold reach tau, they are ties at tau but
-// for a few: those above tau are listed and the rest is filled up by walking the ties in index order.  Rows with NaN, and rows that
-// defeat even this (thousands above tau), take the k largest one after another.
+// for a few: those above tau are listed and the rest is filled up by walking the ties in index order.  Where that list runs over as
+// well (sorted rows: thousands above tau), tau becomes the k-th largest value itself, found by counting (4096 sorted rows of 50257
+// bf16, top 64: 0.54 ms, one after another 12.6).  Rows with NaN take the k largest one after another.
 constexpr int U = 4;                      // pieces per group
 
 template <int NT> struct PickLds {
@@ -214,6 +215,53 @@ __device__ __forceinline__ float lanes_nth2(float a, float b, int n) {
     }
 }
 
+// Which of 256 bins, from the highest, holds the need-th element (need comes back as the rank inside it).  Every wave finds it.
+__device__ __forceinline__ int bin_of(const int* hist, int lane, int& need) {
+    int c[4], s = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += c[i] = hist[255 - 4 * lane - i];
+    int upto = s;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += v;
+    }
+    int left = need - (upto - s), at = 0;
+    const int src = (__ffsll((long long)__ballot(upto >= need)) - 1) & 63;      // at least `need` elements are counted
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+        if (at == i && left > c[i]) { left -= c[i]; ++at; }
+    need = __builtin_amdgcn_readlane(left, src);
+    return 255 - 4 * src - __builtin_amdgcn_readlane(at, src);
+}
+// The k-th largest value of x[0, n), of which at least k reach `tau` (no NaN): four counts of eight bits of the order each.  Every count
+// is a walk over the part from the caches: for rows whose large values stand together (sorted ones), where the lists run over.
+template <class T, int NT> __device__ __forceinline__ float kth_value(const T* x, int n, float tau, int k, PickLds<NT>& l) {
+    constexpr int E = Pack<T>::N;
+    const int t = threadIdx.x, lane = t & 63;
+    int* hist = (int*)l.key;
+    unsigned prefix = 0;
+    int need = k;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = t; i < 256; i += NT) hist[i] = 0;
+        team_sync<NT>();
+        for (long i0 = (long)t * E; i0 < n; i0 += NT * E) {
+            const Raw16 d = load_piece(x, (int)i0, n, -INFINITY);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float f = elem<T>(d, e);
+                const unsigned b = order_bits(f);
+                if (f >= tau && i0 + e < n && (shift == 24 || b >> (shift + 8) == prefix >> (shift + 8)))
+                    atomicAdd(&hist[b >> shift & 255], 1);
+            }
+        }
+        team_sync<NT>();
+        prefix |= (unsigned)bin_of(hist, lane, need) << shift;
+        team_sync<NT>();
+    }
+    return order_value(prefix);
+}
+
 // Leaves the k best of x[0, n) (indices from `base`) at out_val / out_idx in order, places without an element as index -1.
 // gmax[it * NT + t]: the group maxima of x[head, n); head (0 or 1) elements in front are in no group.  sum: the part's s (NaN tells
 // of NaN or +inf).
@@ -225,8 +273,7 @@ __device__ __forceinline__ void pick(const T* x0, int n0, int base0, int head, i
     const T* x = x0 + head;
     const int n = n0 - head, base = base0 + head;
     const float front = head ? to_f32(x0[0]) : 0.f;
-    bool slow = sum != sum;
-    if (!slow) {
+    if (sum == sum) {
         const float share = W == 1 ? lanes_nth2(tmax, next, k) : lanes_nth(tmax, (k + W - 1) / W);
         const float own = W > 1 && n < NT * E ? lanes_nth(tmax, k) : -INFINITY;
         if (lane == 0) { l.tau[wave] = share; l.own[wave] = own; }
@@ -241,7 +288,7 @@ __device__ __forceinline__ void pick(const T* x0, int n0, int base0, int head, i
         tau = fmaxf(tau, best);
         int total = 0;
         bool ties = false;
-        for (int pass = 0; pass < 2; ++pass) {
+        for (int pass = 0;; ++pass) {
             for (int it = 0; it < niter; ++it) {
                 const float gm = gmax[it * NT + t];
                 if (pass ? gm > tau : gm >= tau) {
@@ -270,69 +317,65 @@ __device__ __forceinline__ void pick(const T* x0, int n0, int base0, int head, i
             team_sync<NT>();
             total = l.count;
             team_sync<NT>();
-            if (groups <= GROUPS && total <= CAND) break;
-            if (pass == 0) {
-                ties = true;
-                if (t == 0) l.count = l.groups = 0;
-                team_sync<NT>();
-            } else {
-                slow = true;
-            }
+            if ((groups <= GROUPS && total <= CAND) || pass == 2) break;
+            // fewer than k elements are above the k-th largest value, so that the third pass is the last
+            if (pass == 1) tau = kth_value<T, NT>(x0, n0, tau, k, l);
+            ties = true;
+            if (t == 0) l.count = l.groups = 0;
+            team_sync<NT>();
         }
-        if (!slow) {
-            // order by counting: the list is short, every thread reads all of it (broadcasts)
-            for (int a = t; a < total; a += NT) {
-                const unsigned long long key = l.key[a];
-                int rank = 0;
+        // order by counting: the list is short, every thread reads all of it (broadcasts)
+        for (int a = t; a < total; a += NT) {
+            const unsigned long long key = l.key[a];
+            int rank = 0;
 #pragma unroll 8
-                for (int b = 0; b < total; ++b) rank += l.key[b] > key;
-                if (rank < k) {
-                    const int i = (int)~(unsigned)key;
-                    out_val[rank] = to_f32(x0[i - base0]);
-                    out_idx[rank] = i;
-                }
+            for (int b = 0; b < total; ++b) rank += l.key[b] > key;
+            if (rank < k) {
+                const int i = (int)~(unsigned)key;
+                out_val[rank] = to_f32(x0[i - base0]);
+                out_idx[rank] = i;
             }
-            int have = total;
-            if (ties && have < k) {
-                // ties at tau in index order, E elements per thread at a time, until there are enough
-                if (head && front == tau) {
-                    if (t == 0) { out_val[have] = tau; out_idx[have] = base0; }
-                    ++have;
-                }
-                for (long p0 = 0; p0 * E < n && have < k; p0 += NT) {
-                    const long i0 = (p0 + t) * E;
-                    unsigned hit = 0;
-                    if (i0 < n) {
-                        const Raw16 d = load_piece(x, (int)i0, n, -INFINITY);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) hit |= (elem<T>(d, e) == tau && i0 + e < n) ? 1u << e : 0u;
-                    }
-                    int before = __popc(hit);                           // inclusive count over the lanes
-#pragma unroll
-                    for (int o = 1; o < 64; o <<= 1) {
-                        const int v = __shfl_up(before, o, 64);
-                        if (lane >= o) before += v;
-                    }
-                    if (lane == 63) l.run[wave] = before;
-                    team_sync<NT>();
-                    int at = have + before - __popc(hit), all = 0;
-#pragma unroll
-                    for (int i = 0; i < W; ++i) {
-                        if (i < wave) at += l.run[i];
-                        all += l.run[i];
-                    }
-                    for (int e = 0; e < E; ++e)
-                        if (hit >> e & 1) {
-                            if (at < k) { out_val[at] = tau; out_idx[at] = base + (int)i0 + e; }
-                            ++at;
-                        }
-                    have += all;
-                    team_sync<NT>();
-                }
-            }
-            for (int a = have + t; a < k; a += NT) { out_val[a] = -INFINITY; out_idx[a] = -1; }
-            return;
         }
+        int have = total;
+        if (ties && have < k) {
+            // ties at tau in index order, E elements per thread at a time, until there are enough
+            if (head && front == tau) {
+                if (t == 0) { out_val[have] = tau; out_idx[have] = base0; }
+                ++have;
+            }
+            for (long p0 = 0; p0 * E < n && have < k; p0 += NT) {
+                const long i0 = (p0 + t) * E;
+                unsigned hit = 0;
+                if (i0 < n) {
+                    const Raw16 d = load_piece(x, (int)i0, n, -INFINITY);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) hit |= (elem<T>(d, e) == tau && i0 + e < n) ? 1u << e : 0u;
+                }
+                int before = __popc(hit);                           // inclusive count over the lanes
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int v = __shfl_up(before, o, 64);
+                    if (lane >= o) before += v;
+                }
+                if (lane == 63) l.run[wave] = before;
+                team_sync<NT>();
+                int at = have + before - __popc(hit), all = 0;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    if (i < wave) at += l.run[i];
+                    all += l.run[i];
+                }
+                for (int e = 0; e < E; ++e)
+                    if (hit >> e & 1) {
+                        if (at < k) { out_val[at] = tau; out_idx[at] = base + (int)i0 + e; }
+                        ++at;
+                    }
+                have += all;
+                team_sync<NT>();
+            }
+        }
+        for (int a = have + t; a < k; a += NT) { out_val[a] = -INFINITY; out_idx[a] = -1; }
+        return;
     }
     unsigned long long last = ~0ull;
     for (int j = 0; j < k; ++j) {
@@ -636,7 +679,9 @@ template <class T, int G, int R> __global__ __launch_bounds__(256) void scores_f
             }
         }
     }
-    // one alternative after another: best of the lane, best of the team, and the winner looks for its next
+    // one alternative after another: best of the lane, best of the team, and the winner looks for its next.  Rows with NaN, short teams,
+    // and rows whose list runs over without ties (16384 sorted rows of 1500 bf16, top 64: 0.4 ms; the count of kth_value here costs
+    // every row 65 registers, and random ones 50 us instead of 31)
     unsigned long long done = 0;                              // elements of this lane already given
     for (int j = 0; j < g.k; ++j) {
         unsigned best = 0;
