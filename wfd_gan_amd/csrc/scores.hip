@@ -424,8 +424,8 @@ __device__ __forceinline__ Stat walk(const T* x, int n, float c, float* gmax, fl
         take(d);
     }
     if ((long)it * STEP < n) {
-        // the rest, as far as any lane of the wave has a piece.  All loads first, and none under a condition (see team_load): a piece that
-        // would reach past the end starts earlier, its elements before i0 are another piece's
+        // the rest, as far as any lane of the wave has a piece.  All loads first, and none under a condition (see team_load): a piece
+        // that would reach past the end starts earlier, its elements before i0 are another piece's
         float group = -INFINITY;
         const int first = (t & ~63) * E, i0 = it * STEP + t * E, last = max(n - E, 0);
         Raw16 d[U];
@@ -775,8 +775,8 @@ constexpr int MAX_V = 1 << 23, MAX_K = 64;   // 64 parts of 32 fp32 steps
 // cheap (16384 x 100, top 64: 38.1 us in rounds of 16 lanes, 28 in the whole wave's list; top 5: 11.5 and 14.5).  Many
 // rows up to 16384 (8192) classes take a wave each: no barriers, four times the rows in flight (16384 x 4000 bf16, top 5: 38.5 us
 // instead of 65.7) -- unless most of 64 lanes would have only one group to find 64 alternatives in, for then the bound is too low
-// and the list runs over (16384 x 2100, top 64: 346 us, 102 in a workgroup; top 48: 59 in a wave).  Beyond, a workgroup walks a row in steps of 4 pieces per thread (8192 16-bit or 4096 fp32 classes).  A row of
-// more than 7 steps is split over workgroups (64 at most) where there are fewer than 512 rows: a join costs a launch (32000 bf16, top
+// and the list runs over (16384 x 2100, top 64: 346 us, 102 in a workgroup; top 48: 59 in a wave).  Beyond, a workgroup walks a row
+// in steps of 4 pieces per thread (8192 16-bit or 4096 fp32 classes).  A row of more than 7 steps is split over workgroups (64 at most) where there are fewer than 512 rows: a join costs a launch (32000 bf16, top
 // 20, us: 1 row 9.4 whole, 11.4 split; 600 rows 17.6, 22.0; 65000: 1 row 12.6, 11.4), and so is one whose group maxima would
 // take more than 32 steps' room in LDS.
 constexpr int FEW = 256;                  // lanes * pieces of the team form: up to 2048 16-bit or 1024 fp32 classes
