@@ -199,6 +199,23 @@ template <class T, class WT> __global__ __launch_bounds__(1024) void ln_fwd_long
     }
 }
 
+// What an element behind the last whole piece adds to the row's two sums, and its dx.  A row of one or two columns has no others, and
+// there nearly everything cancels: dx of one column is 0, of two what eps leaves of the difference.  Each product is therefore rounded
+// before it is added, so that equal terms cancel to the bit; fused, the one column's dx was rstd times the rounding of dy w.
+__device__ __forceinline__ void rest_add(float& a, float& b, float v, float xh) {
+#pragma clang fp contract(off)
+    a += v;
+    b += v * xh;
+}
+__device__ __forceinline__ float rest_dx(float rstd, float v, float xh, float c1, float c2) {
+#pragma clang fp contract(off)
+    return rstd * (v - c1 - xh * c2);
+}
+__device__ __forceinline__ float rest_product(float dy, float w) {
+#pragma clang fp contract(off)
+    return dy * w;
+}
+
 // ---- backward: a team walks rows, its threads keep the sums of dy xh and dy of their columns in registers ---------------
 // No sum is shared while rows run, so none depends on an order; a workgroup leaves 2 N sums at its end, and a second launch adds them.
 template <class T, class WT, int G, int R>
@@ -265,10 +282,9 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
                 sb[r][e] += d;
             }
         }
-        const float xhl = (k.xl - k.mean) * k.rstd;
+        const float xhl = (k.xl - k.mean) * k.rstd, vl = rest_product(k.dyl, wl);
         if (rest) {
-            a = fmaf(k.dyl, wl, a);
-            b = fmaf(k.dyl * wl, xhl, b);
+            rest_add(a, b, vl, xhl);
             swl = fmaf(k.dyl, xhl, swl);
             sbl += k.dyl;
         }
@@ -288,7 +304,7 @@ __global__ __launch_bounds__(G < 256 ? 512 : G) void ln_bwd_kernel(LnBwd g) {
                 }
                 store16(o + (r * G + t) * E, pack<T>(f));
             }
-        if (t < rest) o[P * E + t] = from_f32<T>(k.rstd * (k.dyl * wl - fmaf(xhl, c2, c1)));
+        if (t < rest) o[P * E + t] = from_f32<T>(rest_dx(k.rstd, vl, xhl, c1, c2));
         if constexpr (!AHEAD)
             if (row + step < g.M) fetch(n, row + step);
         k = n;
@@ -431,7 +447,7 @@ template <class T, class WT, int G, int R> __device__ __forceinline__ void bwd_r
     }
     if (t < rest) {
         xhl = (to_f32(x[P * E + t]) - mean) * rstd;
-        vl = to_f32(dy[P * E + t]) * (g.W ? to_f32(((const WT*)g.W)[P * E + t]) : 1.f);
+        vl = rest_product(to_f32(dy[P * E + t]), g.W ? to_f32(((const WT*)g.W)[P * E + t]) : 1.f);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -440,8 +456,7 @@ template <class T, class WT, int G, int R> __device__ __forceinline__ void bwd_r
             a += v[r][e];
             b = fmaf(v[r][e], xh[r][e], b);
         }
-    a += vl;
-    b = fmaf(vl, xhl, b);
+    rest_add(a, b, vl, xhl);
     const float2 c = team_sum2<G>(a, b, slot);
     const float c1 = c.x * inv, c2 = c.y * inv;
 #pragma unroll
@@ -452,7 +467,7 @@ template <class T, class WT, int G, int R> __device__ __forceinline__ void bwd_r
             for (int e = 0; e < E; ++e) f[e] = rstd * (v[r][e] - fmaf(xh[r][e], c2, c1));
             store16(o + (r * G + t) * E, pack<T>(f));
         }
-    if (t < rest) o[P * E + t] = from_f32<T>(rstd * (vl - fmaf(xhl, c2, c1)));
+    if (t < rest) o[P * E + t] = from_f32<T>(rest_dx(rstd, vl, xhl, c1, c2));
 }
 template <class T, class WT, int G, int R>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void ln_bwd_few_kernel(LnBwd g, int first) {
