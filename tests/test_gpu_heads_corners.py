@@ -1,4 +1,5 @@
-"""GPU: corners of the classifier-head operators' documented range: rows of one and two columns."""
+"""GPU: corners of the classifier-head operators' documented range: rows of one and two columns, masks of the type's
+lowest value at low temperatures."""
 import pytest
 import torch
 
@@ -36,3 +37,49 @@ def test_norm_backward_of_one_and_two_columns(n, m, t):
         want = (rstd * (v - total(v) / n - xh * (total(v * xh) / n))).to(t)
         assert n == 2 or float(dx.abs().max()) == 0
         assert torch.equal(dx, want)
+
+
+# ---- entropy under masks of the type's lowest value -------------------------------------------------------------------------
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("temp", [1e-6, 1e-5, 1e-4, 1e-3])
+@pytest.mark.parametrize("m,v", [(1, 100), (3, 1401), (3, 5003), (2050, 5003), (1, 50257), (3, 50257), (600, 50257), (1, 128000),
+                                 (3, 128000), (600, 128000)])
+def test_entropy_of_one_class_left_among_the_lowest_values(m, v, temp, t):
+    """Whole lanes, waves and parts hold masked classes only.  Everything but one class has share 0, so log probability and entropy
+    are 0 to the bit, and so is the gradient of both."""
+    from wfd_gan_amd import heads
+    at = torch.randint(0, v, (m,), generator=gen(v + m)).to(DEV)
+    x = torch.full((m, v), torch.finfo(t).min, dtype=t, device=DEV)
+    x[torch.arange(m, device=DEV), at] = 1.5
+    y = at.to(torch.int32)
+    for k in (0, 1):
+        r = heads.label_logprobs(x, y, k, temperature=temp)
+        assert float(r.entropy.abs().max()) == 0 and float(r.logprob.abs().max()) == 0
+        if k:
+            assert torch.equal(r.top_index[:, 0], y) and float(r.top_logprob.abs().max()) == 0
+    one = torch.ones(m, device=DEV)
+    d = heads.label_logprobs_backward(x, y, r, one, one, temperature=temp)
+    assert float(d.abs().max()) == 0
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("temp", [1e-5, 1e-3, 1.0])
+@pytest.mark.parametrize("m,v", [(4, 1000), (4, 20011), (2050, 4000), (4, 131072)])
+def test_entropy_of_a_short_run_left_among_the_lowest_values(m, v, temp, t):
+    """Seven classes in a row are left: against the definition, with the gradient of log probability and entropy."""
+    from wfd_gan_amd import heads
+    g = gen(v)
+    x = torch.full((m, v), torch.finfo(t).min, dtype=t)
+    lo = v // 3
+    x[:, lo:lo + 7] = (torch.randn(m, 7, generator=g) * temp).to(t)
+    y = (lo + torch.randint(0, 7, (m,), generator=g)).to(torch.int32)
+    r = heads.label_logprobs(x.to(DEV), y.to(DEV), 5, temperature=temp)
+    rows = [0, 1, 2, m - 1]
+    want = R.scores(x[rows], y[rows], 5, temp)
+    R.check(r.entropy[rows], want["entropy"], want["b_entropy"], F32, "entropy")
+    R.check(r.logprob[rows], want["logprob"], want["b_logprob"], F32, "logprob")
+    assert torch.equal(r.top_index[rows].cpu().long(), want["top_index"])
+    dl, dh = torch.randn(m, generator=g), torch.randn(m, generator=g)
+    d = heads.label_logprobs_backward(x.to(DEV), y.to(DEV), r, dl.to(DEV), dh.to(DEV), temperature=temp)
+    want, bound = R.scores_backward(x[rows], y[rows], r.stat[rows], r.entropy[rows], dl[rows], dh[rows], temp)
+    R.check(d[rows], want, bound, t, "dlogits")

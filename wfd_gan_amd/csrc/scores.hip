@@ -63,7 +63,7 @@ struct Stat {
     float m, s, u;
 };
 __device__ __forceinline__ void stat_to(Stat& a, float m, float c) {          // moves a to a maximum m >= a.m
-    const float d = fmaxf(a.m - m, -1e30f) * c, w = exp2_of(d);
+    const float d = fmaxf((a.m - m) * c, FAINT), w = exp2_of(d);         // floored last: s * d stays finite where w is 0
     a.u = w * fmaf(a.s, d, a.u);
     a.s *= w;
     a.m = m;
