@@ -1,5 +1,5 @@
 """GPU: corners of the classifier-head operators' documented range: rows of one and two columns, masks of the type's
-lowest value at low temperatures."""
+lowest value at low temperatures, NaN at the first class."""
 import pytest
 import torch
 
@@ -83,3 +83,23 @@ def test_entropy_of_a_short_run_left_among_the_lowest_values(m, v, temp, t):
     d = heads.label_logprobs_backward(x.to(DEV), y.to(DEV), r, dl.to(DEV), dh.to(DEV), temperature=temp)
     want, bound = R.scores_backward(x[rows], y[rows], r.stat[rows], r.entropy[rows], dl[rows], dh[rows], temp)
     R.check(d[rows], want, bound, t, "dlogits")
+
+
+# ---- NaN at the first class -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,v", [(3, 5), (3, 64), (3, 100), (3, 1401), (3, 2049), (3, 9001), (2050, 3001), (600, 33000), (3, 131075)])
+def test_nan_at_the_first_class_is_the_first_alternative(m, v, t):
+    """NaN stand before all numbers and by index among themselves, in every form: rows in a wave, in a workgroup, in parts."""
+    from wfd_gan_amd import heads
+    x = torch.randn(m, v, generator=gen(v)).to(t)
+    x[:, 0] = float("nan")
+    x[1, 2] = float("nan")
+    x[2, v // 2] = INF
+    if m > 600:
+        x[600] = float("nan")                             # nothing else in the row
+    rows = [0, 1, 2, min(m - 1, 600)]
+    for k in (1, min(v, 20)):
+        r = heads.label_logprobs(x.to(DEV), None, k)
+        want = R.scores(x[rows], None, k, 1.0)
+        assert torch.equal(r.top_index[rows].cpu().long(), want["top_index"])
+        assert int(r.top_index[:, 0].abs().max()) == 0 and bool(r.top_logprob.isnan().all())

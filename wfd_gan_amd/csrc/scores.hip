@@ -40,9 +40,11 @@ struct ScoresBwd {
     bool past;            // the gradient is written past the caches
 };
 
-// order of alternatives: larger value first (NaN before every number, -0 as 0), then the lower index
+// order of alternatives: larger value first (NaN before every number, -0 as 0), then the lower index.  NaN's place is one below the
+// largest, so that the key of ~0 belongs to no element: a walk that takes one after another starts above it.
+constexpr unsigned NAN_BITS = 0xfffffffeu;
 __device__ __forceinline__ unsigned order_bits(float v) {
-    if (v != v) return 0xffffffffu;
+    if (v != v) return NAN_BITS;
     const unsigned u = __float_as_uint(v + 0.f);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
@@ -51,7 +53,7 @@ __device__ __forceinline__ unsigned long long order_key(float v, int i) {
 }
 
 __device__ __forceinline__ float order_value(unsigned b) {
-    return b == 0xffffffffu ? NAN : __uint_as_float((b & 0x80000000u) ? b ^ 0x80000000u : ~b);
+    return b == NAN_BITS ? NAN : __uint_as_float((b & 0x80000000u) ? b ^ 0x80000000u : ~b);
 }
 
 // ---- what one workgroup knows of its part of a row -----------------------------------------------------------------------
