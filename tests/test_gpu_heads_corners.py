@@ -1,5 +1,5 @@
 """GPU: corners of the classifier-head operators' documented range: rows of one and two columns, masks of the type's
-lowest value at low temperatures, NaN at the first class."""
+lowest value at low temperatures, NaN at the first class, rows whose only entry of the teacher is wrong."""
 import pytest
 import torch
 
@@ -103,3 +103,24 @@ def test_nan_at_the_first_class_is_the_first_alternative(m, v, t):
         want = R.scores(x[rows], None, k, 1.0)
         assert torch.equal(r.top_index[rows].cpu().long(), want["top_index"])
         assert int(r.top_index[:, 0].abs().max()) == 0 and bool(r.top_logprob.isnan().all())
+
+
+# ---- a teacher whose only entry is wrong --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("v", [5, 100, 1401, 40003, 140001])
+@pytest.mark.parametrize("temp", [1.0, 2.0])
+def test_a_wrong_index_alone_in_its_row_shows_in_loss_and_gradient(v, temp, t):
+    """Index V with no other entry, with absent ones and with ones at -inf; without labels, and with label -1."""
+    from wfd_gan_amd import heads
+    x = torch.randn(4, v, generator=gen(v)).to(t).to(DEV)
+    y = torch.full((4,), -1, dtype=torch.int32, device=DEV)
+    good = [0, 1, 2]
+    for ti, tv in (([[v], [0], [v + 5], [v]], [[0.5]] * 4),
+                   ([[v, -1, -1], good, [-1, v, -1], [1, v, 2]], [[0.5] * 3, [0.1, 0.2, 0.3], [0.5] * 3, [-INF, 1.0, -INF]])):
+        ti, tv = torch.tensor(ti, dtype=torch.int32, device=DEV), torch.tensor(tv, device=DEV)
+        for kw in (dict(), dict(labels=y, weight=0.6, label_weight=0.4)):
+            r = heads.distill_loss(x, ti, tv, temperature=temp, **kw)
+            assert r.loss.isnan().tolist() == [True, False, True, True]
+            assert r.dlogits.isnan().all(1).tolist() == [True, False, True, True]
+            assert bool(r.dlogits[1].isfinite().all())
+            assert heads.distill_loss(x, ti, tv, temperature=temp, grad=False, **kw).loss.isnan().tolist() == [True, False, True, True]

@@ -145,12 +145,12 @@ __device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Ta
     GradRow d;
     d.m = s.m;
     d.r = g.scale * (g.row_scale ? g.row_scale[row] : 1.f);
-    if (wrong) d.r = NAN;
     const bool empty = s.s == 0.f, on = t.sum != 0.f;
     d.rt = on ? d.r * g.w * g.temp / t.sum : 0.f;
     d.cw = on ? d.r * g.w * g.temp / s.s : 0.f;
     d.cu = y >= 0 ? d.r * g.u / s.s1 : 0.f;
-    if (empty) d.cw = d.cu = wrong ? NAN : 0.f;
+    if (empty) d.cw = d.cu = 0.f;
+    if (wrong) d.r = d.cw = d.cu = NAN;              // also where nothing else is left of the row
     if constexpr (!TWO) d.cw += d.cu;
     d.R = d.m * c;
     d.R1 = d.m * LOG2E;
