@@ -1,5 +1,6 @@
 """GPU: corners of the classifier-head operators' documented range: rows of one and two columns, masks of the type's
-lowest value at low temperatures, NaN at the first class, rows whose only entry of the teacher is wrong."""
+lowest value at low temperatures, NaN at the first class, rows whose only entry of the teacher is wrong, rows
+without a term."""
 import pytest
 import torch
 
@@ -124,3 +125,41 @@ def test_a_wrong_index_alone_in_its_row_shows_in_loss_and_gradient(v, temp, t):
             assert r.dlogits.isnan().all(1).tolist() == [True, False, True, True]
             assert bool(r.dlogits[1].isfinite().all())
             assert heads.distill_loss(x, ti, tv, temperature=temp, grad=False, **kw).loss.isnan().tolist() == [True, False, True, True]
+
+
+# ---- rows without a term ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("v", [5, 100, 1401, 40003, 140001])
+def test_distill_rows_without_a_term_have_gradient_zero_whatever_they_hold(v, t):
+    """Padding rows: no entry (or none above -inf) and no label.  Their loss is 0, so their gradient is, also where the logits are NaN
+    or infinite; the rows beside them keep theirs, and a NaN row with a term is NaN."""
+    from wfd_gan_amd import heads
+    m = 9
+    x = torch.randn(m, v, generator=gen(v)).to(t)
+    x[0] = float("nan")
+    x[1, v // 2] = INF
+    x[2] = -INF
+    x[3, 0] = float("nan")
+    x[4, v - 1] = float("nan")
+    x[7, 1] = float("nan")
+    ti = torch.tensor([[-1, -1]] * 6 + [[0, 1]] * 3, dtype=torch.int32)
+    ti[4] = torch.tensor([0, 1])
+    tv = torch.zeros(m, 2)
+    tv[4] = -INF
+    y = torch.tensor([-1] * 6 + [2, 2, -1], dtype=torch.int32)
+    none, bad, fine = slice(0, 6), 7, [6, 8]
+    for kw in (dict(), dict(labels=y.to(DEV), weight=0.5, label_weight=0.5),
+               dict(labels=y.to(DEV), temperature=2.0, weight=0.5, label_weight=0.5), dict(temperature=0.5)):
+        r = heads.distill_loss(x.to(DEV), ti.to(DEV), tv.to(DEV), **kw)
+        assert float(r.loss[none].abs().max()) == 0 and float(r.dlogits[none].abs().max()) == 0
+        assert bool(r.loss[bad].isnan()) and bool(r.dlogits[bad].isnan().all())
+        w, u = kw.get("weight", 1.0), kw.get("label_weight", 0.0)
+        loss, bl, d, bd = R.distill(x[fine], ti[fine], tv[fine], y[fine] if u else None, kw.get("temperature", 1.0), w, u,
+                                    torch.ones(2))
+        R.check(r.loss[fine], loss, bl, F32, "loss")
+        R.check(r.dlogits[fine], d, bd, t, "dlogits")
+    # the label's term alone
+    r = heads.distill_loss(x.to(DEV), ti.to(DEV), tv.to(DEV), y.to(DEV), weight=0.0, label_weight=1.0)
+    rows = [0, 1, 2, 3, 4, 5, 8]
+    assert float(r.loss[rows].abs().max()) == 0 and float(r.dlogits[rows].abs().max()) == 0
+    assert bool(r.dlogits[bad].isnan().all()) and bool(r.dlogits[6].isfinite().all()) and float(r.dlogits[6].abs().max()) > 0

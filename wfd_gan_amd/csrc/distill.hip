@@ -3,7 +3,8 @@
 // Student row x over V classes, p = softmax(x / T), p1 = softmax(x):
 //   loss = w T^2 sum_j q_j (ln q_j - ln p(i_j)) - u ln p1(y)
 //   d x_i = r (w T (p_i [any entry] - sum_{j: i_j = i} q_j) + u (p1_i - [i = y]))          r = grad_scale * row_scale[row]
-// An index that occurs twice counts twice.  No entry (or none above -inf): the first term is 0; y < 0: the second is 0.
+// An index that occurs twice counts twice.  No entry (or none above -inf): the first term is 0; y < 0: the second is 0; a row without
+// either has gradient 0 whatever it holds, NaN too.
 // A row that holds nothing but -inf has loss +inf and gradient 0; an index or label >= V makes its row NaN.
 // Bound by memory: the row is read once and, with a gradient, written once.  In between it stays packed in the registers of its
 // team (up to 1024 threads x 16 pieces: 131072 16-bit or 65536 fp32 classes), so that maximum, sum and gradient cost one read.  A few
@@ -137,7 +138,8 @@ __device__ __forceinline__ float row_loss(const Distill& g, long row, int lane, 
 struct GradRow {
     float m, cw, cu, r, rt;        // r = grad_scale * row_scale, rt = r w T / (sum of the teacher's exponentials)
     float R, R1, kw, ku;           // m c and m log2(e) rounded, cw and cu with what the rounding left
-    bool wide;                     // m c beyond WIDE
+    bool wide;                     // m c beyond WIDE, or no term left
+    bool none;                     // no term left: gradient 0
 };
 template <bool TWO>
 __device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Taught& t, const RowSums& s, int y, bool wrong,
@@ -154,7 +156,8 @@ __device__ __forceinline__ GradRow grad_row(const Distill& g, long row, const Ta
     if constexpr (!TWO) d.cw += d.cu;
     d.R = d.m * c;
     d.R1 = d.m * LOG2E;
-    d.wide = !(fabsf(d.R) < WIDE && fabsf(d.R1) < WIDE);
+    d.none = !on && y < 0 && !wrong;
+    d.wide = d.none || !(fabsf(d.R) < WIDE && fabsf(d.R1) < WIDE);       // one test per piece for both
     d.kw = d.cw * exp2_of(-fmaf(d.m, c, -d.R));
     d.ku = d.cu * exp2_of(-fmaf(d.m, LOG2E, -d.R1));
     return d;
@@ -164,6 +167,7 @@ template <bool TWO> __device__ __forceinline__ float grad_dense(const GradRow& d
         const float v = d.kw * exp2_of(fmaf(x, c, -d.R));
         return TWO ? fmaf(d.ku, exp2_of(fmaf(x, LOG2E, -d.R1)), v) : v;
     }
+    if (d.none) return 0.f;
     const float v = d.cw * exp2_of((x - d.m) * c);
     return TWO ? fmaf(d.cu, exp2_of((x - d.m) * LOG2E), v) : v;
 }

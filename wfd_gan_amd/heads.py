@@ -326,7 +326,8 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_valu
 
     ``teacher_index`` (int32) and ``teacher_value`` (float32: logits or log probabilities, their offset does not matter) are
     (..., K) with K <= 256; an index < 0 is no entry, an index that occurs twice counts twice.  ``labels`` (int32) are needed
-    when ``label_weight`` is not 0; negative = no label.  ``dlogits`` carries ``grad_scale * row_scale`` (the losses do not).
+    when ``label_weight`` is not 0; negative = no label.  A row with neither entry nor label has loss and gradient 0 whatever it
+    holds.  ``dlogits`` carries ``grad_scale * row_scale`` (the losses do not).
     An index or label >= classes makes its row NaN.  ``out.dlogits`` may be ``logits``."""
     who = "distill_loss"
     code = _code(logits, "logits")
