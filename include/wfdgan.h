@@ -523,7 +523,8 @@ int wfd_label_scores(const void* logits, int ldl, int dtype, int M, int V, const
                      void* stream);
 int wfd_label_scores_floats(int M, int V, int dtype, int k);
 /* dlogits = the gradient of sum_m d_logprob[m] * logprob[m] + d_entropy[m] * entropy[m]; either may be NULL (0).  stat and
- * entropy are wfd_label_scores' at the same temperature.  A row of nothing but -inf has gradient 0.  dlogits may be logits. */
+ * entropy are wfd_label_scores' at the same temperature.  A row of nothing but -inf has gradient 0, and so has one without a label
+ * where d_entropy is NULL, whatever it holds.  dlogits may be logits. */
 int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, const int* labels, float temperature,
                          const float* stat, const float* entropy, const float* d_logprob, const float* d_entropy,
                          void* dlogits, int lddl, void* stream);

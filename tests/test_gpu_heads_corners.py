@@ -163,3 +163,22 @@ def test_distill_rows_without_a_term_have_gradient_zero_whatever_they_hold(v, t)
     rows = [0, 1, 2, 3, 4, 5, 8]
     assert float(r.loss[rows].abs().max()) == 0 and float(r.dlogits[rows].abs().max()) == 0
     assert bool(r.dlogits[bad].isnan().all()) and bool(r.dlogits[6].isfinite().all()) and float(r.dlogits[6].abs().max()) > 0
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("v", [5, 100, 1401, 40003])
+def test_scores_rows_without_a_label_have_gradient_zero_whatever_they_hold(v, t):
+    """Without a label the log probability is 0 and without d_entropy nothing else is left to differentiate."""
+    from wfd_gan_amd import heads
+    x = torch.randn(5, v, generator=gen(v)).to(t)
+    x[0] = float("nan")
+    x[1, v // 2] = INF
+    x[3, 1] = float("nan")
+    y = torch.tensor([-1, -3, -1, 2, 2], dtype=torch.int32, device=DEV)
+    one = torch.ones(5, device=DEV)
+    r = heads.label_logprobs(x.to(DEV), y)
+    assert float(r.logprob[:3].abs().max()) == 0
+    d = heads.label_logprobs_backward(x.to(DEV), y, r, one)
+    assert float(d[:3].abs().max()) == 0 and bool(d[3].isnan().all()) and bool(d[4].isfinite().all()) and float(d[4].abs().max()) > 0
+    d = heads.label_logprobs_backward(x.to(DEV), y, r, one, one)
+    assert d.isnan().all(1).tolist() == [True, True, False, True, False]

@@ -709,14 +709,14 @@ template <class T, int G, int R> __global__ __launch_bounds__(256) void scores_f
 struct BwdRow {
     float m, log_s, q0, q1, dl;      // d = -p (q0 + q1 ln p), + dl at y
     int y;
-    bool empty;
+    bool zero;                       // nothing but -inf, or nothing to differentiate: no label and no entropy, whatever the row holds
 };
 __device__ __forceinline__ BwdRow bwd_row(const ScoresBwd& g, long row) {
     BwdRow r;
     r.m = g.stat[2 * row];
     r.log_s = g.stat[2 * row + 1];
-    r.empty = r.m == -INFINITY && r.log_s == 0.f;
     r.y = g.labels ? g.labels[row] : -1;
+    r.zero = (r.m == -INFINITY && r.log_s == 0.f) || (r.y < 0 && !g.d_ent);
     r.dl = g.d_lp && r.y >= 0 ? g.d_lp[row] * g.inv_t : 0.f;
     if (r.y >= g.V) r.dl = NAN;
     r.q1 = g.d_ent ? g.d_ent[row] * g.inv_t : 0.f;
@@ -735,7 +735,7 @@ template <class T> __device__ __forceinline__ void bwd_piece(const ScoresBwd& g,
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (i0 + e == r.y) f[e] += r.dl;
-    if (r.empty)
+    if (r.zero)
 #pragma unroll
         for (int e = 0; e < E; ++e) f[e] = 0.f;
     store_piece(o, i0, g.V, f, g.past);
