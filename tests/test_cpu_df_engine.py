@@ -1,0 +1,25 @@
+"""CPU: host-side decisions of the DF observer's engine around the classifier-head operators; nothing here reaches a GPU."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from wfd_gan_amd import df_engine
+
+
+def test_observer_batches_are_on_the_observers_device_wherever_the_rows_are(monkeypatch):
+    """Kernels get the addresses of these buffers: rows on the host must not put them there ("meta" stands for the GPU)."""
+    seen = []
+    buffers = dict(Y=None, PO=None, F1=None, F2=None, LOG=torch.zeros(3, 4), ldc=4)
+    monkeypatch.setattr(df_engine, "observer_buffers", lambda df, n, dev: (seen.append(torch.device(dev)), buffers)[1])
+    monkeypatch.setattr(df_engine, "observer_forward", lambda pl, df, xin, *a: seen.append(xin.device))
+    monkeypatch.setattr(df_engine, "Plan", lambda ws: SimpleNamespace(run=lambda: None))
+    df = SimpleNamespace(L=5, C=2, fc_w=torch.empty(2, 512, device="meta"))
+    got = [(a, tuple(l.shape)) for a, l in df_engine.observer_logits(df, torch.zeros(7, 5), None, 3)]
+    assert [a for a, _ in got] == [0, 3, 6] and got[0][1] == (3, 2)
+    assert len(seen) == 4 and all(d.type == "meta" for d in seen)
+
+
+def test_teacher_alternatives_refuses_rows_on_the_host():
+    with pytest.raises(ValueError, match="must be on the GPU"):
+        df_engine.teacher_alternatives({}, 5, 2, torch.zeros(7, 5), 1)

@@ -1,0 +1,21 @@
+"""GPU: the DF observer's read-outs over rows that are on the host, on the GPU, or in another layout."""
+import pytest
+import torch
+
+from oracle import wfdgan_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def test_read_outs_of_rows_on_the_host():
+    """accuracy() and evaluate() copy each batch to the GPU; the numbers are those of rows that are there already."""
+    from wfd_gan_amd.df_engine import DFTrainEngine
+    L, C, N = 120, 7, 150
+    torch.manual_seed(3)
+    eng = DFTrainEngine(L, C, 8, O.make_df_state(L, C), device=DEV)
+    g = torch.Generator().manual_seed(7)
+    X, y = torch.rand(N, L, generator=g), torch.randint(0, C, (N,), generator=g)
+    there = eng.accuracy(X.to(DEV), y.to(DEV), bs=64), eng.evaluate(X.to(DEV), y.to(DEV), 3, bs=64)
+    assert (eng.accuracy(X, y, bs=64), eng.evaluate(X, y, 3, bs=64)) == there
+    assert (eng.accuracy(X[:, None], y, bs=64), eng.evaluate(X.double(), y.to(DEV), 3, bs=64)) == there

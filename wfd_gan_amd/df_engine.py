@@ -53,9 +53,10 @@ class Distill(NamedTuple):
 
 
 def observer_logits(df: ObserverDF, X: torch.Tensor, ws: torch.Tensor, bs: int):
-    """(first row, logits of rows [first, first + n)) of an eval-mode observer over device-resident X (N, L), in batches of
-    ``bs``; the logits are a view of a buffer that the next batch of that size writes again."""
-    N, dev, plans = X.shape[0], X.device, {}
+    """(first row, logits of rows [first, first + n)) of an eval-mode observer over X (N, L), in batches of ``bs``; X may be
+    anywhere, the batches and their buffers are on the observer's device.  The logits are a view of a buffer that the next batch
+    of that size writes again."""
+    N, dev, plans = X.shape[0], df.fc_w.device, {}
     for a in range(0, N, bs):
         n = min(bs, N - a)
         if n not in plans:
@@ -72,7 +73,10 @@ def observer_logits(df: ObserverDF, X: torch.Tensor, ws: torch.Tensor, bs: int):
 
 def teacher_alternatives(state: Dict[str, torch.Tensor], length: int, num_classes: int, X: torch.Tensor, k: int,
                          workspace_mb: int = 256, bs: int = 2048):
-    """(index (N, k) int32, log probability (N, k) fp32) of a trained observer's k best classes for every row of X."""
+    """(index (N, k) int32, log probability (N, k) fp32) of a trained observer's k best classes for every row of X, which is on
+    the GPU that works on it."""
+    if not X.is_cuda:
+        raise ValueError(f"teacher_alternatives: X must be on the GPU, got a {X.device} tensor")
     df = ObserverDF(state, length, num_classes, X.device)
     ws = torch.empty(workspace_mb * (1 << 18), dtype=torch.float32, device=X.device)
     index = torch.empty(X.shape[0], k, dtype=torch.int32, device=X.device)
