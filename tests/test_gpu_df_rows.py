@@ -19,3 +19,24 @@ def test_read_outs_of_rows_on_the_host():
     there = eng.accuracy(X.to(DEV), y.to(DEV), bs=64), eng.evaluate(X.to(DEV), y.to(DEV), 3, bs=64)
     assert (eng.accuracy(X, y, bs=64), eng.evaluate(X, y, 3, bs=64)) == there
     assert (eng.accuracy(X[:, None], y, bs=64), eng.evaluate(X.double(), y.to(DEV), 3, bs=64)) == there
+
+
+def test_read_outs_run_on_their_own_device(monkeypatch):
+    """Launch plans take the current device's stream: the read-outs make theirs the current one, so that the plans' work is ordered
+    with what the tensors' own device does."""
+    from wfd_gan_amd import df_engine
+    entered = []
+
+    class Device(torch.cuda.device):
+        def __init__(self, device):
+            entered.append(torch.device(device))
+            super().__init__(device)
+    torch.manual_seed(3)
+    eng = df_engine.DFTrainEngine(96, 5, 4, O.make_df_state(96, 5), device=DEV)
+    X, y = torch.rand(9, 96, device=DEV), torch.zeros(9, dtype=torch.int64, device=DEV)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for call in (lambda: eng.accuracy(X, y), lambda: eng.evaluate(X, y, 2),
+                 lambda: df_engine.teacher_alternatives(eng.state_dict(), 96, 5, X, 2)):
+        entered.clear()
+        call()
+        assert torch.device(DEV) in entered

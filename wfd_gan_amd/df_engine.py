@@ -77,14 +77,15 @@ def teacher_alternatives(state: Dict[str, torch.Tensor], length: int, num_classe
     the GPU that works on it."""
     if not X.is_cuda:
         raise ValueError(f"teacher_alternatives: X must be on the GPU, got a {X.device} tensor")
-    df = ObserverDF(state, length, num_classes, X.device)
-    ws = torch.empty(workspace_mb * (1 << 18), dtype=torch.float32, device=X.device)
-    index = torch.empty(X.shape[0], k, dtype=torch.int32, device=X.device)
-    value = torch.empty(X.shape[0], k, dtype=torch.float32, device=X.device)
-    for a, logits in observer_logits(df, X, ws, bs):
-        top = heads.label_logprobs(logits, None, k)
-        index[a:a + logits.shape[0]] = top.top_index
-        value[a:a + logits.shape[0]] = top.top_logprob
+    with torch.cuda.device(X.device):          # plans run on the current device's stream, tensors and heads on their own's
+        df = ObserverDF(state, length, num_classes, X.device)
+        ws = torch.empty(workspace_mb * (1 << 18), dtype=torch.float32, device=X.device)
+        index = torch.empty(X.shape[0], k, dtype=torch.int32, device=X.device)
+        value = torch.empty(X.shape[0], k, dtype=torch.float32, device=X.device)
+        for a, logits in observer_logits(df, X, ws, bs):
+            top = heads.label_logprobs(logits, None, k)
+            index[a:a + logits.shape[0]] = top.top_index
+            value[a:a + logits.shape[0]] = top.top_logprob
     return index, value
 
 
@@ -384,15 +385,17 @@ class DFTrainEngine:
     def accuracy(self, X: torch.Tensor, y: torch.Tensor, bs: int = 128) -> float:
         """Eval-mode argmax accuracy (src/train_df.py:134-157) of the current parameters on device-resident
         X (N, L) / y (N,), in batches of ``bs``."""
-        df = ObserverDF(self.state_dict(), self.length, self.C, self.dev)
-        correct = torch.zeros(1, dtype=torch.int32, device=self.dev)
-        st = torch.cuda.current_stream().cuda_stream
         N = X.shape[0]
-        y32 = y.to(self.dev).to(torch.int32).contiguous()
-        for a, logits in observer_logits(df, X, self.buf["ws"], bs):
-            n = logits.shape[0]
-            self.L.argmax_correct(logits.data_ptr(), logits.stride(0), n, self.C, y32[a:a + n].data_ptr(), correct.data_ptr(), st)
-        return int(correct.item()) / max(1, N)
+        with torch.cuda.device(self.dev):      # plans run on the current device's stream, tensors and heads on their own's
+            df = ObserverDF(self.state_dict(), self.length, self.C, self.dev)
+            correct = torch.zeros(1, dtype=torch.int32, device=self.dev)
+            st = torch.cuda.current_stream().cuda_stream
+            y32 = y.to(self.dev).to(torch.int32).contiguous()
+            for a, logits in observer_logits(df, X, self.buf["ws"], bs):
+                n = logits.shape[0]
+                self.L.argmax_correct(logits.data_ptr(), logits.stride(0), n, self.C, y32[a:a + n].data_ptr(), correct.data_ptr(),
+                                      st)
+            return int(correct.item()) / max(1, N)
 
     def evaluate(self, X: torch.Tensor, y: torch.Tensor, k: int = 5, bs: int = 2048) -> Dict[str, float]:
         """Eval-mode quality of the current parameters on device-resident X (N, L) / y (N,): ``top1`` and ``top_k`` accuracy,
@@ -400,14 +403,15 @@ class DFTrainEngine:
         if not 1 <= k <= heads.MAX_ALTERNATIVES:
             raise ValueError(f"evaluate: k must be 1 .. {heads.MAX_ALTERNATIVES}, got {k}")
         k = min(k, self.C)
-        df = ObserverDF(self.state_dict(), self.length, self.C, self.dev)
-        y32 = y.to(self.dev).to(torch.int32).contiguous()
-        sums = torch.zeros(4, dtype=torch.float64, device=self.dev)
-        for a, logits in observer_logits(df, X, self.buf["ws"], bs):
-            lab = y32[a:a + logits.shape[0]]
-            r = heads.label_logprobs(logits, lab, k)
-            hit = r.top_index == lab[:, None]
-            sums += torch.stack([hit[:, 0].sum(), hit.sum(), r.logprob.sum(dtype=torch.float64),
-                                 r.entropy.sum(dtype=torch.float64)]).to(torch.float64)
+        with torch.cuda.device(self.dev):
+            df = ObserverDF(self.state_dict(), self.length, self.C, self.dev)
+            y32 = y.to(self.dev).to(torch.int32).contiguous()
+            sums = torch.zeros(4, dtype=torch.float64, device=self.dev)
+            for a, logits in observer_logits(df, X, self.buf["ws"], bs):
+                lab = y32[a:a + logits.shape[0]]
+                r = heads.label_logprobs(logits, lab, k)
+                hit = r.top_index == lab[:, None]
+                sums += torch.stack([hit[:, 0].sum(), hit.sum(), r.logprob.sum(dtype=torch.float64),
+                                     r.entropy.sum(dtype=torch.float64)]).to(torch.float64)
         top1, topk, lp, ent = (sums / max(1, X.shape[0])).tolist()
         return {"top1": top1, "top_k": topk, "logprob": lp, "entropy": ent}
