@@ -23,3 +23,15 @@ def test_observer_batches_are_on_the_observers_device_wherever_the_rows_are(monk
 def test_teacher_alternatives_refuses_rows_on_the_host():
     with pytest.raises(ValueError, match="must be on the GPU"):
         df_engine.teacher_alternatives({}, 5, 2, torch.zeros(7, 5), 1)
+
+
+def test_read_outs_refuse_fewer_labels_than_rows():
+    """Kernels read a label per row; the engine here is a shell that was never built."""
+    eng = object.__new__(df_engine.DFTrainEngine)
+    eng.dev = torch.device("cpu")
+    X = torch.zeros(7, 5)
+    for shape in ((6,), (0,), (7, 2), (3, 3), ()):
+        with pytest.raises(ValueError, match="accuracy: 7 rows"):
+            eng._labels(X, torch.zeros(shape, dtype=torch.int64), "accuracy")
+    for shape in ((7,), (7, 1), (9,)):
+        assert eng._labels(X, torch.arange(9)[:shape[0]].reshape(shape), "accuracy").tolist()[:7] == list(range(7))

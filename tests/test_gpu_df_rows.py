@@ -40,3 +40,16 @@ def test_read_outs_run_on_their_own_device(monkeypatch):
         entered.clear()
         call()
         assert torch.device(DEV) in entered
+
+
+def test_labels_of_the_read_outs():
+    """A column of labels counts as labels; fewer than there are rows are refused before anything reads them."""
+    from wfd_gan_amd.df_engine import DFTrainEngine
+    torch.manual_seed(3)
+    eng = DFTrainEngine(96, 5, 4, O.make_df_state(96, 5), device=DEV)
+    g = torch.Generator().manual_seed(4)
+    X, y = torch.rand(40, 96, generator=g).to(DEV), torch.randint(0, 5, (40,), generator=g)
+    assert eng.evaluate(X, y[:, None], 2) == eng.evaluate(X, y, 2) and eng.accuracy(X, y[:, None]) == eng.accuracy(X, y)
+    for who in ("accuracy", "evaluate"):
+        with pytest.raises(ValueError, match=f"{who}: 40 rows"):
+            getattr(eng, who)(X, y[:39])

@@ -382,15 +382,21 @@ class DFTrainEngine:
         return float(self.buf["loss"].item())
 
     # ------------------------------------------------------------------------------------------------------
+    def _labels(self, X: torch.Tensor, y: torch.Tensor, who: str) -> torch.Tensor:
+        """One int32 label per row of X (kernels read as many labels as there are rows)."""
+        if y.dim() == 0 or y.shape[0] != y.numel() or y.numel() < X.shape[0]:
+            raise ValueError(f"{who}: {X.shape[0]} rows need a label each, got {tuple(y.shape)}")
+        return y.to(self.dev).to(torch.int32).reshape(-1).contiguous()
+
     def accuracy(self, X: torch.Tensor, y: torch.Tensor, bs: int = 128) -> float:
         """Eval-mode argmax accuracy (src/train_df.py:134-157) of the current parameters on device-resident
         X (N, L) / y (N,), in batches of ``bs``."""
         N = X.shape[0]
         with torch.cuda.device(self.dev):      # plans run on the current device's stream, tensors and heads on their own's
+            y32 = self._labels(X, y, "accuracy")
             df = ObserverDF(self.state_dict(), self.length, self.C, self.dev)
             correct = torch.zeros(1, dtype=torch.int32, device=self.dev)
             st = torch.cuda.current_stream().cuda_stream
-            y32 = y.to(self.dev).to(torch.int32).contiguous()
             for a, logits in observer_logits(df, X, self.buf["ws"], bs):
                 n = logits.shape[0]
                 self.L.argmax_correct(logits.data_ptr(), logits.stride(0), n, self.C, y32[a:a + n].data_ptr(), correct.data_ptr(),
@@ -402,10 +408,10 @@ class DFTrainEngine:
         mean ``logprob`` of the label and mean ``entropy`` of the prediction."""
         if not 1 <= k <= heads.MAX_ALTERNATIVES:
             raise ValueError(f"evaluate: k must be 1 .. {heads.MAX_ALTERNATIVES}, got {k}")
-        k = min(k, self.C)
+        k, N = min(k, self.C), X.shape[0]
         with torch.cuda.device(self.dev):
+            y32 = self._labels(X, y, "evaluate")
             df = ObserverDF(self.state_dict(), self.length, self.C, self.dev)
-            y32 = y.to(self.dev).to(torch.int32).contiguous()
             sums = torch.zeros(4, dtype=torch.float64, device=self.dev)
             for a, logits in observer_logits(df, X, self.buf["ws"], bs):
                 lab = y32[a:a + logits.shape[0]]
@@ -413,5 +419,5 @@ class DFTrainEngine:
                 hit = r.top_index == lab[:, None]
                 sums += torch.stack([hit[:, 0].sum(), hit.sum(), r.logprob.sum(dtype=torch.float64),
                                      r.entropy.sum(dtype=torch.float64)]).to(torch.float64)
-        top1, topk, lp, ent = (sums / max(1, X.shape[0])).tolist()
+        top1, topk, lp, ent = (sums / max(1, N)).tolist()
         return {"top1": top1, "top_k": topk, "logprob": lp, "entropy": ent}
