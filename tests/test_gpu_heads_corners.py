@@ -1,6 +1,6 @@
 """GPU: corners of the classifier-head operators' documented range: rows of one and two columns, masks of the type's
 lowest value at low temperatures, NaN at the first class, rows whose only entry of the teacher is wrong, rows
-without a term."""
+without a term, results passed in again for a call that writes less."""
 import pytest
 import torch
 
@@ -182,3 +182,30 @@ def test_scores_rows_without_a_label_have_gradient_zero_whatever_they_hold(v, t)
     assert float(d[:3].abs().max()) == 0 and bool(d[3].isnan().all()) and bool(d[4].isfinite().all()) and float(d[4].abs().max()) > 0
     d = heads.label_logprobs_backward(x.to(DEV), y, r, one, one)
     assert d.isnan().all(1).tolist() == [True, True, False, True, False]
+
+
+# ---- a result passed in again for a call that writes less ---------------------------------------------------------------------
+def test_a_result_passed_in_again_holds_what_the_call_wrote():
+    """What a call does not write is None in what it returns, not the numbers of the call before; the tensors that it does write are
+    those passed in."""
+    from wfd_gan_amd import heads
+    x = torch.randn(4, 300, generator=gen(1)).to(DEV)
+    z = torch.randn(4, 300, generator=gen(2)).to(DEV)
+    y = torch.tensor([3, 1, -1, 299], dtype=torch.int32, device=DEV)
+    full = heads.layer_norm(x)
+    bare = heads.layer_norm(z, stats=False, out=full)
+    assert bare.y is full.y and bare.mean is None and bare.rstd is None
+    full = heads.label_logprobs(x, y, 5)
+    r = heads.label_logprobs(z, y, 0, out=full)
+    assert r.top_logprob is None and r.top_index is None and r.logprob is full.logprob and r.entropy is full.entropy
+    r = heads.label_logprobs(z, None, 5, out=full)
+    assert r.logprob is None and r.top_index is full.top_index and r.stat is full.stat
+    ti, tv = torch.zeros(4, 1, dtype=torch.int32, device=DEV), torch.zeros(4, 1, device=DEV)
+    full = heads.distill_loss(x, ti, tv)
+    alone = heads.distill_loss(z, ti, tv, grad=False, out=full)
+    assert alone.loss is full.loss and alone.dlogits is None
+    # nothing left out: the very result
+    for again, out in ((heads.layer_norm(z, out=(o := heads.norm_output_like(z))), o),
+                       (heads.label_logprobs(z, y, 5, out=(o := heads.scores_like(z, 5))), o),
+                       (heads.distill_loss(z, ti, tv, out=(o := heads.distill_output_like(z))), o)):
+        assert again is out

@@ -7,8 +7,9 @@ read where they are, anything else is copied first.  As everywhere in this packa
 form (no autograd graph), there is no CPU path, and a call only enqueues work on the current stream of the tensors' device.
 
 Results go into fresh tensors, or into those of an earlier call's result passed as ``out=`` (same sizes): then a call allocates
-nothing, which is what a loop or a captured graph wants.  Such a result belongs to one call in flight: give calls that may
-overlap (other streams, graphs that replay side by side) results of their own.
+nothing, which is what a loop or a captured graph wants.  What such a call does not write (no ``stats``, no labels, ``k`` = 0, no
+``grad``) is None in what it returns.  A result belongs to one call in flight: give calls that may overlap (other streams, graphs
+that replay side by side) results of their own.
 """
 from __future__ import annotations
 
@@ -187,7 +188,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     mean = _result(out.mean, who, "mean", m, torch.float32, dev) if stats else 0
     rstd = _result(out.rstd, who, "rstd", m, torch.float32, dev) if stats else 0
     _launch(dev, lib().layer_norm_fwd, xr.data_ptr(), ld, code, _ptr(w), _ptr(b), _CODES[wd], m, n, eps, y, n, mean, rstd)
-    return out
+    return out if stats or out.mean is out.rstd is None else out._replace(mean=None, rstd=None)
 
 
 def norm_gradients_like(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -250,8 +251,8 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int 
     """Log probability of each row's label under softmax(logits / temperature), the entropy of that distribution and its ``k``
     largest classes in order (equal logits: the lower index first), all in one pass over the logits.
 
-    ``labels``: int32, one per row; negative = no label (log probability 0), >= classes = NaN; None: ``logprob`` is left
-    unwritten.  A row of nothing but -inf has log probabilities -inf and entropy 0; one with NaN or +inf is NaN."""
+    ``labels``: int32, one per row; negative = no label (log probability 0), >= classes = NaN; None: no ``logprob``.
+    A row of nothing but -inf has log probabilities -inf and entropy 0; one with NaN or +inf is NaN."""
     who = "label_logprobs"
     code = _code(logits, "logits")
     xr, m, v, ld = _rows(logits, "logits")
@@ -263,8 +264,6 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int 
     dev = _device(logits, who, y)
     if out is None:
         out = scores_like(logits, k)
-        if y is None:
-            out = out._replace(logprob=None)
     f32 = torch.float32
     lp = 0 if y is None else _result(out.logprob, who, "logprob", m, f32, dev)
     ent = 0 if out.entropy is None else _result(out.entropy, who, "entropy", m, f32, dev)
@@ -273,6 +272,10 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int 
     idx = _result(out.top_index, who, "top_index", m * k, torch.int32, dev) if k else 0
     work = _scratch(out.work, who, _floats("label_scores_floats", m, v, code, k), dev)
     _launch(dev, lib().label_scores, xr.data_ptr(), ld, code, m, v, _ptr(y), temperature, k, lp, ent, stat, top, idx, work)
+    if y is None and out.logprob is not None:
+        out = out._replace(logprob=None)
+    if k == 0 and (out.top_logprob is not None or out.top_index is not None):
+        out = out._replace(top_logprob=None, top_index=None)
     return out
 
 
@@ -360,4 +363,4 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_valu
     work = _scratch(out.work, who, _floats("distill_floats", m, v, code), dev)
     _launch(dev, lib().distill, xr.data_ptr(), ld, code, m, v, _ptr(ti) if k else 0, _ptr(tv) if k else 0, k, k, _ptr(y),
             temperature, weight, label_weight, _ptr(rs), grad_scale, loss, dx, v, work)
-    return out
+    return out if grad or out.dlogits is None else out._replace(dlogits=None)
