@@ -53,3 +53,33 @@ def test_labels_of_the_read_outs():
     for who in ("accuracy", "evaluate"):
         with pytest.raises(ValueError, match=f"{who}: 40 rows"):
             getattr(eng, who)(X, y[:39])
+
+
+def test_a_step_that_learns_from_a_teacher_needs_the_batchs_entries():
+    """Without them it would train on the labels' share of the loss alone, or on the entries of the batch before, without a word."""
+    from wfd_gan_amd.df_engine import DFTrainEngine, Distill
+    torch.manual_seed(3)
+    state = O.make_df_state(96, 5)
+    eng = DFTrainEngine(96, 5, 4, state, device=DEV, distill=Distill(3))
+    g = torch.Generator().manual_seed(4)
+    x, y = torch.rand(4, 96, generator=g), torch.randint(0, 5, (4,), generator=g)
+    ti, tv = torch.tensor([[0, 1, 2]] * 4, dtype=torch.int32), torch.randn(4, 3, generator=g)
+    eng.draw_masks()
+    with pytest.raises(RuntimeError, match="set_teacher was not called"):
+        eng.train_step()
+    for _ in range(2):
+        eng.set_batch(x, y)
+        with pytest.raises(RuntimeError, match="set_teacher was not called"):
+            eng.train_step()
+        eng.set_teacher(ti, tv)
+        for _ in range(2):                                # several steps on one batch
+            eng.train_step()
+    eng.set_teacher(ti, tv)                               # the other way round
+    eng.set_batch(x, y)
+    eng.train_step()
+    assert int(eng.step.item()) == 5
+    eng.forward_train()                                   # the forward pass alone needs no teacher
+    plain = DFTrainEngine(96, 5, 4, state, device=DEV, distill=Distill(3, 2.0, 0.0))
+    plain.set_batch(x, y)
+    plain.draw_masks()
+    plain.train_step()                                    # nor does a share of 0

@@ -157,6 +157,7 @@ class DFTrainEngine:
             b["t_index"] = torch.full((B, distill.k), -1, dtype=torch.int32, device=dev)
             b["t_value"] = z(B, distill.k)
             b["t_work"] = z(max(1, self.L.distill_floats(B, C, 0)))
+        self.new_batch, self.new_teacher = True, False                   # since the last step (train_step)
         b["WT"] = [None] + [z(DF_CONVS[k][2], 8 * DF_CONVS[k][3]) for k in range(1, 7)]
         self.rpc = max(64, (B * Ls[0] + 1023) // 1024)                   # rows per chunk of the tall reductions
         nchunk = (B * Ls[0] + self.rpc - 1) // self.rpc
@@ -332,9 +333,11 @@ class DFTrainEngine:
         """x (B, L) or (B, 1, L) scaled features without the burst-count column; y (B,) labels."""
         self.buf["X"].copy_(x.reshape(self.B, self.length).to(self.dev, torch.float32))
         self.buf["labels"].copy_(y.to(self.dev).to(torch.int32))
+        self.new_batch = True
 
     def set_teacher(self, index: torch.Tensor, value: torch.Tensor):
-        """The batch's rows of ``teacher_alternatives``: index (B, k), value (B, k)."""
+        """The batch's rows of ``teacher_alternatives``: index (B, k), value (B, k); an index of -1 is no entry.  Before or after
+        ``set_batch``; every new batch needs its own."""
         if self.distill is None:
             raise RuntimeError("set_teacher: the engine was built without distill")
         if index.shape != self.buf["t_index"].shape or value.shape != index.shape:
@@ -342,6 +345,7 @@ class DFTrainEngine:
                              f"{tuple(self.buf['t_index'].shape)} each")
         self.buf["t_index"].copy_(index)
         self.buf["t_value"].copy_(value)
+        self.new_teacher = True
 
     def set_masks(self, masks: Sequence[torch.Tensor]):
         """Explicit dropout keep-masks in the reference's layouts ((B, C, L) x4, (B, 512) x2), values {0, 1/(1-p)}."""
@@ -369,6 +373,9 @@ class DFTrainEngine:
         return self.buf["LOG"][:, : self.C]
 
     def train_step(self):
+        if self.distill is not None and self.distill.weight > 0 and self.new_batch and not self.new_teacher:
+            raise RuntimeError("train_step: the engine learns from a teacher, and set_teacher was not called for this batch")
+        self.new_batch = self.new_teacher = False
         self.plan.run()
         self._count_batch()
 
