@@ -1,6 +1,7 @@
 """GPU: corners of the classifier-head operators' documented range: rows of one and two columns, masks of the type's
 lowest value at low temperatures, NaN at the first class, rows whose only entry of the teacher is wrong, rows
-without a term, results passed in again for a call that writes less."""
+without a term, results passed in again for a call that writes less, gradients
+that are not wanted."""
 import pytest
 import torch
 
@@ -209,3 +210,30 @@ def test_a_result_passed_in_again_holds_what_the_call_wrote():
                        (heads.label_logprobs(z, y, 5, out=(o := heads.scores_like(z, 5))), o),
                        (heads.distill_loss(z, ti, tv, out=(o := heads.distill_output_like(z))), o)):
         assert again is out
+
+
+# ---- gradients that are not wanted ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n", [16385, 40001])
+def test_norm_backward_of_long_rows_without_some_of_the_weights_gradients(n, t):
+    """dx alone needs no walk down the columns: the partial sums stay as they were.  One of the two gradients alone, and dx, have the
+    bits of the full call; in place as well."""
+    from wfd_gan_amd import heads
+    g = gen(n)
+    x, dy = (torch.randn(5, n, generator=g).to(t).to(DEV) for _ in range(2))
+    w = torch.randn(n, generator=g).to(DEV)
+    r = heads.layer_norm(x, w, w)
+    full = heads.layer_norm_backward(dy, x, w, r.mean, r.rstd)
+    for dw, db in ((None, None), (full.dweight, None), (None, full.dbias)):
+        work = torch.full_like(full.work, 77.0)
+        o = heads.NormGradients(torch.empty_like(x), None if dw is None else torch.empty_like(dw),
+                                None if db is None else torch.empty_like(db), work)
+        got = heads.layer_norm_backward(dy, x, w, r.mean, r.rstd, out=o)
+        assert torch.equal(got.dx, full.dx)
+        assert all(a is None if b is None else torch.equal(a, b) for a, b in ((got.dweight, dw), (got.dbias, db)))
+        if dw is None and db is None:
+            assert bool((work == 77.0).all())
+    for where in (dy.clone(), x.clone()):
+        args = (where, x) if torch.equal(where, dy) else (dy, where)
+        o = heads.NormGradients(where, None, None, full.work)
+        assert torch.equal(heads.layer_norm_backward(*args, w, r.mean, r.rstd, out=o).dx, full.dx)

@@ -660,7 +660,7 @@ template <class T, class WT> int ln_bwd(LnBwd g, WT* dw, WT* db, hipStream_t st)
         default:
             if (!launchable(g.M, 1024)) return WFD_ERR_ARG;
             // the columns first: dx may lie over dy or x
-            hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3(cdiv(g.N, 256), s.blocks), dim3(256), 0, st, g);
+            if (dw || db) hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3(cdiv(g.N, 256), s.blocks), dim3(256), 0, st, g);
             hipLaunchKernelGGL((ln_bwd_long_kernel<T, WT>), dim3(g.M), dim3(1024), 0, st, g);
     }
     WFD_CHECK_LAUNCH();
