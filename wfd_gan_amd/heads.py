@@ -64,15 +64,30 @@ def _code(t: torch.Tensor, name: str) -> int:
     return c
 
 
+def _no_rows(t: torch.Tensor, name: str):
+    if not t.shape or t.shape[-1] == 0:
+        raise ValueError(f"{name}: needs a last dimension of at least one element, got shape {tuple(t.shape)}")
+    raise ValueError(f"{name}: {t.numel() // t.shape[-1]} rows of {t.shape[-1]} are more than 2^31 - 1")
+
+
+def _sizes(t: torch.Tensor, name: str):
+    """(rows, columns) of rows whose buffers are asked for, checked as _rows does"""
+    n = t.shape[-1] if t.shape else 0
+    m = t.numel() // n if n else 0
+    if n == 0 or m >= _INT32 or n >= _INT32:
+        _no_rows(t, name)
+    return m, n
+
+
 def _rows(t: torch.Tensor, name: str):
     """(tensor whose storage is read, rows, columns, row stride)"""
     shape = t.shape
     if not shape or shape[-1] == 0:
-        raise ValueError(f"{name}: needs a last dimension of at least one element, got shape {tuple(shape)}")
+        _no_rows(t, name)
     n = shape[-1]
     m = t.numel() // n
     if m >= _INT32 or n >= _INT32:
-        raise ValueError(f"{name}: {m} rows of {n} are more than 2^31 - 1")
+        _no_rows(t, name)
     if t.is_contiguous():
         return t, m, n, n
     if len(shape) == 2 and (t.stride(1) == 1 or n == 1) and n <= t.stride(0) < _INT32:
@@ -164,8 +179,10 @@ def _norm_weights(who, code, n, weight, bias):
 
 def norm_output_like(x: torch.Tensor, stats: bool = True) -> NormOutput:
     """Buffers for ``layer_norm(x, ..., out=...)``."""
-    f = dict(dtype=torch.float32, device=x.device)
+    _code(x, "x")
+    _sizes(x, "x")
     lead = x.shape[:-1]
+    f = dict(dtype=torch.float32, device=x.device)
     return NormOutput(torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(lead, **f) if stats else None,
                       torch.empty(lead, **f) if stats else None)
 
@@ -194,8 +211,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 def norm_gradients_like(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                         bias: Optional[torch.Tensor] = None) -> NormGradients:
     """Buffers for ``layer_norm_backward(..., out=...)``; without a weight (bias) there is no dweight (dbias)."""
-    n = x.shape[-1]
-    floats = _floats("layer_norm_bwd_floats", x.numel() // n, n, _code(x, "x"))
+    code = _code(x, "x")
+    m, n = _sizes(x, "x")
+    floats = _floats("layer_norm_bwd_floats", m, n, code)
     if floats < 0:
         raise ValueError(f"layer_norm_backward: rows of {n} are not supported")
     grad = lambda w: None if w is None else torch.empty(n, dtype=w.dtype, device=x.device)
@@ -234,8 +252,9 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
 # ---- scores of given labels ------------------------------------------------------------------------------------------
 def scores_like(logits: torch.Tensor, k: int = 0) -> LabelScores:
     """Buffers for ``label_logprobs(logits, ..., k, out=...)``."""
-    v = logits.shape[-1]
-    floats = _floats("label_scores_floats", logits.numel() // v, v, _code(logits, "logits"), k)
+    code = _code(logits, "logits")
+    m, v = _sizes(logits, "logits")
+    floats = _floats("label_scores_floats", m, v, code, k) if 0 <= k <= MAX_ALTERNATIVES else -1
     if floats < 0:
         raise ValueError(f"label_logprobs: {k} alternatives of {v} classes are not supported (at most {MAX_ALTERNATIVES})")
     lead, dev = logits.shape[:-1], logits.device
@@ -309,8 +328,9 @@ def label_logprobs_backward(logits: torch.Tensor, labels: Optional[torch.Tensor]
 # ---- distillation ------------------------------------------------------------------------------------------------------
 def distill_output_like(logits: torch.Tensor, grad: bool = True) -> DistillOutput:
     """Buffers for ``distill_loss(logits, ..., out=...)``."""
-    v = logits.shape[-1]
-    floats = _floats("distill_floats", logits.numel() // v, v, _code(logits, "logits"))
+    code = _code(logits, "logits")
+    m, v = _sizes(logits, "logits")
+    floats = _floats("distill_floats", m, v, code)
     if floats < 0:
         raise ValueError(f"distill_loss: {v} classes are not supported")
     f = dict(dtype=torch.float32, device=logits.device)
