@@ -117,6 +117,22 @@ def _vector(t, who: str, name: str, numel: int, dtype) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _wide(shape) -> list:
+    return [n for n in shape if n != 1]
+
+
+def _in_order(rows: torch.Tensor, who: str, **operands):
+    """Rows with several leading dimensions: a per-row operand (``name_2``: of two elements each) has the same ones, or a single
+    one, dimensions of 1 aside; any other shape of as many elements would be read in another order than it is meant."""
+    lead = rows.shape[:-1]
+    for name, t in operands.items():
+        if t is None or t.dim() < 2:
+            continue
+        last = (2,) if name.endswith("_2") else ()
+        if _wide(t.shape) not in (_wide((*lead, *last)), _wide((lead.numel(), *last))):
+            raise ValueError(f"{who}: {name[:-2] if last else name} has shape {tuple(t.shape)}, the rows' is {tuple(lead)}")
+
+
 def _result(t, who: str, name: str, numel: int, dtype, dev: int) -> int:
     """The address of one tensor of an earlier result that is written again."""
     if t is None or t.dtype != dtype or t.numel() != numel or t.get_device() != dev or not t.is_contiguous():
@@ -236,6 +252,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     if mean is None or rstd is None:
         raise ValueError(f"{who}: needs the mean and rstd that layer_norm returned")
     mean, rstd = _vector(mean, who, "mean", m, torch.float32), _vector(rstd, who, "rstd", m, torch.float32)
+    if x.dim() > 2:
+        _in_order(x, who, mean=mean, rstd=rstd)
     dev = _device(x, who, dyr, w, mean, rstd)
     if out is None:
         like = torch.empty(0, dtype=wd, device=x.device)
@@ -279,6 +297,8 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int 
     if not 0 <= k <= min(v, MAX_ALTERNATIVES):
         raise ValueError(f"{who}: k must be 0 .. {min(v, MAX_ALTERNATIVES)}, got {k}")
     y = _vector(labels, who, "labels", m, torch.int32)
+    if logits.dim() > 2:
+        _in_order(logits, who, labels=y)
     temperature = _temperature(temperature, who)
     dev = _device(logits, who, y)
     if out is None:
@@ -315,6 +335,8 @@ def label_logprobs_backward(logits: torch.Tensor, labels: Optional[torch.Tensor]
     stat = _vector(scores.stat, who, "scores.stat", 2 * m, torch.float32)
     ent = _vector(scores.entropy, who, "scores.entropy", m, torch.float32) if d_entropy is not None else None
     dl, dh = _vector(d_logprob, who, "d_logprob", m, torch.float32), _vector(d_entropy, who, "d_entropy", m, torch.float32)
+    if logits.dim() > 2:
+        _in_order(logits, who, labels=y, stat_2=stat, entropy=ent, d_logprob=dl, d_entropy=dh)
     temperature = _temperature(temperature, who)
     dev = _device(logits, who, y, stat, ent, dl, dh)
     if out is None:
@@ -374,6 +396,8 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_valu
     if label_weight != 0.0 and y is None:
         raise ValueError(f"{who}: label_weight needs labels")
     rs = _vector(row_scale, who, "row_scale", m, torch.float32)
+    if logits.dim() > 2:
+        _in_order(logits, who, labels=y, row_scale=rs)
     temperature = _temperature(temperature, who)
     dev = _device(logits, who, ti, tv, y, rs)
     if out is None:
