@@ -35,3 +35,9 @@ def test_read_outs_refuse_fewer_labels_than_rows():
             eng._labels(X, torch.zeros(shape, dtype=torch.int64), "accuracy")
     for shape in ((7,), (7, 1), (9,)):
         assert eng._labels(X, torch.arange(9)[:shape[0]].reshape(shape), "accuracy").tolist()[:7] == list(range(7))
+
+
+@pytest.mark.parametrize("k", [0, -1, 6, 65])
+def test_teacher_alternatives_refuses_a_k_that_an_engine_does_not_take(k):
+    with pytest.raises(ValueError, match="k must be 1 .. 5"):
+        df_engine.teacher_alternatives({}, 5, 5, torch.zeros(7, 5), k)

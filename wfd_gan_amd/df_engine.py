@@ -75,6 +75,8 @@ def teacher_alternatives(state: Dict[str, torch.Tensor], length: int, num_classe
                          workspace_mb: int = 256, bs: int = 2048):
     """(index (N, k) int32, log probability (N, k) fp32) of a trained observer's k best classes for every row of X, which is on
     the GPU that works on it."""
+    if not 1 <= k <= min(num_classes, heads.MAX_ALTERNATIVES):
+        raise ValueError(f"teacher_alternatives: k must be 1 .. {min(num_classes, heads.MAX_ALTERNATIVES)}, got {k}")
     if not X.is_cuda:
         raise ValueError(f"teacher_alternatives: X must be on the GPU, got a {X.device} tensor")
     with torch.cuda.device(X.device):          # plans run on the current device's stream, tensors and heads on their own's
