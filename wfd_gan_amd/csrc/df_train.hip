@@ -54,7 +54,9 @@ __global__ void bn_tall_partial_kernel(const float* __restrict__ Z, int ldz, int
 // variance, as nn.BatchNorm1d does in training mode.
 constexpr int CG = 16;
 // The roundings are spelled out (contraction off; `fused`: one rounding for the product and its sum), so that the result does
-// not hang on what the compiler fuses: these are the bits that checkpoints trained with earlier builds were made with.
+// not hang on what the compiler fuses: these are the bits that checkpoints trained with earlier builds were made with.  Those builds
+// left the choice to the compiler, which fused all folds of a group's chunks and, of the 15 folds of groups behind them, only the
+// 4th and the 10th: the two indices below mean nothing else.
 __device__ __forceinline__ void chan_fold(float& mu, float& m2, float& cnt, float mb, float qb, float cb, bool fused) {
 #pragma clang fp contract(off)
     if (cb <= 0.f) return;
