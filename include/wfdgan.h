@@ -533,6 +533,7 @@ int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, c
  * q = softmax(t_value / T) over the entries of a row of t_index / t_value [M][ldt] whose index is >= 0, p = softmax(x / T),
  * p1 = softmax(x) (weight 0: the entries are not looked at):
  *   loss[m] = weight * T^2 * sum_j q_j (ln q_j - ln p(index_j)) - label_weight * ln p1(labels[m])
+ * (logarithms of fp32 sums: the first term is good to about 1e-7 * weight * T^2, which is all of it at temperatures in the thousands)
  * and, when dlogits is not NULL, its gradient times grad_scale * row_scale[m] (row_scale NULL: 1) in the same call.  An index
  * that occurs twice counts twice.  No entry: the first term is 0; a label < 0: the second is 0 (labels may be NULL when
  * label_weight is 0); a row without either (padding) has gradient 0 whatever its logits hold.  An index or a label >= V is a

@@ -10,7 +10,8 @@
 // team (up to 1024 threads x 16 pieces: 131072 16-bit or 65536 fp32 classes), so that maximum, sum and gradient cost one read.  A few
 // long rows are split over workgroups instead: partial sums in a first launch, loss and gradient in a second.
 // Measured (a large copy reaches 5.47 TB/s): 2048 x 128000 bf16 with gradient 210 us = 5.0 TB/s, loss alone 97 us = 5.4 TB/s; 4096 x
-// 32000 bf16 105 us = 5.0 TB/s, loss alone 47 us = 5.6 TB/s; 128 x 100 fp32 5.2 us.
+// 32000 bf16 105 us = 5.0 TB/s, loss alone 47 us = 5.6 TB/s; 128 x 100 fp32 5.5 us.  Split rows, read twice: 500 x 200000 bf16 with gradient
+// 128 us = 3.1 TB/s, 390 x 128000 fp32 123.
 #include "rowops.h"
 
 namespace {

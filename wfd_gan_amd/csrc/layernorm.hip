@@ -5,7 +5,8 @@
 // Bound by memory: forward reads and writes a row once, backward reads two and writes one.  A row is held packed in the registers
 // of its team (16 / 64 / 256 / 1024 threads), so the variance is the two-pass one about the true mean and costs no second read.
 // Measured (a large copy reaches 5.47 TB/s): forward 4096 x 2048 fp32 11.6 us = 5.8 TB/s, 8191 x 1401 bf16 10.5 us = 4.4 TB/s;
-// backward 16384 x 4096 bf16 78.5 us = 5.1 TB/s, 5.1 of them the second launch; one row of 2048 2.2 us.
+// backward 16384 x 4096 bf16 79 us = 5.1 TB/s, 5.2 of them the second launch; one row of 2048 2.1 us.  Rows beyond the registers: 2048 x
+// 32768 bf16 forward 60 us = 4.5 TB/s, backward 185 = 2.2 TB/s (dx alone 105), 512 x 40001 30, 65 and 35.
 #include "rowops.h"
 
 namespace {
@@ -561,7 +562,9 @@ __global__ __launch_bounds__(1024) void ln_bwd_reduce_kernel(const float* part, 
 
 // The team of a row: the smallest whose registers hold it, from what was measured at 200 MB of rows (us; a large copy takes 37):
 // 16-bit 1401 wide in 64 x 3 pieces 45.7 (64 x 4: 59.8, 256 x 1: 69.6), 2048 in 256 x 1 40.7 (64 x 4: 51.4), 8192 in 1024 x 1 43.1
-// (256 x 4: 54.7); fp32 4096 in 256 x 4 39.6 (1024 x 1: 50.7).  Workgroups: enough for 16 waves on each of 256 CUs, 32 where the
+// (256 x 4: 54.7); fp32 4096 in 256 x 4 39.6 (1024 x 1: 50.7).  Above 8192 (4096) columns a whole CU of threads is the only form that holds
+// a row, half of its places empty at 9000; beside it stands the long form (twice as many rows, us, registers / long form: 9000 bf16 104 /
+// 123, 12288 86 / 109, 16384 81 / 108; fp32 5000 77 / 101, 8192 77 / 88, 16384 79 / 106).  Workgroups: enough for 16 waves on each of 256 CUs, 32 where the
 // team is small and holds little; fp32 rows of a wave or less hold so few weights that a team per row is faster (25000 x 1000 36.7, in
 // 1024 workgroups 39.8; 32768 x 300 14.2, 16.1; bf16 1401 wide 44.9, 40.5).
 template <class T, class WT> int ln_fwd(const LnFwd& g, hipStream_t st) {
@@ -596,10 +599,14 @@ struct LnBwdShape {
 // bytes of partial sums each, written and read.  Measured at 200 MB of rows (us): 32768 x 1024 bf16 with 256 workgroups of 8 teams
 // 43.0 (384: 52.4, 512: 47.2), 24000 x 2048 with 1024 of one team 64.2 (768: 68.0, 512: 83.6), 12000 x 4096 with 512 62.1 (768: 67.0,
 // 256: 84.0), 6103 x 8192 with 256 71.5 (512: 78.2).  1401 wide: 64 x 3 pieces 66.0 (256 x 1: 92.7); 5000: 256 x 3 67.2 (1024 x 1:
-// 84.9).
+// 84.9).  1024 x 2 (16-bit) and 1024 x 4 (fp32) pieces spill 4 to 16 of their 128 registers; the long form, which reads everything
+// twice, is beside them still far behind (twice as many rows, us: 9000 bf16 141 / 328, 12288 130 / 283, 16384 130 / 258; fp32 16384 133 / 225).
 // Few rows: a second launch costs more than a second reading.  us in one launch / two: 1024 rows x 100 bf16 9.8 / 12.9, x 1024 10.3 /
 // 12.4, x 1401 13.8 / 12.8, x 4096 13.4 / 15.1, x 16384 28.4 / 40.6; 1536 x 1024 15.6 / 12.5; fp32 1024 x 2048 11.7 / 12.6, x 6000
-// 22.9 / 19.6, 512 x 6000 13.6 / 13.9, x 16384 28.5 / 39.2; 512 x 3 bf16 (no whole piece) 13.7 / 13.4.
+// 22.9 / 19.6, 512 x 6000 13.6 / 13.9, x 16384 28.5 / 39.2; 512 x 3 bf16 (no whole piece) 13.7 / 13.4.  Those are calls from the host;
+// replayed from a graph, where a second launch costs less, the border lies lower for narrow rows: 1024 rows x 100 bf16 8.1 / 6.4, x 512 8.3 /
+// 6.6, x 1024 8.3 / 7.9, x 1401 10.5 / 10.4, x 2048 9.0 / 16.0, x 4096 11.5 / 17.4; fp32 x 100 7.9 / 6.0, x 1000 9.0 / 11.8, x 2048 9.9 / 12.1.  One
+// border for all widths of a type loses up to 2 us there and 1 us at 1401 from the host.
 LnBwdShape ln_bwd_shape(int M, int N, int E) {
     const int forms[][2] = {{16, 1}, {64, 1}, {64, 2}, {64, 3}, {256, 1}, {256, 2}, {256, 3}, {1024, 1}, {1024, 2}, {1024, 4}};
     for (auto& f : forms)

@@ -6,8 +6,9 @@
 // Bound by memory: the forward reads a row once and writes a few words, the gradient reads and writes it once.  So one walk does all:
 // running maximum and sums, one exponential and four other operations per class, and for the alternatives no more than one maximum per
 // 4 pieces; the few groups that can hold an alternative are read again from the caches.
-// Measured (a large copy reaches 5.47 TB/s): 4096 x 50257 bf16 82 us = 5.0 TB/s without alternatives, 89 with 10, 109 with 64; the
-// gradient of 4096 x 32000 bf16 94 us = 5.6 TB/s; one row of 131072 with 20 alternatives 7.0 us and 4.4 for the join.
+// Measured (a large copy reaches 5.47 TB/s): 4096 x 50257 bf16, three buffers in turn, 84 us = 4.9 TB/s without alternatives, 95 with 10,
+// 115 with 64 (one buffer again and again, part of which stays in the last-level cache: 88 with 10); the gradient of 4096 x 32000 bf16
+// 94 us = 5.6 TB/s; one row of 131072 with 20 alternatives 7.2 us and 4.3 for the join.
 // A row that holds nothing but -inf: logprob -inf, entropy 0, gradient 0.  NaN and +inf make the row's numbers NaN.
 #include "rowops.h"
 
