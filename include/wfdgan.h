@@ -535,10 +535,11 @@ int wfd_label_scores_bwd(const void* logits, int ldl, int dtype, int M, int V, c
  *   loss[m] = weight * T^2 * sum_j q_j (ln q_j - ln p(index_j)) - label_weight * ln p1(labels[m])
  * (logarithms of fp32 sums: the first term is good to about 1e-7 * weight * T^2, which is all of it at temperatures in the thousands)
  * and, when dlogits is not NULL, its gradient times grad_scale * row_scale[m] (row_scale NULL: 1) in the same call.  An index
- * that occurs twice counts twice.  No entry: the first term is 0; a label < 0: the second is 0 (labels may be NULL when
- * label_weight is 0); a row without either (padding) has gradient 0 whatever its logits hold.  An index or a label >= V is a
- * mistake: the row's loss and gradient are NaN.  A row of nothing but -inf: loss +inf where a term is left, gradient 0.  A row with
- * a term and NaN or +inf: NaN (row_scale is a factor: 0 leaves the NaN).  dlogits may be logits. */
+ * that occurs twice counts twice; an entry less than 2^-126 times as likely as the best one may count as 0, also where the student
+ * has -inf.  No entry: the first term is 0; a label < 0: the second is 0 (labels may be NULL when label_weight is 0); a row without
+ * either (padding) has gradient 0 whatever its logits hold.  An index or a label >= V is a mistake: the row's loss and gradient
+ * are NaN.  A row of nothing but -inf: loss +inf where a term is left, gradient 0.  A row with a term and NaN or +inf: NaN (row_scale
+ * is a factor: 0 leaves the NaN).  dlogits may be logits. */
 int wfd_distill(const void* logits, int ldl, int dtype, int M, int V, const int* t_index, const float* t_value, int ldt, int K,
                 const int* labels, float temperature, float weight, float label_weight, const float* row_scale,
                 float grad_scale, float* loss, void* dlogits, int lddl, float* work, void* stream);

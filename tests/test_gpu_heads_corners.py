@@ -1,7 +1,7 @@
 """GPU: corners of the classifier-head operators' documented range: rows of one and two columns, masks of the type's
 lowest value at low temperatures, NaN at the first class, rows whose only entry of the teacher is wrong, rows
 without a term, results passed in again for a call that writes less, gradients
-that are not wanted."""
+that are not wanted, shares of a masked class."""
 import itertools
 
 import numpy as np
@@ -247,3 +247,23 @@ def test_norm_backward_of_long_rows_without_some_of_the_weights_gradients(n, t):
         args = (where, x) if torch.equal(where, dy) else (dy, where)
         o = heads.NormGradients(where, None, None, full.work)
         assert torch.equal(heads.layer_norm_backward(*args, w, r.mean, r.rstd, out=o).dx, full.dx)
+
+
+# ---- a teacher's share of a class that the student has masked -----------------------------------------------------------------
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("v", [9, 1401, 140001])
+def test_a_teachers_share_of_a_masked_class(v, t):
+    """Any share within fp32's range makes the loss infinite; one beyond it (e^-200) is none, and the rest of the row keeps its
+    digits."""
+    from wfd_gan_amd import heads
+    x = torch.randn(3, v, generator=gen(v)).to(t)
+    x[:, 1] = -INF
+    ti = torch.tensor([[0, 1, 2]] * 3, dtype=torch.int32)
+    tv = torch.tensor([[0.5, -60.0, 0.2], [0.5, -200.0, 0.2], [0.5, -INF, 0.2]])
+    r = heads.distill_loss(x.to(DEV), ti.to(DEV), tv.to(DEV))
+    assert float(r.loss[0]) == INF and float(r.loss[1]) != INF
+    one = torch.ones(2)
+    loss, bl, d, bd = R.distill(x[1:], torch.tensor([[0, -1, 2]] * 2), tv[1:], None, 1.0, 1.0, 0.0, one)
+    R.check(r.loss[1:], loss, bl, F32, "loss")
+    R.check(r.dlogits[1:], d, bd, t, "dlogits")
+    assert bool(r.dlogits[0].isfinite().all())
