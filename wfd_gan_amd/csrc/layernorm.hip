@@ -564,9 +564,9 @@ __global__ __launch_bounds__(1024) void ln_bwd_reduce_kernel(const float* part, 
 // 16-bit 1401 wide in 64 x 3 pieces 45.7 (64 x 4: 59.8, 256 x 1: 69.6), 2048 in 256 x 1 40.7 (64 x 4: 51.4), 8192 in 1024 x 1 43.1
 // (256 x 4: 54.7); fp32 4096 in 256 x 4 39.6 (1024 x 1: 50.7).  Above 8192 (4096) columns a whole CU of threads is the only form that holds
 // a row, half of its places empty at 9000; beside it stands the long form (twice as many rows, us, registers / long form: 9000 bf16 104 /
-// 123, 12288 86 / 109, 16384 81 / 108; fp32 5000 77 / 101, 8192 77 / 88, 16384 79 / 106).  Workgroups: enough for 16 waves on each of 256 CUs, 32 where the
-// team is small and holds little; fp32 rows of a wave or less hold so few weights that a team per row is faster (25000 x 1000 36.7, in
-// 1024 workgroups 39.8; 32768 x 300 14.2, 16.1; bf16 1401 wide 44.9, 40.5).
+// 123, 12288 86 / 109, 16384 81 / 108; fp32 5000 77 / 101, 8192 77 / 88, 16384 79 / 106).  Workgroups: enough for 16 waves on each of
+// 256 CUs, 32 where the team is small and holds little; fp32 rows of a wave or less hold so few weights that a team per row is faster
+// (25000 x 1000 36.7, in 1024 workgroups 39.8; 32768 x 300 14.2, 16.1; bf16 1401 wide 44.9, 40.5).
 template <class T, class WT> int ln_fwd(const LnFwd& g, hipStream_t st) {
     constexpr int E = Pack<T>::N;
 #define LN_GO(G, R)                                                                                                      \
